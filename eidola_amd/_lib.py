@@ -103,12 +103,13 @@ class BatchInfo(C.Structure):
 
 EXPORTS = ("eid_kv_write", "eid_rope_kv_write", "eid_qkv_rope_kv_write", "eid_attn_decode",
            "eid_attn_decode_noalloc", "eid_attn_varlen", "eid_lse_merge", "eid_o_proj",
-           "eid_workspace_bytes", "eid_partition_size", "eid_last_error", "eid_version")
+           "eid_attn_tree", "eid_attn_tree_workspace_bytes", "eid_kv_score", "eid_kv_select",
+           "eid_kv_compact", "eid_workspace_bytes", "eid_partition_size", "eid_last_error", "eid_version")
 # only in the measurement build (include/eidola_attn_measure.h)
 MEASURE_EXPORTS = ("eid_debug_set_timeline", "eid_debug_set_kernel_events",
                    "eid_debug_set_store_every_partition")
 SCHED_EXPORTS = ("eid_sched_create", "eid_sched_destroy", "eid_sched_add_seq",
-                 "eid_sched_free_seq", "eid_sched_seq_len", "eid_sched_free_blocks",
+                 "eid_sched_free_seq", "eid_sched_truncate", "eid_sched_seq_len", "eid_sched_free_blocks",
                  "eid_sched_block_refs", "eid_sched_build_batch")
 
 _lib = None
@@ -168,6 +169,17 @@ def _bind(path, measure):
         fn = getattr(lib, name)
         fn.argtypes = [C.POINTER(AttnDesc), C.POINTER(AttnArgs), P]
         fn.restype = C.c_int32
+    lib.eid_attn_tree.argtypes = [C.POINTER(AttnDesc), C.POINTER(AttnArgs), P, C.c_int32, P]
+    lib.eid_attn_tree.restype = C.c_int32
+    lib.eid_attn_tree_workspace_bytes.argtypes = [C.POINTER(AttnDesc)]
+    lib.eid_attn_tree_workspace_bytes.restype = C.c_size_t
+    lib.eid_kv_score.argtypes = [C.POINTER(AttnDesc), P, P, P, P, P, P, P, P, P]
+    lib.eid_kv_score.restype = C.c_int32
+    lib.eid_kv_select.argtypes = [C.POINTER(AttnDesc), P, P, P, C.c_int32, C.c_int32, C.c_int32, P, P, P]
+    lib.eid_kv_select.restype = C.c_int32
+    lib.eid_kv_compact.argtypes = [C.POINTER(AttnDesc), C.c_int32, P, P, P, P, P, P, C.c_int64, C.c_int64,
+                                   C.c_int64, C.c_int32, P, P, P]
+    lib.eid_kv_compact.restype = C.c_int32
     lib.eid_workspace_bytes.argtypes = [C.POINTER(AttnDesc)]
     lib.eid_workspace_bytes.restype = C.c_size_t
     lib.eid_partition_size.argtypes = [C.POINTER(AttnDesc)]
@@ -192,6 +204,8 @@ def _bind(path, measure):
     lib.eid_sched_add_seq.restype = C.c_int32
     lib.eid_sched_free_seq.argtypes = [P, C.c_int64]
     lib.eid_sched_free_seq.restype = C.c_int32
+    lib.eid_sched_truncate.argtypes = [P, C.c_int64, C.c_int32, C.c_int32]
+    lib.eid_sched_truncate.restype = C.c_int32
     lib.eid_sched_seq_len.argtypes = [P, C.c_int64]
     lib.eid_sched_seq_len.restype = C.c_int32
     lib.eid_sched_free_blocks.argtypes = [P]

@@ -6,7 +6,7 @@
 #ifdef EID_MEASURE
 #include "../../include/eidola_attn_measure.h"
 #endif
-#include "eid_params.h"
+#include "eid_cache_params.h"
 #include <algorithm>
 #include <cmath>
 #include <cstdarg>
@@ -54,6 +54,13 @@ hipError_t launch_kv_write(const uint16_t *k_new, const uint16_t *v_new, uint8_t
                            uint8_t *v_cache, const int64_t *slot_mapping, const float *k_scale,
                            const float *v_scale, int Hkv, int64_t num_slots, int num_tokens,
                            bool fp8, hipStream_t st);
+int tree_tile_tokens(int max_q_len);
+hipError_t launch_tree(const TreeParams &p, bool fp8, hipStream_t st);
+hipError_t launch_tree_merge(const TreeParams &p, hipStream_t st);
+int score_few_rows();
+hipError_t launch_score(const ScoreParams &p, bool fp8, bool few, bool many, hipStream_t st);
+hipError_t launch_select(const SelectParams &p, hipStream_t st);
+hipError_t launch_compact(const CompactParams &p, int num_layers, hipStream_t st);
 }  // namespace eid
 
 static_assert(EID_STATIC_WORKSPACE_BYTES == eid::kStaticScratchBytes,
@@ -1130,6 +1137,251 @@ int32_t eid_o_proj(const void *attn_out, const void *weight, const void *bias,
       static_cast<uint16_t *>(out), num_tokens, out_features, in_features,
       static_cast<hipStream_t>(hip_stream));
   if (e != hipSuccess) return hip_fail(e, "o_proj launch");
+  return EID_OK;
+}
+
+}  // extern "C"
+
+// ---- trees of drafted tokens ---------------------------------------------------------------
+namespace {
+
+struct TreePlan {
+  int32_t ranges;  // workgroups per KV head
+  size_t o_bytes, ml_bytes;
+};
+
+TreePlan make_tree_plan(const eid_attn_desc *d) {
+  TreePlan pl;
+  const long long tile = eid::tree_tile_tokens(d->max_q_len);
+  // an upper bound of the launch's 64-key chunks, by what the descriptor says of the lengths
+  const long long tiles = std::min<long long>((d->max_q_len + tile - 1) / tile, d->num_q_tokens);
+  long long keys = d->sum_kv_len ? d->sum_kv_len : (long long)d->num_seqs * d->max_kv_len;
+  if (d->window > 0) {
+    const long long span = (long long)d->window + d->max_q_len + eid::kBlock;
+    keys = std::min(keys, span * d->num_seqs);
+  }
+  const long long chunks = tiles * (keys / eid::kChunk + d->num_seqs);
+  const long long fill = std::max(1, 2 * eid::device_cus() / d->num_kv_heads);
+  const long long most = (chunks + eid::kTreeMinChunks - 1) / eid::kTreeMinChunks;
+  pl.ranges = (int32_t)std::max(1LL, std::min(fill, most));
+  const size_t rows = (size_t)pl.ranges * d->num_kv_heads * 2 * tile * eid::kGroup;
+  pl.o_bytes = rows * eid::kHeadDim * sizeof(float);
+  pl.ml_bytes = rows * 2 * sizeof(float);
+  return pl;
+}
+
+int32_t check_tree_desc(const eid_attn_desc *d) {
+  if (int32_t rc = check_attn_desc(d)) return rc;
+  if (d->max_q_len > eid::kTreeMax)
+    return fail(EID_ERR_UNSUPPORTED, "max_q_len %d: a tree has at most %d tokens", d->max_q_len, eid::kTreeMax);
+  return EID_OK;
+}
+
+// What the operators over a cache's rows read of a descriptor.
+int32_t check_rows_desc(const eid_attn_desc *d) {
+  if (int32_t rc = check_geometry(d)) return rc;
+  if (d->num_seqs <= 0) return fail(EID_ERR_INVALID_ARG, "num_seqs must be positive");
+  if (d->num_seqs > 65535) return fail(EID_ERR_UNSUPPORTED, "num_seqs > 65535");
+  if (d->max_blocks_per_seq <= 0) return fail(EID_ERR_INVALID_ARG, "max_blocks_per_seq must be positive");
+  if (d->max_blocks_per_seq > 0x7fffffff / eid::kBlock)
+    return fail(EID_ERR_UNSUPPORTED, "max_blocks_per_seq %d too large", d->max_blocks_per_seq);
+  return EID_OK;
+}
+
+int32_t last_block_of(const eid_attn_desc *d) { return (int32_t)std::min<int64_t>(d->num_blocks - 1, 0x7fffffff); }
+
+}  // namespace
+
+extern "C" {
+
+size_t eid_attn_tree_workspace_bytes(const eid_attn_desc *desc) {
+  if (check_tree_desc(desc)) return 0;
+  const TreePlan pl = make_tree_plan(desc);
+  return pl.o_bytes + pl.ml_bytes;
+}
+
+int32_t eid_attn_tree(const eid_attn_desc *desc, const eid_attn_args *args, const int64_t *tree_mask,
+                      int32_t mask_words, void *hip_stream) {
+  g_err[0] = 0;
+  if (int32_t rc = check_tree_desc(desc)) return rc;
+  if (int32_t rc = check_attn_args(desc, args, true, true, false)) return rc;
+  if (args->k_new || args->v_new)
+    return fail(EID_ERR_INVALID_ARG, "k_new / v_new are taken by eid_attn_decode only");
+  if (!tree_mask) return fail(EID_ERR_INVALID_ARG, "tree_mask is NULL");
+  if (reinterpret_cast<uintptr_t>(tree_mask) & 7u) return fail(EID_ERR_INVALID_ARG, "tree_mask must be 8-byte aligned");
+  if (mask_words < (desc->max_q_len + 63) / 64 || mask_words > eid::kTreeWordsMax)
+    return fail(EID_ERR_INVALID_ARG, "mask_words %d: max_q_len %d needs %d to %d", mask_words, desc->max_q_len,
+                (desc->max_q_len + 63) / 64, eid::kTreeWordsMax);
+  if ((long long)desc->num_q_tokens * desc->num_kv_heads > 0x7fffffffLL)
+    return fail(EID_ERR_UNSUPPORTED, "num_q_tokens %d too large", desc->num_q_tokens);
+  const TreePlan pl = make_tree_plan(desc);
+  const size_t need = pl.o_bytes + pl.ml_bytes;
+  if (!args->workspace || args->workspace_bytes < need)
+    return fail(EID_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need,
+                args->workspace ? args->workspace_bytes : (size_t)0);
+  if ((reinterpret_cast<uintptr_t>(args->workspace) & 255u) != 0)
+    return fail(EID_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+  const bool fp8 = desc->kv_dtype == EID_KV_FP8_E4M3;
+  eid::TreeParams p;
+  std::memset(&p, 0, sizeof p);
+  p.q = static_cast<const uint16_t *>(args->q);
+  p.out = static_cast<uint16_t *>(args->out);
+  p.lse = args->lse;
+  p.k_cache = static_cast<const uint8_t *>(args->k_cache);
+  p.v_cache = static_cast<const uint8_t *>(args->v_cache);
+  p.block_table = args->block_table;
+  p.cu_seqlens_q = args->cu_seqlens_q;
+  p.seq_lens = args->seq_lens;
+  p.sinks = args->sinks;
+  p.k_scale = fp8 ? args->k_scale : nullptr;
+  p.v_scale = fp8 ? args->v_scale : nullptr;
+  p.mask = reinterpret_cast<const uint64_t *>(tree_mask);
+  p.ws_o = static_cast<float *>(args->workspace);
+  p.ws_ml = reinterpret_cast<float *>(static_cast<uint8_t *>(args->workspace) + pl.o_bytes);
+  p.num_seqs = desc->num_seqs;
+  p.num_q_heads = desc->num_q_heads;
+  p.num_kv_heads = desc->num_kv_heads;
+  p.max_blocks_per_seq = desc->max_blocks_per_seq;
+  p.last_block = last_block_of(desc);
+  p.num_q_tokens = desc->num_q_tokens;
+  p.mask_words = mask_words;
+  p.window = desc->window;
+  p.max_q_len = desc->max_q_len;
+  p.ranges = pl.ranges;
+  p.min_chunks = eid::kTreeMinChunks;
+  p.softmax_scale = desc->softmax_scale;
+  hipStream_t st = static_cast<hipStream_t>(hip_stream);
+  hipError_t e = eid::launch_tree(p, fp8, st);
+  if (e != hipSuccess) return hip_fail(e, "tree launch");
+  if (args->split_done_event) {
+    e = hipEventRecord(static_cast<hipEvent_t>(args->split_done_event), st);
+    if (e != hipSuccess) return hip_fail(e, "split_done_event record");
+  }
+  if (pl.ranges > 1) {  // (one range holds every row whole)
+    e = eid::launch_tree_merge(p, st);
+    if (e != hipSuccess) return hip_fail(e, "tree merge launch");
+  }
+  return EID_OK;
+}
+
+// ---- thinning a cache out ------------------------------------------------------------------
+int32_t eid_kv_score(const eid_attn_desc *desc, const void *q, const float *lse, const void *k_cache,
+                     const int32_t *block_table, const int32_t *cu_seqlens_q, const int32_t *seq_lens,
+                     const float *k_scale, float *scores, void *hip_stream) {
+  g_err[0] = 0;
+  if (int32_t rc = check_attn_desc(desc)) return rc;
+  if (!q || !lse || !k_cache || !block_table || !cu_seqlens_q || !seq_lens || !scores)
+    return fail(EID_ERR_INVALID_ARG, "q, lse, k_cache, block_table, cu_seqlens_q, seq_lens and scores must be non-NULL");
+  if (!aligned16(q) || !aligned16(lse) || !aligned16(k_cache) || !aligned16(scores))
+    return fail(EID_ERR_INVALID_ARG, "q, lse, k_cache and scores must be 16-byte aligned");
+  const bool fp8 = desc->kv_dtype == EID_KV_FP8_E4M3;
+  if (fp8 && !k_scale) return fail(EID_ERR_INVALID_ARG, "fp8 KV needs k_scale");
+  eid::ScoreParams p;
+  std::memset(&p, 0, sizeof p);
+  p.q = static_cast<const uint16_t *>(q);
+  p.lse = lse;
+  p.k_cache = static_cast<const uint8_t *>(k_cache);
+  p.block_table = block_table;
+  p.cu_seqlens_q = cu_seqlens_q;
+  p.seq_lens = seq_lens;
+  p.k_scale = k_scale;
+  p.scores = scores;
+  p.num_seqs = desc->num_seqs;
+  p.num_q_heads = desc->num_q_heads;
+  p.num_kv_heads = desc->num_kv_heads;
+  p.max_blocks_per_seq = desc->max_blocks_per_seq;
+  p.last_block = last_block_of(desc);
+  p.num_q_tokens = desc->num_q_tokens;
+  p.window = desc->window;
+  p.max_q_len = desc->max_q_len;
+  p.max_kv_len = desc->max_kv_len;
+  p.softmax_scale = desc->softmax_scale;
+  // Sequences are sorted into two classes by their rows on the device; when every sequence has
+  // max_q_len rows (num_q_tokens says so) only one of them is populated.
+  const bool uniform = (int64_t)desc->num_seqs * desc->max_q_len == desc->num_q_tokens;
+  const bool many = desc->max_q_len > eid::score_few_rows();
+  const hipError_t e = eid::launch_score(p, fp8, !many || !uniform, many, static_cast<hipStream_t>(hip_stream));
+  if (e != hipSuccess) return hip_fail(e, "kv_score launch");
+  return EID_OK;
+}
+
+int32_t eid_kv_select(const eid_attn_desc *desc, const float *scores, const int32_t *block_table,
+                      const int32_t *seq_lens, int32_t budget, int32_t keep_first, int32_t keep_last,
+                      int32_t *keep, int32_t *counts, void *hip_stream) {
+  g_err[0] = 0;
+  if (int32_t rc = check_rows_desc(desc)) return rc;
+  if (budget <= 0) return fail(EID_ERR_INVALID_ARG, "budget %d must be positive", budget);
+  if (keep_first < 0 || keep_last < 0 || (int64_t)keep_first + keep_last > budget)
+    return fail(EID_ERR_INVALID_ARG, "keep_first %d and keep_last %d must be >= 0 and fit the budget %d", keep_first,
+                keep_last, budget);
+  if (!scores || !block_table || !seq_lens || !keep || !counts)
+    return fail(EID_ERR_INVALID_ARG, "scores, block_table, seq_lens, keep and counts must be non-NULL");
+  if (!aligned16(scores)) return fail(EID_ERR_INVALID_ARG, "scores must be 16-byte aligned");
+  eid::SelectParams p;
+  std::memset(&p, 0, sizeof p);
+  p.scores = scores;
+  p.block_table = block_table;
+  p.seq_lens = seq_lens;
+  p.keep = keep;
+  p.counts = counts;
+  p.num_seqs = desc->num_seqs;
+  p.num_kv_heads = desc->num_kv_heads;
+  p.max_blocks_per_seq = desc->max_blocks_per_seq;
+  p.last_block = last_block_of(desc);
+  p.budget = budget;
+  p.keep_first = keep_first;
+  p.keep_last = keep_last;
+  const hipError_t e = eid::launch_select(p, static_cast<hipStream_t>(hip_stream));
+  if (e != hipSuccess) return hip_fail(e, "kv_select launch");
+  return EID_OK;
+}
+
+int32_t eid_kv_compact(const eid_attn_desc *desc, int32_t num_layers, const int64_t *k_caches, const int64_t *v_caches,
+                       const int64_t *scores, const int32_t *block_table, const int32_t *seq_lens, const int32_t *keep,
+                       int64_t keep_layer_stride, int64_t keep_seq_stride, int64_t keep_head_stride, int32_t max_rows,
+                       const int32_t *counts, const int32_t *starts, void *hip_stream) {
+  g_err[0] = 0;
+  if (int32_t rc = check_rows_desc(desc)) return rc;
+  if (num_layers < 0) return fail(EID_ERR_INVALID_ARG, "num_layers %d < 0", num_layers);
+  if (max_rows < 0) return fail(EID_ERR_INVALID_ARG, "max_rows %d < 0", max_rows);
+  if (keep_layer_stride < 0 || keep_seq_stride < 0 || keep_head_stride < 0)
+    return fail(EID_ERR_INVALID_ARG, "strides of keep must be >= 0");
+  if (num_layers == 0 || max_rows == 0) return EID_OK;
+  if (!k_caches || !v_caches || !block_table || !seq_lens || !keep || !counts)
+    return fail(EID_ERR_INVALID_ARG, "k_caches, v_caches, block_table, seq_lens, keep and counts must be non-NULL");
+  for (int32_t l = 0; l < num_layers; ++l) {
+    const int64_t all = k_caches[l] | v_caches[l] | (scores ? scores[l] : 0);
+    if (!k_caches[l] || !v_caches[l] || (scores && !scores[l]))
+      return fail(EID_ERR_INVALID_ARG, "layer %d: a cache or its scores are NULL", l);
+    if (all & 15) return fail(EID_ERR_INVALID_ARG, "layer %d: caches and scores must be 16-byte aligned", l);
+  }
+  eid::CompactParams p;
+  std::memset(&p, 0, sizeof p);
+  p.block_table = block_table;
+  p.seq_lens = seq_lens;
+  p.counts = counts;
+  p.starts = starts;
+  p.keep_layer = keep_layer_stride;
+  p.keep_seq = keep_seq_stride;
+  p.keep_head = keep_head_stride;
+  p.num_seqs = desc->num_seqs;
+  p.num_kv_heads = desc->num_kv_heads;
+  p.max_blocks_per_seq = desc->max_blocks_per_seq;
+  p.last_block = last_block_of(desc);
+  p.max_rows = max_rows;
+  p.elt = desc->kv_dtype == EID_KV_FP8_E4M3 ? 1 : 2;
+  p.has_scores = scores ? 1 : 0;
+  for (int32_t l0 = 0; l0 < num_layers; l0 += eid::kCompactLayers) {
+    const int32_t n = std::min(eid::kCompactLayers, num_layers - l0);
+    for (int32_t i = 0; i < n; ++i) {
+      p.k[i] = reinterpret_cast<uint8_t *>(static_cast<uintptr_t>(k_caches[l0 + i]));
+      p.v[i] = reinterpret_cast<uint8_t *>(static_cast<uintptr_t>(v_caches[l0 + i]));
+      p.scores[i] = scores ? reinterpret_cast<float *>(static_cast<uintptr_t>(scores[l0 + i])) : nullptr;
+    }
+    p.keep = keep + (size_t)l0 * keep_layer_stride;
+    const hipError_t e = eid::launch_compact(p, n, static_cast<hipStream_t>(hip_stream));
+    if (e != hipSuccess) return hip_fail(e, "kv_compact launch");
+  }
   return EID_OK;
 }
 

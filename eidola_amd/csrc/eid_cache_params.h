@@ -1,0 +1,63 @@
+// Launch descriptors of the tree attention and of the operators that thin a paged cache out
+// (internal to the library).
+#pragma once
+#include "eid_params.h"
+
+namespace eid {
+
+constexpr int kTreeWordsMax = 4;              // mask words per drafted token
+constexpr int kTreeMax = 64 * kTreeWordsMax;  // drafted tokens per sequence
+constexpr int kTreeWaves = 4;
+constexpr int kTreeMinChunks = 2;             // 64-key chunks per workgroup of a range, at least
+
+struct TreeParams {
+  const uint16_t *q;
+  uint16_t *out;
+  float *lse;  // may be null
+  const uint8_t *k_cache, *v_cache;
+  const int32_t *block_table, *cu_seqlens_q, *seq_lens;
+  const float *sinks;             // may be null
+  const float *k_scale, *v_scale; // fp8 only
+  const uint64_t *mask;           // [num_q_tokens][mask_words]
+  float *ws_o;   // [ranges][Hkv][2][tile rows][64]  sum of e^(s-m) v of a piece, not normalised
+  float *ws_ml;  // [ranges][Hkv][2][tile rows][2]   m (log2 units), l
+  int32_t num_seqs, num_q_heads, num_kv_heads, max_blocks_per_seq, last_block;
+  int32_t num_q_tokens, mask_words, window, max_q_len;
+  int32_t ranges;     // workgroups per KV head
+  int32_t min_chunks; // smallest range
+  float softmax_scale;
+};
+
+struct ScoreParams {
+  const uint16_t *q;
+  const float *lse;
+  const uint8_t *k_cache;
+  const int32_t *block_table, *cu_seqlens_q, *seq_lens;
+  const float *k_scale;  // fp8 only
+  float *scores;         // [num_blocks][Hkv][16]
+  int32_t num_seqs, num_q_heads, num_kv_heads, max_blocks_per_seq, last_block;
+  int32_t num_q_tokens, window, max_q_len, max_kv_len;
+  float softmax_scale;
+};
+
+struct SelectParams {
+  const float *scores;
+  const int32_t *block_table, *seq_lens;
+  int32_t *keep;    // [num_seqs][Hkv][budget]
+  int32_t *counts;  // [num_seqs]
+  int32_t num_seqs, num_kv_heads, max_blocks_per_seq, last_block;
+  int32_t budget, keep_first, keep_last;
+};
+
+constexpr int kCompactLayers = 64;  // layers per launch
+struct CompactParams {
+  uint8_t *k[kCompactLayers], *v[kCompactLayers];
+  float *scores[kCompactLayers];  // all null when none were given
+  const int32_t *block_table, *seq_lens, *keep, *counts, *starts;  // starts may be null
+  int64_t keep_layer, keep_seq, keep_head;  // strides of keep in entries; 0 = shared
+  int32_t num_seqs, num_kv_heads, max_blocks_per_seq, last_block;
+  int32_t max_rows, elt;  // elt: bytes per cache element
+  int32_t has_scores;
+};
+
+}  // namespace eid

@@ -97,14 +97,17 @@ struct eid_sched {
   int64_t allocate() {
     const int64_t b = free_head;
     free_unlink(b);
-    Block &B = blocks[b];
-    if (B.indexed) {
-      auto it = index.find(B.hash);
-      if (it != index.end() && it->second == b) index.erase(it);
-      B.indexed = false;
-    }
-    B.refs = 1;
+    forget(b);
+    blocks[b].refs = 1;
     return b;
+  }
+  // Takes a block out of the prefix index.
+  void forget(int64_t b) {
+    Block &B = blocks[b];
+    if (!B.indexed) return;
+    auto it = index.find(B.hash);
+    if (it != index.end() && it->second == b) index.erase(it);
+    B.indexed = false;
   }
   void release(int64_t b) {
     Block &B = blocks[b];
@@ -206,6 +209,51 @@ int32_t eid_sched_free_seq(eid_sched *s, int64_t seq_id) {
   // prefix chain is recycled before its head and the head stays matchable for longer
   for (size_t i = it->second.blocks.size(); i-- > 0;) s->release(it->second.blocks[i]);
   s->seqs.erase(it);
+  return EID_OK;
+}
+
+int32_t eid_sched_truncate(eid_sched *s, int64_t seq_id, int32_t new_len, int32_t unchanged) {
+  eid::clear_error();
+  if (!s) return fail(EID_ERR_INVALID_ARG, "scheduler is NULL");
+  auto it = s->seqs.find(seq_id);
+  if (it == s->seqs.end()) return fail(EID_ERR_INVALID_ARG, "sequence %lld unknown", (long long)seq_id);
+  Seq &q = it->second;
+  if (new_len < 0 || new_len > q.len)
+    return fail(EID_ERR_INVALID_ARG, "new_len %d is not in [0, %d]", new_len, q.len);
+  if (unchanged < 0 || unchanged > new_len)
+    return fail(EID_ERR_INVALID_ARG, "unchanged %d is not in [0, new_len %d]", unchanged, new_len);
+  const int bs = s->bs;
+  const size_t kept = (size_t)((new_len + bs - 1) / bs);
+  // the first block that is no longer what it was indexed as: rewritten, or open to appends again
+  // (when neither its end nor its rows changed, as in a call that cuts nothing, there is none)
+  const size_t touched = unchanged < new_len ? (size_t)(unchanged / bs)
+                         : new_len < q.len   ? (size_t)(new_len / bs)
+                                             : kept;
+  for (size_t b = touched; b < kept; ++b)
+    if (s->blocks[(size_t)q.blocks[b]].refs > 1)
+      return fail(EID_ERR_INVALID_ARG, "block %zu of sequence %lld is shared with another sequence", b,
+                  (long long)seq_id);
+  if (unchanged < new_len) {
+    q.chained = false;
+    q.tail.clear();
+  } else if (s->reuse && q.chained && new_len < q.len) {
+    // the chain up to the last whole block, and the tokens of the one that is open again
+    // (the blocks' hashes and tokens were kept when they filled up)
+    const int whole = new_len / bs, open = new_len % bs;
+    if (open > 0 && whole < q.len / bs) {  // that block was full
+      const int32_t *tok = &s->block_tokens[(size_t)q.blocks[(size_t)whole] * bs];
+      q.tail.assign(tok, tok + open);  // (capacity of bs entries was reserved: no allocation)
+    } else {
+      q.tail.resize((size_t)open);
+    }
+    q.chain = whole > 0 ? s->blocks[(size_t)q.blocks[(size_t)whole - 1]].hash : kRootHash;
+  }
+  for (size_t b = touched; b < kept; ++b) s->forget(q.blocks[b]);
+  while (q.blocks.size() > kept) {
+    s->release(q.blocks.back());
+    q.blocks.pop_back();
+  }
+  q.len = new_len;
   return EID_OK;
 }
 

@@ -491,6 +491,239 @@ def lse_merge(geom, workspace, seq_lens, cu_seqlens_q, *, num_q_tokens, max_q_le
     return out
 
 
+def _on(device):
+    """The device's current stream, with the device made current for the launch."""
+    return torch.cuda.device(device), C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def _same_device(first, **others):
+    for name, t in others.items():
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{name} is on {t.device}, not on {first.device}")
+
+
+def _scale(t, name, geom):
+    _require(t, name, torch.float32, 1)
+    if t.shape[0] != geom.num_kv_heads:
+        raise ValueError(f"{name} must be [num_kv_heads]")
+
+
+def _rows_desc(geom, block_table, num_blocks):
+    """Descriptor for the operators over cached rows."""
+    S = block_table.shape[0]
+    return make_desc(geom, num_seqs=S, num_q_tokens=max(S, 1), max_q_len=1, max_kv_len=1,
+                     max_blocks_per_seq=block_table.shape[1], num_blocks=num_blocks)
+
+
+def attn_tree_workspace_bytes(desc):
+    return load_library().eid_attn_tree_workspace_bytes(C.byref(desc))
+
+
+def attn_tree(geom, q, k_cache, v_cache, block_table, seq_lens, cu_seqlens_q, tree_mask, *, max_q_len,
+              max_kv_len, sinks=None, k_scale=None, v_scale=None, out=None, lse=None, workspace=None,
+              return_lse=False, sum_kv_len=0):
+    """Attention for trees of drafted tokens: row i of a sequence sees its context and the tokens
+    whose bits are set in tree_mask[i] ([T, words] int64, bit j % 64 of word j / 64 = token j of
+    the same sequence, at most 256 tokens).  The tokens' K/V rows stand in the cache behind the
+    context (seq_lens counts them).  geom.window is measured in depths.  `workspace`: a uint8
+    tensor of attn_tree_workspace_bytes, for callers that keep one (one call at a time)."""
+    _require(q, "q", torch.bfloat16, 3)
+    k_cache = _cache_view(k_cache, geom, "k_cache")
+    v_cache = _cache_view(v_cache, geom, "v_cache")
+    if k_cache.shape != v_cache.shape:
+        raise ValueError("k_cache and v_cache shapes differ")
+    _require(block_table, "block_table", torch.int32, 2)
+    _require(seq_lens, "seq_lens", torch.int32, 1)
+    _require(cu_seqlens_q, "cu_seqlens_q", torch.int32, 1)
+    _require(tree_mask, "tree_mask", torch.int64, 2)
+    S, T = seq_lens.shape[0], q.shape[0]
+    if tuple(q.shape[1:]) != (geom.num_q_heads, geom.head_dim):
+        raise ValueError("q must be [T, num_q_heads, head_dim]")
+    if block_table.shape[0] != S or cu_seqlens_q.shape[0] != S + 1:
+        raise ValueError("block_table must have one row per sequence, cu_seqlens_q one entry more")
+    if tree_mask.shape[0] != T:
+        raise ValueError("tree_mask must have one row per query token")
+    if sinks is not None:
+        _require(sinks, "sinks", torch.float32, 1)
+        if sinks.shape[0] != geom.num_q_heads:
+            raise ValueError("sinks must be [num_q_heads]")
+    if geom.kv_dtype == KV_FP8_E4M3:
+        _scale(k_scale, "k_scale", geom)
+        _scale(v_scale, "v_scale", geom)
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        _require(out, "out", torch.bfloat16, 3)
+        if out.shape != q.shape:
+            raise ValueError("out must have the shape of q")
+    if lse is None and return_lse:
+        lse = torch.empty((T, geom.num_q_heads), dtype=torch.float32, device=q.device)
+    elif lse is not None:
+        _require(lse, "lse", torch.float32, 2)
+        if tuple(lse.shape) != (T, geom.num_q_heads):
+            raise ValueError("lse must be [T, num_q_heads]")
+    _same_device(q, k_cache=k_cache, v_cache=v_cache, block_table=block_table, seq_lens=seq_lens,
+                 cu_seqlens_q=cu_seqlens_q, tree_mask=tree_mask, sinks=sinks, k_scale=k_scale, v_scale=v_scale,
+                 out=out, lse=lse, workspace=workspace)
+    desc = make_desc(geom, num_seqs=S, num_q_tokens=T, max_q_len=max_q_len, max_kv_len=max_kv_len,
+                     max_blocks_per_seq=block_table.shape[1], num_blocks=k_cache.shape[0], sum_kv_len=sum_kv_len)
+    lib = load_library()
+    on, stream = _on(q.device)
+    with on:
+        if workspace is None:
+            need = lib.eid_attn_tree_workspace_bytes(C.byref(desc))
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        args = AttnArgs()
+        args.q, args.out = q.data_ptr(), out.data_ptr()
+        args.lse = lse.data_ptr() if lse is not None else None
+        args.k_cache, args.v_cache = k_cache.data_ptr(), v_cache.data_ptr()
+        args.block_table, args.seq_lens = block_table.data_ptr(), seq_lens.data_ptr()
+        args.cu_seqlens_q = cu_seqlens_q.data_ptr()
+        args.sinks = sinks.data_ptr() if sinks is not None else None
+        args.k_scale = k_scale.data_ptr() if k_scale is not None else None
+        args.v_scale = v_scale.data_ptr() if v_scale is not None else None
+        if workspace is not None:
+            if not workspace.is_contiguous():
+                raise ValueError("workspace must be contiguous")
+            args.workspace = workspace.data_ptr()
+            args.workspace_bytes = workspace.numel() * workspace.element_size()
+        check(lib.eid_attn_tree(C.byref(desc), C.byref(args), tree_mask.data_ptr(), tree_mask.shape[1], stream))
+    return (out, lse) if return_lse else out
+
+
+def _scores_pool(t, name, geom, num_blocks):
+    _require(t, name, torch.float32, 3)
+    if tuple(t.shape) != (num_blocks, geom.num_kv_heads, geom.block_size):
+        raise ValueError(f"{name} must be [{num_blocks}, {geom.num_kv_heads}, {geom.block_size}], got {tuple(t.shape)}")
+
+
+def kv_score(geom, q, lse, k_cache, block_table, seq_lens, cu_seqlens_q, scores, *, max_q_len, max_kv_len,
+             k_scale=None, sum_kv_len=0):
+    """Adds the attention weight that every cached key receives from this step's rows to `scores`
+    ([num_blocks, num_kv_heads, 16] fp32, paged like the caches; the step's own keys start from 0).
+    `lse` is what the step's attention call returned.  Returns `scores`."""
+    _require(q, "q", torch.bfloat16, 3)
+    _require(lse, "lse", torch.float32, 2)
+    k_cache = _cache_view(k_cache, geom, "k_cache")
+    _require(block_table, "block_table", torch.int32, 2)
+    _require(seq_lens, "seq_lens", torch.int32, 1)
+    _require(cu_seqlens_q, "cu_seqlens_q", torch.int32, 1)
+    _scores_pool(scores, "scores", geom, k_cache.shape[0])
+    S, T = seq_lens.shape[0], q.shape[0]
+    if tuple(q.shape[1:]) != (geom.num_q_heads, geom.head_dim):
+        raise ValueError("q must be [T, num_q_heads, head_dim]")
+    if tuple(lse.shape) != (T, geom.num_q_heads):
+        raise ValueError("lse must be [T, num_q_heads]")
+    if block_table.shape[0] != S or cu_seqlens_q.shape[0] != S + 1:
+        raise ValueError("block_table must have one row per sequence, cu_seqlens_q one entry more")
+    if geom.kv_dtype == KV_FP8_E4M3:
+        _scale(k_scale, "k_scale", geom)
+    _same_device(q, lse=lse, k_cache=k_cache, block_table=block_table, seq_lens=seq_lens, cu_seqlens_q=cu_seqlens_q,
+                 scores=scores, k_scale=k_scale)
+    desc = make_desc(geom, num_seqs=S, num_q_tokens=T, max_q_len=max_q_len, max_kv_len=max_kv_len,
+                     max_blocks_per_seq=block_table.shape[1], num_blocks=k_cache.shape[0], sum_kv_len=sum_kv_len)
+    on, stream = _on(q.device)
+    with on:
+        check(load_library().eid_kv_score(
+            C.byref(desc), q.data_ptr(), lse.data_ptr(), k_cache.data_ptr(), block_table.data_ptr(),
+            cu_seqlens_q.data_ptr(), seq_lens.data_ptr(), k_scale.data_ptr() if k_scale is not None else None,
+            scores.data_ptr(), stream))
+    return scores
+
+
+def kv_select(geom, scores, block_table, seq_lens, *, budget, keep_first=0, keep_last=0, max_kv_len, keep=None,
+              counts=None):
+    """The rows of every sequence that stay when its cache is cut to `budget` rows, per KV head: the
+    first keep_first, the last keep_last and the highest scores between them (ties: the lower
+    row).  Returns (keep [S, num_kv_heads, budget] int32, ascending, -1 behind the count; counts
+    [S] int32)."""
+    _require(block_table, "block_table", torch.int32, 2)
+    _require(seq_lens, "seq_lens", torch.int32, 1)
+    _require(scores, "scores", torch.float32, 3)
+    _scores_pool(scores, "scores", geom, scores.shape[0])
+    S = seq_lens.shape[0]
+    if block_table.shape[0] != S:
+        raise ValueError("block_table must have one row per sequence")
+    if max_kv_len > block_table.shape[1] * geom.block_size:
+        raise ValueError(f"block_table cannot hold max_kv_len {max_kv_len}")
+    if budget <= 0:
+        raise ValueError("budget must be positive")
+    if keep is None:
+        keep = torch.empty((S, geom.num_kv_heads, budget), dtype=torch.int32, device=scores.device)
+    else:
+        _require(keep, "keep", torch.int32, 3)
+        if tuple(keep.shape) != (S, geom.num_kv_heads, budget):
+            raise ValueError("keep must be [S, num_kv_heads, budget]")
+    if counts is None:
+        counts = torch.empty((S,), dtype=torch.int32, device=scores.device)
+    else:
+        _require(counts, "counts", torch.int32, 1)
+        if counts.shape[0] != S:
+            raise ValueError("counts must be [S]")
+    _same_device(scores, block_table=block_table, seq_lens=seq_lens, keep=keep, counts=counts)
+    desc = _rows_desc(geom, block_table, scores.shape[0])
+    on, stream = _on(scores.device)
+    with on:
+        check(load_library().eid_kv_select(
+            C.byref(desc), scores.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), budget, keep_first,
+            keep_last, keep.data_ptr(), counts.data_ptr(), stream))
+    return keep, counts
+
+
+def kv_compact(geom, k_caches, v_caches, block_table, seq_lens, keep, counts, *, starts=None, scores=None):
+    """Moves row keep[..., i] of every sequence to row starts[s] + i (i < counts[s]), in place, in the
+    caches of all layers (lists of [num_blocks, 16, Hkv, D] tensors) and in their `scores`
+    (list, optional).  keep is int32 and ascending, keep[..., i] >= starts[s] + i: [S, N] (the same
+    rows in every layer and head), [S, Hkv, N] (in every layer) or [layers, S, Hkv, N]; seq_lens is
+    the length before the move.  The sequence's length afterwards is starts[s] + counts[s]."""
+    n_layers = len(k_caches)
+    if n_layers == 0 or len(v_caches) != n_layers or (scores is not None and len(scores) != n_layers):
+        raise ValueError("k_caches, v_caches (and scores) must be lists with one tensor per layer")
+    k_caches = [_cache_view(t, geom, f"k_caches[{i}]") for i, t in enumerate(k_caches)]
+    v_caches = [_cache_view(t, geom, f"v_caches[{i}]") for i, t in enumerate(v_caches)]
+    num_blocks = k_caches[0].shape[0]
+    pointers = [t.data_ptr() for t in k_caches] + [t.data_ptr() for t in v_caches]
+    if scores is not None:
+        for i, t in enumerate(scores):
+            _scores_pool(t, f"scores[{i}]", geom, num_blocks)
+        pointers += [t.data_ptr() for t in scores]
+    if len(set(pointers)) != len(pointers):
+        raise ValueError("a tensor is given twice")
+    _require(block_table, "block_table", torch.int32, 2)
+    _require(seq_lens, "seq_lens", torch.int32, 1)
+    _require(counts, "counts", torch.int32, 1)
+    S = seq_lens.shape[0]
+    if block_table.shape[0] != S or counts.shape[0] != S:
+        raise ValueError("block_table and counts must have one row per sequence")
+    if starts is not None:
+        _require(starts, "starts", torch.int32, 1)
+        if starts.shape[0] != S:
+            raise ValueError("starts must be [S]")
+    _require(keep, "keep", torch.int32)
+    N = keep.shape[-1] if keep.dim() else 0
+    shapes = {2: (S, N), 3: (S, geom.num_kv_heads, N), 4: (n_layers, S, geom.num_kv_heads, N)}
+    if tuple(keep.shape) != shapes.get(keep.dim()):
+        raise ValueError("keep must be [S, N], [S, num_kv_heads, N] or [layers, S, num_kv_heads, N]")
+    per_head = keep.dim() > 2
+    for name, group in (("k_caches", k_caches), ("v_caches", v_caches), ("scores", scores or [])):
+        for t in group:
+            if t.shape[0] != num_blocks:
+                raise ValueError(f"{name}: every layer must have {num_blocks} blocks")
+            _same_device(keep, **{name: t})
+    _same_device(keep, block_table=block_table, seq_lens=seq_lens, counts=counts, starts=starts)
+    desc = _rows_desc(geom, block_table, num_blocks)
+    at = (C.c_int64 * len(pointers))(*pointers)
+    off = C.sizeof(C.c_int64) * n_layers
+    base = C.addressof(at)
+    on, stream = _on(keep.device)
+    with on:
+        check(load_library().eid_kv_compact(
+            C.byref(desc), n_layers, base, base + off, base + 2 * off if scores is not None else None,
+            block_table.data_ptr(), seq_lens.data_ptr(), keep.data_ptr(),
+            S * geom.num_kv_heads * N if keep.dim() == 4 else 0, (geom.num_kv_heads if per_head else 1) * N,
+            N if per_head else 0, N, counts.data_ptr(), starts.data_ptr() if starts is not None else None, stream))
+
+
 def workspace_layout(desc):
     """(partition, nparts_max, ws_rows, ml_offset, acc_offset): after a 256-byte plan header
     (and, when a sequence can have more than one partition, one int32 per sequence: its number

@@ -57,6 +57,12 @@ class Scheduler:
     def free_seq(self, seq_id):
         check(self._lib.eid_sched_free_seq(self._h, seq_id))
 
+    def truncate(self, seq_id, new_len, unchanged=None):
+        """Cuts a sequence back to its first `new_len` rows and gives the blocks behind them back.
+        `unchanged` (default: new_len) leading rows hold what build_batch's tokens put there; the
+        rest was rewritten in place (kv_compact)."""
+        check(self._lib.eid_sched_truncate(self._h, seq_id, new_len, new_len if unchanged is None else unchanged))
+
     def seq_len(self, seq_id):
         return self._lib.eid_sched_seq_len(self._h, seq_id)
 

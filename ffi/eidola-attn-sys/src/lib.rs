@@ -179,6 +179,60 @@ unsafe extern "C" {
         hip_stream: *mut c_void,
     ) -> i32;
 
+    pub fn eid_attn_tree(
+        desc: *const eid_attn_desc,
+        args: *const eid_attn_args,
+        tree_mask: *const i64,
+        mask_words: i32,
+        hip_stream: *mut c_void,
+    ) -> i32;
+
+    pub fn eid_attn_tree_workspace_bytes(desc: *const eid_attn_desc) -> usize;
+
+    pub fn eid_kv_score(
+        desc: *const eid_attn_desc,
+        q: *const c_void,
+        lse: *const f32,
+        k_cache: *const c_void,
+        block_table: *const i32,
+        cu_seqlens_q: *const i32,
+        seq_lens: *const i32,
+        k_scale: *const f32,
+        scores: *mut f32,
+        hip_stream: *mut c_void,
+    ) -> i32;
+
+    pub fn eid_kv_select(
+        desc: *const eid_attn_desc,
+        scores: *const f32,
+        block_table: *const i32,
+        seq_lens: *const i32,
+        budget: i32,
+        keep_first: i32,
+        keep_last: i32,
+        keep: *mut i32,
+        counts: *mut i32,
+        hip_stream: *mut c_void,
+    ) -> i32;
+
+    pub fn eid_kv_compact(
+        desc: *const eid_attn_desc,
+        num_layers: i32,
+        k_caches: *const i64,
+        v_caches: *const i64,
+        scores: *const i64,
+        block_table: *const i32,
+        seq_lens: *const i32,
+        keep: *const i32,
+        keep_layer_stride: i64,
+        keep_seq_stride: i64,
+        keep_head_stride: i64,
+        max_rows: i32,
+        counts: *const i32,
+        starts: *const i32,
+        hip_stream: *mut c_void,
+    ) -> i32;
+
     pub fn eid_workspace_bytes(desc: *const eid_attn_desc) -> usize;
 
     pub fn eid_partition_size(desc: *const eid_attn_desc) -> i32;
@@ -200,6 +254,8 @@ unsafe extern "C" {
     ) -> i32;
 
     pub fn eid_sched_free_seq(s: *mut eid_sched, seq_id: i64) -> i32;
+
+    pub fn eid_sched_truncate(s: *mut eid_sched, seq_id: i64, new_len: i32, unchanged: i32) -> i32;
 
     pub fn eid_sched_seq_len(s: *const eid_sched, seq_id: i64) -> i32;
 

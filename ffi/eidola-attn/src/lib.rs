@@ -322,6 +322,138 @@ pub unsafe fn o_proj(
     })
 }
 
+/// Attention for trees of drafted tokens; `tree_mask` holds `mask_words` words per query token.
+///
+/// # Safety
+/// As `attn_varlen`, with a workspace of `tree_workspace_bytes` bytes and a device `tree_mask`.
+pub unsafe fn attn_tree(
+    desc: &sys::eid_attn_desc,
+    bufs: &AttnBuffers<'_>,
+    tree_mask: *const i64,
+    mask_words: i32,
+    stream: *mut c_void,
+) -> Result<(), AttnError> {
+    let args = bufs.raw();
+    check(unsafe { sys::eid_attn_tree(desc, &args, tree_mask, mask_words, stream) })
+}
+
+/// Bytes of workspace `attn_tree` needs (0 for an invalid descriptor).
+pub fn tree_workspace_bytes(desc: &sys::eid_attn_desc) -> usize {
+    // SAFETY: desc is a valid reference; planning touches no device memory.
+    unsafe { sys::eid_attn_tree_workspace_bytes(desc) }
+}
+
+/// Adds the attention weight every cached key receives from this step's rows to `scores`.
+///
+/// # Safety
+/// Device pointers of the extents `eid_kv_score` states.
+#[allow(clippy::too_many_arguments)]
+pub unsafe fn kv_score(
+    desc: &sys::eid_attn_desc,
+    q: *const c_void,
+    lse: *const f32,
+    k_cache: *const c_void,
+    block_table: *const i32,
+    cu_seqlens_q: *const i32,
+    seq_lens: *const i32,
+    k_scale: Option<*const f32>,
+    scores: *mut f32,
+    stream: *mut c_void,
+) -> Result<(), AttnError> {
+    check(unsafe {
+        sys::eid_kv_score(
+            desc,
+            q,
+            lse,
+            k_cache,
+            block_table,
+            cu_seqlens_q,
+            seq_lens,
+            k_scale.unwrap_or(ptr::null()),
+            scores,
+            stream,
+        )
+    })
+}
+
+/// The rows that stay when caches are cut to `budget` rows per KV head.
+///
+/// # Safety
+/// Device pointers of the extents `eid_kv_select` states.
+#[allow(clippy::too_many_arguments)]
+pub unsafe fn kv_select(
+    desc: &sys::eid_attn_desc,
+    scores: *const f32,
+    block_table: *const i32,
+    seq_lens: *const i32,
+    budget: i32,
+    keep_first: i32,
+    keep_last: i32,
+    keep: *mut i32,
+    counts: *mut i32,
+    stream: *mut c_void,
+) -> Result<(), AttnError> {
+    check(unsafe {
+        sys::eid_kv_select(
+            desc, scores, block_table, seq_lens, budget, keep_first, keep_last, keep, counts, stream,
+        )
+    })
+}
+
+/// The list of rows `kv_compact` moves: a device array and its strides in entries (0 = shared).
+#[derive(Clone, Copy, Debug)]
+pub struct Keep {
+    pub rows: *const i32,
+    pub layer_stride: i64,
+    pub seq_stride: i64,
+    pub head_stride: i64,
+    pub max_rows: i32,
+}
+
+/// Moves kept rows together in the caches (and scores) of all layers; the slices hold device
+/// addresses.
+///
+/// # Safety
+/// Device pointers of the extents `eid_kv_compact` states; `keep` ascending.
+#[allow(clippy::too_many_arguments)]
+pub unsafe fn kv_compact(
+    desc: &sys::eid_attn_desc,
+    k_caches: &[i64],
+    v_caches: &[i64],
+    scores: Option<&[i64]>,
+    block_table: *const i32,
+    seq_lens: *const i32,
+    keep: &Keep,
+    counts: *const i32,
+    starts: Option<*const i32>,
+    stream: *mut c_void,
+) -> Result<(), AttnError> {
+    if k_caches.len() != v_caches.len() || scores.is_some_and(|s| s.len() != k_caches.len()) {
+        return Err(AttnError::InvalidArg {
+            message: "k_caches, v_caches and scores must be of equal length".into(),
+        });
+    }
+    check(unsafe {
+        sys::eid_kv_compact(
+            desc,
+            k_caches.len() as i32,
+            k_caches.as_ptr(),
+            v_caches.as_ptr(),
+            scores.map_or(ptr::null(), |s| s.as_ptr()),
+            block_table,
+            seq_lens,
+            keep.rows,
+            keep.layer_stride,
+            keep.seq_stride,
+            keep.head_stride,
+            keep.max_rows,
+            counts,
+            starts.unwrap_or(ptr::null()),
+            stream,
+        )
+    })
+}
+
 /// Arrays and scalars of one step, as `Scheduler::build_batch` fills them (host memory).
 #[derive(Clone, Debug, Default)]
 pub struct Batch {
@@ -378,6 +510,12 @@ impl Scheduler {
     pub fn free_seq(&mut self, seq_id: i64) -> Result<(), AttnError> {
         // SAFETY: live handle.
         check(unsafe { sys::eid_sched_free_seq(self.handle, seq_id) })
+    }
+
+    /// Cuts a sequence back to its first `new_len` rows, `unchanged` of which hold what they held.
+    pub fn truncate(&mut self, seq_id: i64, new_len: i32, unchanged: i32) -> Result<(), AttnError> {
+        // SAFETY: live handle.
+        check(unsafe { sys::eid_sched_truncate(self.handle, seq_id, new_len, unchanged) })
     }
 
     /// Tokens in the cache for `seq_id`, `None` if the sequence is unknown.

@@ -306,6 +306,98 @@ int32_t eid_qkv_rope_kv_write(const eid_attn_desc *desc, const void *hidden, con
                               void *v_cache, const int64_t *slot_mapping, int32_t num_tokens,
                               const float *k_scale, const float *v_scale, void *hip_stream);
 
+/*
+ * Attention for trees of drafted tokens (speculative verification of several continuations at
+ * once).  The q_len rows of sequence s are the tokens of one tree; their K/V rows stand in the
+ * cache behind the context, token i at row prefix + i with prefix = seq_lens[s] - q_len.  Row i
+ * sees every context row (0 .. prefix-1) and those tokens j whose bit is set in its mask (its
+ * ancestors and itself; nothing is assumed of the bits, a row may see any set, or none):
+ *   tree_mask   [num_q_tokens, mask_words] int64, bit j % 64 of word j / 64 of row i = "row i sees
+ *               token j of its own sequence"; bits at or beyond the sequence's q_len are ignored
+ * max_q_len <= 256, (max_q_len + 63) / 64 <= mask_words <= 4.
+ * desc->window: the position of a token is prefix + (bits set in its mask) - 1 (its depth), that
+ * of a context row its index; row i sees what lies less than `window` positions behind its own.
+ * Token ids, positions for the rotary embedding (prefix + depth) and slots are the caller's, as
+ * for every append (eid_rope_kv_write takes any positions).  A row that sees nothing yields 0
+ * (lse = the sink, or -inf without one).  A row's answer does not depend on rows it does not see,
+ * whatever they hold (inf and NaN included).
+ * args as for eid_attn_varlen, with a workspace of eid_attn_tree_workspace_bytes(desc) bytes; the
+ * host copies of the lengths, k_new / v_new (must be NULL) and desc->partition_size play no part.
+ * split_done_event is recorded behind the first of the two launches.  `out` rows of no sequence
+ * (behind cu_seqlens_q[num_seqs]) are left as they were.
+ * Partial results are kept in fp32; the softmax weights enter the value product as bf16.
+ * Reference counterpart: none.  Engine call site: per layer of a verification step, in place of
+ * eid_attn_varlen.
+ */
+int32_t eid_attn_tree(const eid_attn_desc *desc, const eid_attn_args *args,
+                      const int64_t *tree_mask, int32_t mask_words, void *hip_stream);
+
+/* Bytes of workspace eid_attn_tree needs for desc.  Returns 0 for an invalid desc. */
+size_t eid_attn_tree_workspace_bytes(const eid_attn_desc *desc);
+
+/*
+ * Attention weight received per cached key, added up over the steps of a sequence:
+ *   scores[page, h, slot of key j] = (key j is new ? 0 : the same) +
+ *       sum over the sequence's rows i that see j and the 8 query heads of KV head h of
+ *       exp(softmax_scale * q_i . k_j - lse_i)
+ * New keys are the last q_len of the sequence: a page needs no clearing when it changes owner, as
+ * long as this is called for every step that appends.  Rows see what eid_attn_decode /
+ * eid_attn_varlen lets them see (causal, desc->window).
+ *   q        [num_q_tokens, num_q_heads, 64] bf16, the step's queries (after rotary embedding)
+ *   lse      [num_q_tokens, num_q_heads] fp32, as the step's attention call returned it (-inf:
+ *            the row saw nothing and adds nothing)
+ *   scores   [num_blocks, num_kv_heads, 16] fp32, paged like the caches
+ * fp32 sums in one order, no atomics: the same call gives the same bits.
+ * Sequences of the batch must not share pages that they score.  q, lse, k_cache and scores
+ * 16-byte aligned.  Reference counterpart: none.  Engine call site: per layer per step, behind
+ * attention, for layers whose cache is cut to a budget.
+ */
+int32_t eid_kv_score(const eid_attn_desc *desc, const void *q, const float *lse,
+                     const void *k_cache, const int32_t *block_table,
+                     const int32_t *cu_seqlens_q, const int32_t *seq_lens, const float *k_scale,
+                     float *scores, void *hip_stream);
+
+/*
+ * Which rows of a sequence stay when its cache is cut to `budget` rows, per KV head: the first
+ * keep_first rows, the last keep_last, and of those between them the ones with the highest
+ * scores.  Equal scores: the lower row stays; NaN ranks below every number, -0 equals +0.
+ *   scores   as eid_kv_score leaves them
+ *   keep     [num_seqs, num_kv_heads, budget] int32, rows in ascending order; -1 behind counts[s]
+ *   counts   [num_seqs] int32 = min(seq_lens[s], budget): sequences within the budget keep all
+ * keep_first + keep_last <= budget.  Of desc only the geometry, num_seqs, max_blocks_per_seq and
+ * num_blocks are read.  Reference counterpart: none.
+ */
+int32_t eid_kv_select(const eid_attn_desc *desc, const float *scores, const int32_t *block_table,
+                      const int32_t *seq_lens, int32_t budget, int32_t keep_first,
+                      int32_t keep_last, int32_t *keep, int32_t *counts, void *hip_stream);
+
+/*
+ * Moves kept rows of sequences together, in place, in the caches of all layers at once:
+ *   row starts[s] + i of sequence s <- its row keep[s, h, i]      for i < counts[s], per KV head h
+ * as if every row were read before any is written.  Serves the accepted path of a drafted tree
+ * (the same rows in every layer and head, behind the context) and a cache cut to a budget (other
+ * rows per head, from row 0 on).
+ *   k_caches, v_caches, scores   HOST arrays [num_layers] of device addresses; scores (as of
+ *            eid_kv_score, moved along) may be NULL.  Read before the call returns.
+ *   keep     entry (layer, s, h, i) at layer * keep_layer_stride + s * keep_seq_stride +
+ *            h * keep_head_stride + i; a stride of 0 shares the list between layers / heads.
+ *            Ascending over i, with keep >= starts[s] + i.
+ *   counts   [num_seqs] int32, at most max_rows entries are used; starts [num_seqs] int32 or NULL
+ *            (all 0)
+ * An entry below starts[s] + i, negative, or at or beyond seq_lens[s] (the length before the move)
+ * moves nothing.  Entries out of order leave unspecified rows, within the sequence's own pages.
+ * The pages written must belong to one sequence of the call alone (no prefix shared with others).
+ * Of desc only the geometry, num_seqs, max_blocks_per_seq and num_blocks are read.  One launch per
+ * 64 layers.  The sequence's new length, starts[s] + counts[s], is the caller's to keep
+ * (eid_sched_truncate).  Reference counterpart: none.
+ */
+int32_t eid_kv_compact(const eid_attn_desc *desc, int32_t num_layers, const int64_t *k_caches,
+                       const int64_t *v_caches, const int64_t *scores,
+                       const int32_t *block_table, const int32_t *seq_lens, const int32_t *keep,
+                       int64_t keep_layer_stride, int64_t keep_seq_stride,
+                       int64_t keep_head_stride, int32_t max_rows, const int32_t *counts,
+                       const int32_t *starts, void *hip_stream);
+
 /* Bytes of workspace eid_attn_decode / eid_attn_varlen / eid_lse_merge need for desc.
  * Returns 0 for an invalid desc. */
 size_t eid_workspace_bytes(const eid_attn_desc *desc);

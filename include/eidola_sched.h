@@ -100,6 +100,18 @@ int32_t eid_sched_build_batch(eid_sched *s, const int64_t *seq_ids, const int32_
                               int32_t *cu_seqlens_q, int32_t *seq_lens, int32_t *positions,
                               eid_batch_info *info);
 
+/*
+ * Cuts a sequence back to its first new_len rows: rejected drafted tokens, or a cache that
+ * eid_kv_compact has cut to a budget.  Blocks behind the new end are released.  `unchanged`
+ * (<= new_len) is the number of leading rows that hold what build_batch's tokens put there; rows
+ * from there to new_len were rewritten in place.  Blocks that hold such rows, and a last block
+ * that is now partly filled (it will be appended to), leave the prefix index, and must not be
+ * shared with another sequence (EID_ERR_INVALID_ARG, nothing changes).  With unchanged < new_len
+ * the sequence's later blocks are no longer indexed: they would not match their tokens.
+ * A step whose new tokens are a tree is built without new_tokens, for the same reason.
+ */
+int32_t eid_sched_truncate(eid_sched *s, int64_t seq_id, int32_t new_len, int32_t unchanged);
+
 #ifdef __cplusplus
 }
 #endif
