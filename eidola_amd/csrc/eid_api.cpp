@@ -1147,7 +1147,8 @@ namespace {
 
 struct TreePlan {
   int32_t ranges;  // workgroups per KV head
-  size_t o_bytes, ml_bytes;
+  size_t rec_bytes, o_bytes, ml_bytes;
+  size_t total() const { return rec_bytes + o_bytes + ml_bytes; }
 };
 
 TreePlan make_tree_plan(const eid_attn_desc *d) {
@@ -1165,6 +1166,7 @@ TreePlan make_tree_plan(const eid_attn_desc *d) {
   const long long most = (chunks + eid::kTreeMinChunks - 1) / eid::kTreeMinChunks;
   pl.ranges = (int32_t)std::max(1LL, std::min(fill, most));
   const size_t rows = (size_t)pl.ranges * d->num_kv_heads * 2 * tile * eid::kGroup;
+  pl.rec_bytes = ((size_t)pl.ranges * sizeof(eid::TreeRecord) + 255) / 256 * 256;
   pl.o_bytes = rows * eid::kHeadDim * sizeof(float);
   pl.ml_bytes = rows * 2 * sizeof(float);
   return pl;
@@ -1196,8 +1198,7 @@ extern "C" {
 
 size_t eid_attn_tree_workspace_bytes(const eid_attn_desc *desc) {
   if (check_tree_desc(desc)) return 0;
-  const TreePlan pl = make_tree_plan(desc);
-  return pl.o_bytes + pl.ml_bytes;
+  return make_tree_plan(desc).total();
 }
 
 int32_t eid_attn_tree(const eid_attn_desc *desc, const eid_attn_args *args, const int64_t *tree_mask,
@@ -1215,7 +1216,7 @@ int32_t eid_attn_tree(const eid_attn_desc *desc, const eid_attn_args *args, cons
   if ((long long)desc->num_q_tokens * desc->num_kv_heads > 0x7fffffffLL)
     return fail(EID_ERR_UNSUPPORTED, "num_q_tokens %d too large", desc->num_q_tokens);
   const TreePlan pl = make_tree_plan(desc);
-  const size_t need = pl.o_bytes + pl.ml_bytes;
+  const size_t need = pl.total();
   if (!args->workspace || args->workspace_bytes < need)
     return fail(EID_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need,
                 args->workspace ? args->workspace_bytes : (size_t)0);
@@ -1236,8 +1237,10 @@ int32_t eid_attn_tree(const eid_attn_desc *desc, const eid_attn_args *args, cons
   p.k_scale = fp8 ? args->k_scale : nullptr;
   p.v_scale = fp8 ? args->v_scale : nullptr;
   p.mask = reinterpret_cast<const uint64_t *>(tree_mask);
-  p.ws_o = static_cast<float *>(args->workspace);
-  p.ws_ml = reinterpret_cast<float *>(static_cast<uint8_t *>(args->workspace) + pl.o_bytes);
+  uint8_t *ws = static_cast<uint8_t *>(args->workspace);
+  p.ws_rec = reinterpret_cast<eid::TreeRecord *>(ws);
+  p.ws_o = reinterpret_cast<float *>(ws + pl.rec_bytes);
+  p.ws_ml = reinterpret_cast<float *>(ws + pl.rec_bytes + pl.o_bytes);
   p.num_seqs = desc->num_seqs;
   p.num_q_heads = desc->num_q_heads;
   p.num_kv_heads = desc->num_kv_heads;

@@ -10,6 +10,13 @@ constexpr int kTreeMax = 64 * kTreeWordsMax;  // drafted tokens per sequence
 constexpr int kTreeWaves = 4;
 constexpr int kTreeMinChunks = 2;             // 64-key chunks per workgroup of a range, at least
 
+// Tile of drafted tokens that begins in a range and ends in a later one (ntok == 0: none).
+struct TreeRecord {
+  int32_t row, ntok;  // first row of q / out, number of tokens
+  int32_t pieces;     // ranges that hold some of it
+  int32_t unused;
+};
+
 struct TreeParams {
   const uint16_t *q;
   uint16_t *out;
@@ -19,6 +26,7 @@ struct TreeParams {
   const float *sinks;             // may be null
   const float *k_scale, *v_scale; // fp8 only
   const uint64_t *mask;           // [num_q_tokens][mask_words]
+  TreeRecord *ws_rec;  // [ranges]
   float *ws_o;   // [ranges][Hkv][2][tile rows][64]  sum of e^(s-m) v of a piece, not normalised
   float *ws_ml;  // [ranges][Hkv][2][tile rows][2]   m (log2 units), l
   int32_t num_seqs, num_q_heads, num_kv_heads, max_blocks_per_seq, last_block;

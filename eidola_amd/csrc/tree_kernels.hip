@@ -2,6 +2,8 @@
 #include "eid_cache_params.h"
 #include "eid_device.h"
 
+#include <utility>
+
 namespace eid {
 
 namespace {
@@ -10,9 +12,6 @@ typedef const __attribute__((address_space(4))) int32_t *const_i32_ptr;
 __device__ __forceinline__ const_i32_ptr as_constant(const int32_t *p) { return (const_i32_ptr)(uintptr_t)p; }
 __device__ __forceinline__ int clamp_id(const int id, const int last) { return min(max(id, 0), last); }
 
-// LDS row strides of the K and V tiles (see the prefill kernel: K is read 16 bytes per lane by 16
-// lanes of one row each, V^T through the transposing read)
-constexpr int kKRow = 144, kVRow = 160;
 constexpr float kLazyLog2 = 8.0f;  // a row's reference moves when a score outgrows it by this
 
 // What one sequence gives the kernels: `chunks` 64-key chunks from key `begin` on for each of
@@ -119,22 +118,55 @@ __device__ __forceinline__ uint64_t chunk_bits(const uint64_t *mask, const int l
 // out[i] = sum_j vis(i, j) e^(c q_i.k_j) v_j / (sum_j vis(i, j) e^(c q_i.k_j) + e^sink), with
 // vis(i, j) = j < prefix, or bit j - prefix of row i's mask; one pass with a running reference.
 //
-// A workgroup of four waves owns tile_tok = 8 NT drafted tokens x the 8 query heads of one KV
-// head: 16 NT rows per wave.  The launch's (sequence, tile) pairs, 64 keys at a time, are laid
-// out in a line and cut into `ranges` equal pieces, one per workgroup, so that a batch of unequal
-// contexts loads every CU alike; a range that ends inside a sequence leaves (o, m, l) for
-// tree_merge_kernel.  K and V chunks go through LDS, double buffered, and are read by all waves.
+// A workgroup of four waves owns up to 8 NT drafted tokens x the 8 query heads of one KV head:
+// 16 NT rows per wave.  The launch's (sequence, tile) pairs,
+// 64 keys at a time, are laid out in a line and cut into `ranges` equal pieces, one per workgroup,
+// so that a batch of unequal contexts loads every CU alike; a range that ends inside a sequence
+// leaves (o, m, l) for tree_merge_kernel.
+//
+// K and V chunks stand in LDS as 64 rows of 128 bytes, read by all four waves; 16-byte segments
+// are permuted by the row (K: segment ^ (row / 2) % 8, V: pairs of segments by (row / 2) % 4),
+// which keeps the operand reads off each other's banks without padding.  bf16 caches: direct
+// global -> LDS loads, three stages, two chunks under way while one is computed.  fp8 caches:
+// through registers, where the bytes are widened once for the four waves, two stages.
+//
+// Chunks that some row does not see whole (the drafted tokens' own, a window's edge) differ in
+// two ways: scores are masked, and values that are not finite are taken out of the operands
+// (0 x inf would be NaN in rows that do not see the key); if there were any, their terms are added
+// afterwards, row by row, where they are seen.
 // ---------------------------------------------------------------------------------------
+typedef __attribute__((address_space(1))) const void gptr_t;
+typedef __attribute__((address_space(3))) void lptr_t;
+constexpr int kTileBytes = kChunk * 128;
+
+template <int... Is, typename F>
+__device__ __forceinline__ void static_for_impl(std::integer_sequence<int, Is...>, F &&f) {
+  (f(std::integral_constant<int, Is>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void static_for(F &&f) {
+  static_for_impl(std::make_integer_sequence<int, N>{}, f);
+}
+template <int I>
+using IC = std::integral_constant<int, I>;
+#define EID_SB() __builtin_amdgcn_sched_barrier(0)
+
 template <int NT, bool FP8>
-__global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_kernel(const TreeParams p) {
+__global__ __launch_bounds__(kTreeWaves * 64, NT == 1 ? 3 : 2) void tree_kernel(const TreeParams p) {
   constexpr int kTok = 2 * NT * kTreeWaves;  // tokens of a tile
   constexpr int kRows = kTok * kGroup;
   constexpr int kElt = FP8 ? 1 : 2;
-  __shared__ __align__(16) uint8_t lds_k[2][kChunk * kKRow];
-  __shared__ __align__(16) uint8_t lds_v[2][kChunk * kVRow];
+  // Q operands of three and four tiles do not fit the registers beside the rest: LDS, in place of
+  // the third stage.
+  constexpr bool QLDS = NT >= 3;
+  constexpr int ST = FP8 || QLDS ? 2 : 3;  // K/V stages
+  constexpr bool DEEP8 = NT <= 3;          // fp8: two chunks under way
+  // (separate arrays: the compiler can then tell the stage being filled from the one being read)
+  __shared__ __align__(1024) uint8_t k_st0[kTileBytes], k_st1[kTileBytes], k_st2[ST == 3 ? kTileBytes : 16];
+  __shared__ __align__(1024) uint8_t v_st0[kTileBytes], v_st1[kTileBytes], v_st2[ST == 3 ? kTileBytes : 16];
+  __shared__ __align__(16) uint8_t lds_q[QLDS ? kTreeWaves * 2 * NT * 1024 : 16];
   __shared__ uint64_t lds_mask[kTok][kTreeWordsMax];
   __shared__ int lds_lo[kTok];
-  __shared__ uint32_t lds_bad[3][2];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i16 = lane & 15, g = lane >> 4;
@@ -148,18 +180,21 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_kernel(const TreePara
   const long long per = range_units(p, total);
   long long u = per * range;
   const long long u_end = min(total, u + per);
-  if (u >= u_end) return;
-  long long before;
-  int s = find_seq(p, kTok, u, before);
+  TreeRecord rec = {0, 0, 0, 0};  // what the merge has to join from this range on
+  long long before = 0;
+  int s = u < u_end ? find_seq(p, kTok, u, before) : 0;
 
   const uint32_t row_bytes = (uint32_t)Hkv * kHeadDim * kElt;
   const size_t page_bytes = (size_t)kBlock * row_bytes;
-  const int ld_row = tid >> 2, ld_seg = tid & 3;  // loader: row of the chunk, 16-element segment
-  const uint32_t gl_off = (uint32_t)(ld_row & 15) * row_bytes + (uint32_t)kvh * (kHeadDim * kElt) +
-                          (uint32_t)ld_seg * (16 * kElt);
+  // operand reads (see above): K row i16 of a page, V rows 4 g + i16 / 4 (transposing read)
+  const int sw_k = (i16 >> 1) & 7;
+  const uint32_t k_off = (uint32_t)i16 * 128 + (uint32_t)((2 * g) ^ sw_k) * 16;
+  const int v_row = 4 * g + (i16 >> 2);
+  const uint32_t v_off = (uint32_t)v_row * 128 + 8 * (i16 & 3);
+  const int v_sw = 32 * ((v_row >> 1) & 3);
 
   while (u < u_end) {
-    TreeSeq v = tree_seq(p, s, kTok);
+    const TreeSeq v = tree_seq(p, s, kTok);
     if (u - before >= units_of(v)) {  // next sequence (those without rows have no units)
       before += units_of(v);
       ++s;
@@ -169,14 +204,86 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_kernel(const TreePara
     const int c0 = (int)((u - before) - (long long)tile * v.chunks);
     const int n = (int)min((long long)(v.chunks - c0), u_end - u);
     const int prefix = v.len - v.qlen;
-    const int tok0 = tile * kTok;  // first token of the tile, in the sequence
+    const int tok0 = tile * kTok;                   // first token of the tile, in the sequence
+    const int ntok = min(kTok, v.qlen - tok0);
+    const int wtok = wave * 2 * NT;                 // the wave's first token in the tile
+    const bool wave_active = wtok < ntok;
     const int t_begin = v.begin + c0 * kChunk;
     const int t_end = min(v.len, t_begin + n * kChunk);
     const const_i32_ptr bt = as_constant(p.block_table + (size_t)s * p.max_blocks_per_seq);
     const int last_page = (v.len + kBlock - 1) / kBlock - 1;
+    auto page_at = [&](const int tc) { return clamp_id(bt[min(tc / kBlock + wave, last_page)], p.last_block); };
+    auto masked = [&](const int tc) {
+      return tc + kChunk > prefix || (p.window > 0 && tc < prefix + v.qlen - p.window);
+    };
 
-    // ---- the tile's masks: bits of tokens of this sequence, those outside the window taken out
+    // ---- loaders: wave w brings page w of a chunk.  Rows past the end of the sequence repeat its
+    // last row: nobody sees them, and the memory behind may never have been written.
+    auto dma = [&](uint8_t *kbuf, uint8_t *vbuf, const int tc, const int page) {
+      const int dr = lane >> 3, sl = lane & 7;
+      const uint8_t *kp = p.k_cache + (size_t)page * page_bytes + (uint32_t)kvh * 128;
+      const uint8_t *vp = p.v_cache + (size_t)page * page_bytes + (uint32_t)kvh * 128;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int tok = min(tc + 16 * wave + 8 * h + dr, v.len - 1);
+        const uint32_t off = (uint32_t)(tok & 15) * row_bytes;
+        const int kseg = sl ^ (4 * h + (dr >> 1)), vseg = sl ^ ((dr >> 1) << 1);
+        __builtin_amdgcn_global_load_lds((gptr_t *)(kp + off + kseg * 16), (lptr_t *)(kbuf + (2 * wave + h) * 1024), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((gptr_t *)(vp + off + vseg * 16), (lptr_t *)(vbuf + (2 * wave + h) * 1024), 16, 0, 0);
+      }
+    };
+    const int fr = lane >> 2, fs = lane & 3;  // fp8: row of the page, 16-element segment
+    auto fetch8 = [&](const int tc, const int page, u32x4 &kr, u32x4 &vr) {
+      const int tok = min(tc + 16 * wave + fr, v.len - 1);
+      const size_t off = (size_t)page * page_bytes + (uint32_t)(tok & 15) * row_bytes + (uint32_t)kvh * 64 + fs * 16;
+      kr = *(const u32x4 *)(p.k_cache + off);
+      vr = *(const u32x4 *)(p.v_cache + off);
+    };
+    auto stash8 = [&](uint8_t *kbuf, uint8_t *vbuf, const u32x4 kr, const u32x4 vr) {
+      const int row = 16 * wave + fr, ks = (row >> 1) & 7, vsw = ((row >> 1) & 3) << 1;
+      Frag8 x;
+      fp8x8_to_bf16x8(kr[0], kr[1], x.w);
+      *(u32x4 *)(kbuf + row * 128 + ((2 * fs) ^ ks) * 16) = x.u;
+      fp8x8_to_bf16x8(kr[2], kr[3], x.w);
+      *(u32x4 *)(kbuf + row * 128 + ((2 * fs + 1) ^ ks) * 16) = x.u;
+      fp8x8_to_bf16x8(vr[0], vr[1], x.w);
+      *(u32x4 *)(vbuf + row * 128 + ((2 * fs) ^ vsw) * 16) = x.u;
+      fp8x8_to_bf16x8(vr[2], vr[3], x.w);
+      *(u32x4 *)(vbuf + row * 128 + ((2 * fs + 1) ^ vsw) * 16) = x.u;
+    };
+
     __syncthreads();  // (the last piece's readers are done)
+    // the first two chunks are requested before anything else of the piece is looked at
+    u32x4 ka, va, kb, vb;  // fp8: two chunks under way
+    int page = page_at(t_begin), page_next = page_at(t_begin + kChunk);
+    if constexpr (FP8) {
+      fetch8(t_begin, page, ka, va);
+      if (DEEP8 && t_begin + kChunk < t_end) fetch8(t_begin + kChunk, page_next, kb, vb);
+    } else {
+      dma(k_st0, v_st0, t_begin, page);
+      if (ST == 3 && t_begin + kChunk < t_end) dma(k_st1, v_st1, t_begin + kChunk, page_next);
+    }
+
+    // ---- Q operands: row i16 of 16-row tile t is token 2 t + i16 / 8, head i16 % 8
+    Frag8 qf[QLDS ? 2 : NT][2];
+    uint8_t *q_lds = lds_q + (QLDS ? wave * (2 * NT * 1024) + lane * 16 : 0);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int tl = wtok + 2 * t + (i16 >> 3);
+      Frag8 x[2];
+      x[0].u = x[1].u = u32x4{0, 0, 0, 0};
+      if (tl < ntok) {
+        const uint16_t *src = p.q + ((size_t)(v.row0 + tok0 + tl) * p.num_q_heads + kvh * kGroup + (i16 & 7)) * kHeadDim + 16 * g;
+        x[0].u = *(const u32x4 *)src;
+        x[1].u = *(const u32x4 *)(src + 8);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if constexpr (QLDS) *(u32x4 *)(q_lds + (2 * t + h) * 1024) = x[h].u;  // (read by this lane alone)
+        else qf[t][h] = x[h];
+      }
+    }
+    // ---- the tile's masks: bits of tokens of this sequence, those outside the window taken out
     if (tid < kTok) {
       const int tok = tok0 + tid;
       int depth = -1;
@@ -192,9 +299,8 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_kernel(const TreePara
       }
       lds_lo[tid] = p.window > 0 ? prefix + depth - p.window + 1 : 0;
     }
-    if (tid < 6) (&lds_bad[0][0])[tid] = 0;
-    __syncthreads();
     if (p.window > 0 && p.window < v.qlen) {  // an ancestor may lie outside the window
+      __syncthreads();
       uint64_t keep = 0;
       const int tl = tid / kTreeWordsMax, w = tid % kTreeWordsMax;
       if (tl < kTok) {
@@ -217,23 +323,8 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_kernel(const TreePara
       }
       __syncthreads();
       if (tl < kTok) lds_mask[tl][w] = keep;
-      __syncthreads();
     }
 
-    // ---- Q operands: row i16 of 16-row tile t is token 2 t + i16 / 8, head i16 % 8
-    const int wtok = wave * 2 * NT;  // the wave's first token in the tile
-    const bool wave_active = tok0 + wtok < v.qlen;
-    Frag8 qf[NT][2];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int tok = tok0 + wtok + 2 * t + (i16 >> 3);
-      qf[t][0].u = qf[t][1].u = u32x4{0, 0, 0, 0};
-      if (tok < v.qlen) {
-        const uint16_t *src = p.q + ((size_t)(v.row0 + tok) * p.num_q_heads + kvh * kGroup + (i16 & 7)) * kHeadDim + 16 * g;
-        qf[t][0].u = *(const u32x4 *)src;
-        qf[t][1].u = *(const u32x4 *)(src + 8);
-      }
-    }
     float m[NT], l[NT];
     f32x4 acc[NT][4];
 #pragma unroll
@@ -243,93 +334,68 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_kernel(const TreePara
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) acc[t][mt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
+    bool odd = false;  // this lane took a value that is not finite out of a masked chunk
 
-    // ---- loader
-    u32x4 kr[kElt], vr[kElt];
-    auto fetch = [&](const int tc) {
-      const int page = clamp_id(bt[min(tc / kBlock + wave, last_page)], p.last_block);
-      const uint8_t *kp = p.k_cache + (size_t)page * page_bytes + gl_off;
-      const uint8_t *vp = p.v_cache + (size_t)page * page_bytes + gl_off;
-#pragma unroll
-      for (int e = 0; e < kElt; ++e) {
-        kr[e] = *(const u32x4 *)(kp + 16 * e);
-        vr[e] = *(const u32x4 *)(vp + 16 * e);
-      }
-    };
-    // A chunk that not every row sees whole: keys past the end read as zero; a value that is not
-    // finite must not reach rows that do not see it (0 x inf is NaN in the matrix product), so it
-    // is taken out of the tile and its key remembered (see below).
-    auto masked = [&](const int tc) {
-      return tc + kChunk > prefix || (p.window > 0 && tc < prefix + v.qlen - p.window);
-    };
-    auto stash = [&](const int tc, const int buf, const int slot) {
-      u32x4 k0, k1, v0, v1;
-      if constexpr (FP8) {
-        uint32_t a[4], b[4];
-        fp8x8_to_bf16x8(kr[0][0], kr[0][1], a);
-        fp8x8_to_bf16x8(kr[0][2], kr[0][3], b);
-        k0 = u32x4{a[0], a[1], a[2], a[3]};
-        k1 = u32x4{b[0], b[1], b[2], b[3]};
-        fp8x8_to_bf16x8(vr[0][0], vr[0][1], a);
-        fp8x8_to_bf16x8(vr[0][2], vr[0][3], b);
-        v0 = u32x4{a[0], a[1], a[2], a[3]};
-        v1 = u32x4{b[0], b[1], b[2], b[3]};
-      } else {
-        k0 = kr[0];
-        k1 = kr[kElt - 1];
-        v0 = vr[0];
-        v1 = vr[kElt - 1];
-      }
-      if (masked(tc)) {
-        const bool past = tc + ld_row >= v.len;
-        bool bad = false;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          auto clean = [&](uint32_t x) {
-            if (past) return 0u;
-            const bool hi = (x & 0x7F800000u) == 0x7F800000u, lo = (x & 0x7F80u) == 0x7F80u;
-            bad |= hi | lo;
-            return x & (hi ? 0xFFFFu : ~0u) & (lo ? 0xFFFF0000u : ~0u);
-          };
-          v0[i] = clean(v0[i]);
-          v1[i] = clean(v1[i]);
-        }
-        if (bad) atomicOr(&lds_bad[slot][ld_row >> 5], 1u << (ld_row & 31));
-      }
-      *(u32x4 *)(&lds_k[buf][ld_row * kKRow + ld_seg * 32]) = k0;
-      *(u32x4 *)(&lds_k[buf][ld_row * kKRow + ld_seg * 32 + 16]) = k1;
-      *(u32x4 *)(&lds_v[buf][ld_row * kVRow + ld_seg * 32]) = v0;
-      *(u32x4 *)(&lds_v[buf][ld_row * kVRow + ld_seg * 32 + 16]) = v1;
-    };
-
-    auto step = [&](const int tc, const int buf, const bool need_mask) {
-      const uint8_t *k_rd = &lds_k[buf][0] + i16 * kKRow + g * 32;
-      const uint8_t *v_rd = &lds_v[buf][0] + (4 * g + (i16 >> 2)) * kVRow + 8 * (i16 & 3);
+    // One chunk.  Its tiles overlap: while tile t's exponentials run, the matrix unit works on the
+    // scores of tile t + 1 and the output of tile t - 1.
+    auto step = [&](const uint8_t *kbuf, const uint8_t *vbuf, const int tc) {
+      const bool need_mask = masked(tc);  // (one stream for both kinds: two would not share registers)
       Frag8 kf[4][2], vf[4][2];
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
-        kf[b][0].u = *(const u32x4 *)(k_rd + b * (kBlock * kKRow));
-        kf[b][1].u = *(const u32x4 *)(k_rd + b * (kBlock * kKRow) + 16);
+        kf[b][0].u = *(const u32x4 *)(kbuf + k_off + b * (kBlock * 128));
+        kf[b][1].u = *(const u32x4 *)(kbuf + (k_off ^ 16) + b * (kBlock * 128));
       }
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
         for (int pr = 0; pr < 2; ++pr) {
-          const u32x2 a = lds_read_tr16(v_rd + 32 * mt + (2 * pr) * (kBlock * kVRow));
-          const u32x2 b = lds_read_tr16(v_rd + 32 * mt + (2 * pr + 1) * (kBlock * kVRow));
+          const uint8_t *src = vbuf + v_off + ((32 * mt) ^ v_sw);
+          const u32x2 a = lds_read_tr16(src + (2 * pr) * (kBlock * 128));
+          const u32x2 b = lds_read_tr16(src + (2 * pr + 1) * (kBlock * 128));
           vf[mt][pr].w[0] = a[0];
           vf[mt][pr].w[1] = a[1];
           vf[mt][pr].w[2] = b[0];
           vf[mt][pr].w[3] = b[1];
         }
+      if (need_mask) {
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        f32x4 S[4];
+        for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          S[b] = mfma16x32(kf[b][0], qf[t][0], f32x4{0.f, 0.f, 0.f, 0.f});
-          S[b] = mfma16x32(kf[b][1], qf[t][1], S[b]);
+          for (int pr = 0; pr < 2; ++pr)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t &x = vf[mt][pr].w[i];
+              const bool hi = (x & 0x7F800000u) == 0x7F800000u, lo = (x & 0x7F80u) == 0x7F80u;
+              odd |= hi | lo;
+              x &= (hi ? 0xFFFFu : ~0u) & (lo ? 0xFFFF0000u : ~0u);
+            }
+      }
+      f32x4 S[2][4];
+      Frag8 P[2][2];
+      auto load_q = [&](auto t_c) {
+        constexpr int t = t_c;
+        if constexpr (QLDS && t < NT) {
+          qf[t & 1][0].u = *(const u32x4 *)(q_lds + (2 * t) * 1024);
+          qf[t & 1][1].u = *(const u32x4 *)(q_lds + (2 * t + 1) * 1024);
         }
+      };
+      // matrix instruction j of 8: scores of tile t / output of tile t
+      auto score = [&](auto t_c, auto j_c) {
+        constexpr int t = t_c, j = j_c, b = j & 3, x = QLDS ? t & 1 : t;
+        if constexpr (j < 4) S[t & 1][b] = mfma16x32(kf[b][0], qf[x][0], f32x4{0.f, 0.f, 0.f, 0.f});
+        else S[t & 1][b] = mfma16x32(kf[b][1], qf[x][1], S[t & 1][b]);
+      };
+      auto value = [&](auto t_c, auto j_c) {
+        constexpr int t = t_c, j = j_c, mt = j & 3, pr = j >> 2;
+        acc[t][mt] = mfma16x32(vf[mt][pr], P[t & 1][pr], acc[t][mt]);
+      };
+      load_q(IC<0>{});
+      load_q(IC<1>{});
+      static_for<8>([&](auto j) { score(IC<0>{}, j); });
+      static_for<NT>([&](auto t_c) {
+        constexpr int t = t_c;
+        f32x4(&Sx)[4] = S[t & 1];
         if (need_mask) {
           const int tl = wtok + 2 * t + (i16 >> 3);
           const uint64_t w = chunk_bits(lds_mask[tl], lds_lo[tl], prefix, tc) >> (4 * g);
@@ -337,12 +403,13 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_kernel(const TreePara
           for (int b = 0; b < 4; ++b)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-              if (!((w >> (16 * b + r)) & 1)) S[b][r] = -INFINITY;
+              if (!((w >> (16 * b + r)) & 1)) Sx[b][r] = -INFINITY;
         }
-        float mx = max3(S[0][0], S[0][1], S[0][2]);
+        float mx = max3(Sx[0][0], Sx[0][1], Sx[0][2]);
 #pragma unroll
-        for (int o = 1; o < 7; ++o) mx = max3(mx, S[(2 * o + 1) >> 2][(2 * o + 1) & 3], S[(2 * o + 2) >> 2][(2 * o + 2) & 3]);
-        mx = max2(mx, S[3][3]) * c2;
+        for (int o = 1; o < 7; ++o)
+          mx = max3(mx, Sx[(2 * o + 1) >> 2][(2 * o + 1) & 3], Sx[(2 * o + 2) >> 2][(2 * o + 2) & 3]);
+        mx = max2(mx, Sx[3][3]) * c2;
         if (__any(mx > m[t] + kLazyLog2)) {
           const float mrow = rowgroup_max(mx);
           const float m_new = mrow > m[t] + kLazyLog2 ? mrow : m[t];
@@ -354,83 +421,131 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_kernel(const TreePara
             for (int r = 0; r < 4; ++r) acc[t][mt][r] *= alpha;
           m[t] = m_new;
         }
-        Frag8 P[2];
-        float sum = 0.f;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float p0 = fast_exp2(__builtin_fmaf(S[(2 * k) >> 2][(2 * k) & 3], c2, -m[t]));
-          const float p1 = fast_exp2(__builtin_fmaf(S[(2 * k + 1) >> 2][(2 * k + 1) & 3], c2, -m[t]));
-          sum += p0 + p1;
-          P[k >> 2].w[k & 3] = pack_bf16(p0, p1);
+        EID_SB();
+        // 16 scores of a lane, spread over the stage's matrix instructions
+        constexpr int n_value = t > 0 ? 8 : 0, n_score = t + 1 < NT ? 8 : 0, n_mfma = n_value + n_score;
+        constexpr int per_slot = n_mfma == 16 ? 1 : 2, slots = 16 / per_slot;
+        static_for<slots>([&](auto i_c) {
+          constexpr int i = i_c;
+          if constexpr (i < n_value) value(IC<(t > 0 ? t - 1 : 0)>{}, i_c);
+          else if constexpr (i < n_mfma) score(IC<(t + 1 < NT ? t + 1 : 0)>{}, IC<i - n_value>{});
+          if constexpr (i == n_mfma - 1) load_q(IC<t + 2>{});
+          static_for<per_slot>([&](auto e_c) {
+            constexpr int e = i * per_slot + e_c;
+            const float x = fast_exp2(__builtin_fmaf(Sx[e >> 2][e & 3], c2, -m[t]));
+            Sx[e >> 2][e & 3] = x;
+            if constexpr (e % 2 == 1) {
+              l[t] += Sx[(e - 1) >> 2][(e - 1) & 3];
+              l[t] += x;
+              uint32_t w = pack_bf16(Sx[(e - 1) >> 2][(e - 1) & 3], x);
+              asm volatile("" : "+v"(w), "+v"(l[t]));  // (pinned here: they would be sunk to where they are used)
+              P[t & 1][e >> 3].w[(e >> 1) & 3] = w;
+            }
+          });
+          EID_SB();
+        });
+      });
+      static_for<8>([&](auto j) { value(IC<NT - 1>{}, j); });
+    };
+    if constexpr (FP8) {
+      // chunk c is in stage c % 2, chunk c + 1 in registers; with registers to spare chunk c + 2 is
+      // requested as well
+      stash8(k_st0, v_st0, ka, va);
+      __syncthreads();
+      auto iter = [&](const uint8_t *kcur, const uint8_t *vcur, uint8_t *knxt, uint8_t *vnxt, u32x4 &k1, u32x4 &v1,
+                      u32x4 &k2, u32x4 &v2, const int tc) {
+        if constexpr (DEEP8) {
+          if (tc + 2 * kChunk < t_end) fetch8(tc + 2 * kChunk, page_at(tc + 2 * kChunk), k2, v2);
+        } else {
+          if (tc + kChunk < t_end) fetch8(tc + kChunk, page_at(tc + kChunk), k1, v1);
         }
-        l[t] += sum;
-#pragma unroll
-        for (int mt = 0; mt < 4; ++mt) {
-          acc[t][mt] = mfma16x32(vf[mt][0], P[0], acc[t][mt]);
-          acc[t][mt] = mfma16x32(vf[mt][1], P[1], acc[t][mt]);
+        if (wave_active) step(kcur, vcur, tc);
+        if (tc + kChunk < t_end) stash8(knxt, vnxt, k1, v1);
+        __syncthreads();
+      };
+      for (int tc = t_begin; tc < t_end; tc += 2 * kChunk) {
+        iter(k_st0, v_st0, k_st1, v_st1, DEEP8 ? kb : ka, DEEP8 ? vb : va, ka, va, tc);
+        if (tc + kChunk < t_end) iter(k_st1, v_st1, k_st0, v_st0, ka, va, kb, vb, tc + kChunk);
+      }
+    } else {
+      page = page_at(t_begin + (ST - 1) * kChunk);
+      // (the first chunk's loads are the oldest; the rows of q behind them have to be here as well)
+      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+      __syncthreads();
+      auto iter = [&](const uint8_t *kcur, const uint8_t *vcur, uint8_t *kfar, uint8_t *vfar, const int tc) {
+        const bool more = tc + (ST - 1) * kChunk < t_end;
+        if (more) {
+          dma(kfar, vfar, tc + (ST - 1) * kChunk, page);
+          page = page_at(tc + ST * kChunk);
+        }
+        if (wave_active) step(kcur, vcur, tc);
+        // The next chunk has landed (three stages: its four loads are older than those just issued).
+        // Not __syncthreads(): it would wait for all of them.
+        if (ST == 3 && more) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+      };
+      for (int tc = t_begin; tc < t_end; tc += ST * kChunk) {
+        if constexpr (ST == 3) {
+          iter(k_st0, v_st0, k_st2, v_st2, tc);
+          if (tc + kChunk < t_end) iter(k_st1, v_st1, k_st0, v_st0, tc + kChunk);
+          if (tc + 2 * kChunk < t_end) iter(k_st2, v_st2, k_st1, v_st1, tc + 2 * kChunk);
+        } else {
+          iter(k_st0, v_st0, k_st1, v_st1, tc);
+          if (tc + kChunk < t_end) iter(k_st1, v_st1, k_st0, v_st0, tc + kChunk);
         }
       }
-    };
+    }
 
-    // Values that are not finite, taken out of a masked chunk's tile: their keys' terms are added
-    // row by row, for the rows that see them.  (Rare, and slow: one dot product per row and key.)
-    auto add_bad = [&](const int tc, uint64_t bad) {
-      while (bad) {
-        const int b = __builtin_ctzll(bad);
-        bad &= bad - 1;
-        const int j = tc + b;
-        const int page = clamp_id(bt[min(j / kBlock, last_page)], p.last_block);
-        const size_t off = (size_t)page * page_bytes + (size_t)(j % kBlock) * row_bytes + (size_t)kvh * (kHeadDim * kElt);
-        auto elem = [&](const uint8_t *base, const int d) {
+    // Values that are not finite were taken out of masked chunks: their keys' terms are added row
+    // by row, for the rows that see them.  (Rare, and slow: one dot product per row and key.)
+    if (wave_active && __any(odd)) {
+      for (int tc = t_begin; tc < t_end; tc += kChunk) {
+        if (!masked(tc)) continue;
+        auto row_at = [&](const int j) {
+          const int pg = clamp_id(bt[min(j / kBlock, last_page)], p.last_block);
+          return (size_t)pg * page_bytes + (size_t)(j % kBlock) * row_bytes + (size_t)kvh * (kHeadDim * kElt);
+        };
+        auto elem = [&](const uint8_t *row, const int d) {
           if constexpr (FP8) {
             uint32_t o[4];
-            fp8x8_to_bf16x8(base[off + d], 0, o);
+            fp8x8_to_bf16x8(row[d], 0, o);
             return bf16_bits_to_f32(o[0] & 0xFFFFu);
           } else {
-            return bf16_bits_to_f32(*(const uint16_t *)(base + off + 2 * d));
+            return bf16_bits_to_f32(*(const uint16_t *)(row + 2 * d));
           }
         };
+        auto finite = [](const float x) { return (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u; };
+        bool has = false;  // of key tc + lane
+        if (tc + lane < v.len) {
+          const uint8_t *row = p.v_cache + row_at(tc + lane);
+          for (int d = 0; d < kHeadDim; ++d) has |= !finite(elem(row, d));
+        }
+        uint64_t bad = __ballot(has);
+        while (bad) {
+          const int b = __builtin_ctzll(bad);
+          bad &= bad - 1;
+          const uint8_t *krow = p.k_cache + row_at(tc + b), *vrow = p.v_cache + row_at(tc + b);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const int tl = wtok + 2 * t + (i16 >> 3), tok = tok0 + tl;
-          if (tok < v.qlen && (chunk_bits(lds_mask[tl], lds_lo[tl], prefix, tc) >> b & 1)) {
-            const uint16_t *qr = p.q + ((size_t)(v.row0 + tok) * p.num_q_heads + kvh * kGroup + (i16 & 7)) * kHeadDim;
-            float dot = 0.f;
-            for (int d = 0; d < kHeadDim; ++d) dot += bf16_bits_to_f32(qr[d]) * elem(p.k_cache, d);
-            const float w = fast_exp2(__builtin_fmaf(dot, c2, -m[t]));
+          for (int t = 0; t < NT; ++t) {
+            const int tl = wtok + 2 * t + (i16 >> 3);
+            if (tl < ntok && (chunk_bits(lds_mask[tl], lds_lo[tl], prefix, tc) >> b & 1)) {
+              const uint16_t *qr = p.q + ((size_t)(v.row0 + tok0 + tl) * p.num_q_heads + kvh * kGroup + (i16 & 7)) * kHeadDim;
+              float dot = 0.f;
+              for (int d = 0; d < kHeadDim; ++d) dot += bf16_bits_to_f32(qr[d]) * elem(krow, d);
+              const float w = fast_exp2(__builtin_fmaf(dot, c2, -m[t]));
 #pragma unroll
-            for (int mt = 0; mt < 4; ++mt)
+              for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const float x = elem(p.v_cache, 16 * mt + 4 * g + r);
-                if ((__float_as_uint(x) & 0x7F800000u) == 0x7F800000u) acc[t][mt][r] += w * x;
-              }
+                for (int r = 0; r < 4; ++r) {
+                  const float x = elem(vrow, 16 * mt + 4 * g + r);
+                  if (!finite(x)) acc[t][mt][r] += w * x;
+                }
+            }
           }
         }
       }
-    };
-
-    fetch(t_begin);
-    stash(t_begin, 0, 0);
-    __syncthreads();
-    int cur = 0, slot = 0;
-    for (int tc = t_begin; tc < t_end; tc += kChunk, cur ^= 1) {
-      const bool has_next = tc + kChunk < t_end;
-      const int slot1 = slot == 2 ? 0 : slot + 1, slot2 = slot1 == 2 ? 0 : slot1 + 1;
-      if (has_next) fetch(tc + kChunk);
-      const bool mk = masked(tc);
-      if (tid < 2) lds_bad[slot2][tid] = 0;  // (read last before the barrier that opened this chunk)
-      if (wave_active) {
-        step(tc, cur, mk);
-        if (mk) {
-          const uint64_t bad = (uint64_t)__builtin_amdgcn_readfirstlane(lds_bad[slot][0]) |
-                               (uint64_t)__builtin_amdgcn_readfirstlane(lds_bad[slot][1]) << 32;
-          if (bad) add_bad(tc, bad);
-        }
-      }
-      if (has_next) stash(tc + kChunk, cur ^ 1, slot1);
-      __syncthreads();
-      slot = slot1;
     }
 
     // ---- this piece's rows: the answer, or a partial
@@ -438,20 +553,25 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_kernel(const TreePara
     const int part = c0 == 0 ? 1 : 0;  // a range holds at most one piece of each kind that is not whole
     float *ws_o = p.ws_o + ((size_t)(range * Hkv + kvh) * 2 + part) * (kRows * kHeadDim);
     float *ws_ml = p.ws_ml + ((size_t)(range * Hkv + kvh) * 2 + part) * (kRows * 2);
+    if (!whole && c0 == 0) {
+      const long long last = u - c0 + v.chunks - 1;  // the tile's last unit
+      rec = {v.row0 + tok0, ntok, (int)(last / per) - range + 1, 0};
+    }
     if (wave_active) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const int tl = wtok + 2 * t + (i16 >> 3), tok = tok0 + tl;
+        const int tl = wtok + 2 * t + (i16 >> 3);
         const float lt = rowgroup_sum(l[t]);
-        if (tok >= v.qlen) continue;
+        if (tl >= ntok) continue;
         if (whole) {
           const int head = kvh * kGroup + (i16 & 7);
           const float sink = p.sinks ? p.sinks[head] * kLog2e : -INFINITY;
           // (a row that sees nothing, m = kNegBig, has only its sink)
           const float M = max2(m[t], sink), a = fast_exp2(m[t] - M);
           const float den = lt * a + fast_exp2(sink - M);
-          const float f = den > 0.f || den != den ? vs * a / den : 0.f;
-          const size_t orow = (size_t)(v.row0 + tok) * p.num_q_heads + head;
+          const bool any = den > 0.f || den != den;
+          const float f = any ? vs * a / den : 0.f;
+          const size_t orow = (size_t)(v.row0 + tok0 + tl) * p.num_q_heads + head;
 #pragma unroll
           for (int mt = 0; mt < 4; ++mt) {
             u32x2 w;
@@ -459,7 +579,7 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_kernel(const TreePara
             w[1] = pack_bf16(acc[t][mt][2] * f, acc[t][mt][3] * f);
             *(u32x2 *)(p.out + orow * kHeadDim + 16 * mt + 4 * g) = w;
           }
-          if (p.lse && g == 0) p.lse[orow] = den > 0.f || den != den ? (M + __log2f(den)) * kLn2 : -INFINITY;
+          if (p.lse && g == 0) p.lse[orow] = any ? (M + __log2f(den)) * kLn2 : -INFINITY;
         } else {
           const int row = tl * kGroup + (i16 & 7);
 #pragma unroll
@@ -473,77 +593,106 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_kernel(const TreePara
     }
     u += n;
   }
+  if (kvh == 0 && tid == 0) p.ws_rec[range] = rec;
 }
 
-// Joins the pieces of the rows that a range's end cut: out = sum 2^(m - M) o / (sum 2^(m - M) l + 2^(sink - M)).
-// One workgroup per (row, KV head); a thread per (head, pair of dims).
+// Joins the pieces of a tile that range ends cut: out = sum 2^(m - M) o / (sum 2^(m - M) l + 2^(sink - M)).
+// At most one tile begins in a range without ending there (its record).  A workgroup takes two
+// tokens of it: 16 rows x 4 quarters of the dims x every fourth piece.
 __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeParams p, const int tile_tok) {
-  const int Hkv = p.num_kv_heads, kvh = blockIdx.x % Hkv, row = blockIdx.x / Hkv;
-  int lo = 0, hi = p.num_seqs - 1;
-  while (lo < hi) {  // the last sequence that starts at or before the row
-    const int mid = (lo + hi + 1) >> 1;
-    if (p.cu_seqlens_q[mid] <= row) lo = mid; else hi = mid - 1;
-  }
-  const int s = lo;
-  const TreeSeq v = tree_seq(p, s, tile_tok);
-  const int tok = row - v.row0;
-  if (tok < 0 || tok >= v.qlen) return;
-  long long total, before;
-  count_units(p, tile_tok, s, total, before);
-  const long long per = range_units(p, total);
-  const int tile = tok / tile_tok;
-  const long long u0 = before + (long long)tile * v.chunks, u1 = u0 + v.chunks;
-  const int r0 = (int)(u0 / per), r1 = (int)((u1 - 1) / per);
-  if (r0 == r1) return;  // one range held it whole
-  const int h = threadIdx.x >> 5, d = (threadIdx.x & 31) * 2;
-  const int head = kvh * kGroup + h, prow = (tok - tile * tile_tok) * kGroup + h;
-  const float sink = p.sinks ? p.sinks[head] * kLog2e : -INFINITY;
+  const int Hkv = p.num_kv_heads;
+  int b = blockIdx.x;
+  const int pair = b % (tile_tok / 2);
+  b /= tile_tok / 2;
+  const int kvh = b % Hkv, range = b / Hkv;
+  const TreeRecord rec = p.ws_rec[range];
+  const int lane = threadIdx.x & 63;
+  // lane = (row of four, quarter, piece group): the piece groups of a row are four lanes of a wave
+  const int pg = lane & 3, quarter = (lane >> 2) & 3, row = (threadIdx.x >> 6) * 4 + (lane >> 4);
+  const int tl = 2 * pair + (row >> 3), h = row & 7;
+  if (2 * pair >= rec.ntok) return;
   const int rows = tile_tok * kGroup;
-  auto cell = [&](const int r) { return ((size_t)(r * Hkv + kvh) * 2 + (r == r0 ? 1 : 0)) * rows + prow; };
-  float M = max2(sink, kNegBig), den = 0.f, o0 = 0.f, o1 = 0.f;
-  for (int r = r0; r <= r1; ++r) {
-    const size_t c = cell(r);
-    const float2 ml = *(const float2 *)(p.ws_ml + 2 * c);
-    const float2 o = *(const float2 *)(p.ws_o + c * kHeadDim + d);
-    const float M1 = max2(M, ml.x), a = fast_exp2(M - M1), w = fast_exp2(ml.x - M1);
-    den = den * a + ml.y * w;
-    o0 = o0 * a + o.x * w;
-    o1 = o1 * a + o.y * w;
-    M = M1;
+  const size_t cell0 = (size_t)(range * Hkv + kvh) * 2 * rows + tl * kGroup + h;
+  const int head = kvh * kGroup + h;
+  f32x4 o[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) o[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float M = kNegBig, den = 0.f;
+  if (tl < rec.ntok) {
+    for (int i = pg; i < rec.pieces; i += 4) {
+      const size_t c = cell0 + (size_t)i * Hkv * 2 * rows + (i == 0 ? rows : 0);
+      const float2 ml = *(const float2 *)(p.ws_ml + 2 * c);
+      const f32x4 *src = (const f32x4 *)(p.ws_o + c * kHeadDim + 16 * quarter);
+      const float M1 = max2(M, ml.x), a = fast_exp2(M - M1), w = fast_exp2(ml.x - M1);
+      den = den * a + ml.y * w;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const f32x4 x = src[k];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[k][r] = o[k][r] * a + x[r] * w;
+      }
+      M = M1;
+    }
   }
-  den += fast_exp2(sink - M);
+  const float sink = p.sinks ? p.sinks[head] * kLog2e : -INFINITY;
+  float all = max2(M, __shfl_xor(M, 1));
+  all = max2(all, __shfl_xor(all, 2));
+  all = max2(all, sink);
+  const float a = fast_exp2(M - all);
+  den *= a;
+  den += __shfl_xor(den, 1);
+  den += __shfl_xor(den, 2);
+  den += fast_exp2(sink - all);
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      float x = o[k][r] * a;
+      x += __shfl_xor(x, 1);
+      x += __shfl_xor(x, 2);
+      o[k][r] = x;
+    }
+  if (tl >= rec.ntok) return;
   const float vs = p.v_scale ? p.v_scale[kvh] : 1.0f;
   const bool any = den > 0.f || den != den;
   const float f = any ? vs / den : 0.f;
-  const size_t orow = (size_t)row * p.num_q_heads + head;
-  *(uint32_t *)(p.out + orow * kHeadDim + d) = pack_bf16(o0 * f, o1 * f);
-  if (p.lse && d == 0) p.lse[orow] = any ? (M + __log2f(den)) * kLn2 : -INFINITY;
+  const size_t orow = (size_t)(rec.row + tl) * p.num_q_heads + head;
+  const f32x4 mine = pg == 0 ? o[0] : pg == 1 ? o[1] : pg == 2 ? o[2] : o[3];
+  u32x2 w;
+  w[0] = pack_bf16(mine[0] * f, mine[1] * f);
+  w[1] = pack_bf16(mine[2] * f, mine[3] * f);
+  *(u32x2 *)(p.out + orow * kHeadDim + 16 * quarter + 4 * pg) = w;
+  if (p.lse && pg == 0 && quarter == 0) p.lse[orow] = any ? (all + __log2f(den)) * kLn2 : -INFINITY;
 }
 
 }  // namespace
 
-// 16-row tiles per wave: the fewest that hold the longest tree in one workgroup, or the most.
-int tree_tiles(const int max_q_len) { return max_q_len <= 8 ? 1 : max_q_len <= 16 ? 2 : 4; }
+// 16-row tiles per wave: a tree is cut into the fewest tiles of at most 32 tokens, of about equal size.
+int tree_tiles(const int max_q_len) {
+  const int tiles = (max_q_len + 31) / 32;
+  return ((max_q_len + tiles - 1) / tiles + 7) / 8;
+}
 int tree_tile_tokens(const int max_q_len) { return 2 * tree_tiles(max_q_len) * kTreeWaves; }
+
+template <bool FP8>
+static void launch_tree_tiles(const TreeParams &p, const int nt, hipStream_t st) {
+  const dim3 grid((unsigned)(p.ranges * p.num_kv_heads)), block(kTreeWaves * 64);
+  if (nt == 1) tree_kernel<1, FP8><<<grid, block, 0, st>>>(p);
+  else if (nt == 2) tree_kernel<2, FP8><<<grid, block, 0, st>>>(p);
+  else if (nt == 3) tree_kernel<3, FP8><<<grid, block, 0, st>>>(p);
+  else tree_kernel<4, FP8><<<grid, block, 0, st>>>(p);
+}
 
 hipError_t launch_tree(const TreeParams &p, const bool fp8, hipStream_t st) {
   const int nt = tree_tiles(p.max_q_len);
-  const dim3 grid((unsigned)(p.ranges * p.num_kv_heads)), block(kTreeWaves * 64);
-  if (nt == 1) {
-    if (fp8) tree_kernel<1, true><<<grid, block, 0, st>>>(p);
-    else tree_kernel<1, false><<<grid, block, 0, st>>>(p);
-  } else if (nt == 2) {
-    if (fp8) tree_kernel<2, true><<<grid, block, 0, st>>>(p);
-    else tree_kernel<2, false><<<grid, block, 0, st>>>(p);
-  } else {
-    if (fp8) tree_kernel<4, true><<<grid, block, 0, st>>>(p);
-    else tree_kernel<4, false><<<grid, block, 0, st>>>(p);
-  }
+  if (fp8) launch_tree_tiles<true>(p, nt, st);
+  else launch_tree_tiles<false>(p, nt, st);
   return hipGetLastError();
 }
 
 hipError_t launch_tree_merge(const TreeParams &p, hipStream_t st) {
-  tree_merge_kernel<<<(unsigned)p.num_kv_heads * (unsigned)p.num_q_tokens, 256, 0, st>>>(p, tree_tile_tokens(p.max_q_len));
+  const int tile = tree_tile_tokens(p.max_q_len);
+  tree_merge_kernel<<<(unsigned)(p.ranges * p.num_kv_heads * (tile / 2)), 256, 0, st>>>(p, tile);
   return hipGetLastError();
 }
 
