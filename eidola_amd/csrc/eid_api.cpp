@@ -1176,6 +1176,10 @@ int32_t check_tree_desc(const eid_attn_desc *d) {
   if (int32_t rc = check_attn_desc(d)) return rc;
   if (d->max_q_len > eid::kTreeMax)
     return fail(EID_ERR_UNSUPPORTED, "max_q_len %d: a tree has at most %d tokens", d->max_q_len, eid::kTreeMax);
+  // the kernel counts the launch's 64-key chunks in 32 bits
+  const long long tile = eid::tree_tile_tokens(d->max_q_len);
+  if ((d->max_q_len + tile - 1) / tile * (d->max_kv_len / eid::kChunk + 2LL) * d->num_seqs > 0x3fffffffLL)
+    return fail(EID_ERR_UNSUPPORTED, "batch of %d sequences of up to %d keys is too large", d->num_seqs, d->max_kv_len);
   return EID_OK;
 }
 
@@ -1250,6 +1254,7 @@ int32_t eid_attn_tree(const eid_attn_desc *desc, const eid_attn_args *args, cons
   p.mask_words = mask_words;
   p.window = desc->window;
   p.max_q_len = desc->max_q_len;
+  p.max_kv_len = desc->max_kv_len;
   p.ranges = pl.ranges;
   p.min_chunks = eid::kTreeMinChunks;
   p.softmax_scale = desc->softmax_scale;

@@ -30,7 +30,7 @@ struct TreeParams {
   float *ws_o;   // [ranges][Hkv][2][tile rows][64]  sum of e^(s-m) v of a piece, not normalised
   float *ws_ml;  // [ranges][Hkv][2][tile rows][2]   m (log2 units), l
   int32_t num_seqs, num_q_heads, num_kv_heads, max_blocks_per_seq, last_block;
-  int32_t num_q_tokens, mask_words, window, max_q_len;
+  int32_t num_q_tokens, mask_words, window, max_q_len, max_kv_len;
   int32_t ranges;     // workgroups per KV head
   int32_t min_chunks; // smallest range
   float softmax_scale;

@@ -14,7 +14,7 @@ __device__ __forceinline__ int clamp_id(const int id, const int last) { return m
 
 constexpr float kLazyLog2 = 8.0f;  // a row's reference moves when a score outgrows it by this
 
-// What one sequence gives the kernels: `chunks` 64-key chunks from key `begin` on for each of
+// What one sequence gives the kernel: `chunks` 64-key chunks from key `begin` on for each of
 // `tiles` tiles of drafted tokens.
 struct TreeSeq {
   int row0, qlen, len, begin, chunks, tiles;
@@ -22,77 +22,75 @@ struct TreeSeq {
 
 // The rows at and behind prefix = len - qlen stand for the drafted tokens.  A token's position is
 // prefix + (ancestors it sees) >= prefix - 1, so no row sees keys below prefix - window.
-__device__ __forceinline__ TreeSeq tree_seq(const TreeParams &p, const int s, const int tile_tok) {
+__device__ __forceinline__ TreeSeq tree_seq(const TreeParams &p, const int row0, const int row1, const int len,
+                                            const int tile_tok) {
   TreeSeq v;
-  const const_i32_ptr cu = as_constant(p.cu_seqlens_q), sl = as_constant(p.seq_lens);
-  v.row0 = cu[s];
-  v.qlen = cu[s + 1] - v.row0;
-  v.len = min(sl[s], p.max_blocks_per_seq * kBlock);
+  v.row0 = row0;
+  v.qlen = row1 - row0;
+  v.len = min(len, p.max_kv_len);
   // (junk lengths: nothing of the sequence is computed, nothing is read)
-  if (v.qlen < 0 || v.qlen > kTreeMax || v.qlen > p.mask_words * 64 || v.len < v.qlen || v.row0 < 0 ||
-      v.row0 + v.qlen > p.num_q_tokens)
-    v.qlen = 0;
+  if (row0 < 0 || row1 < row0 || row1 > p.num_q_tokens || v.qlen > p.max_q_len || v.len < v.qlen) v.qlen = 0;
   v.begin = p.window > 0 ? max(0, v.len - v.qlen - p.window) & ~(kBlock - 1) : 0;
   v.tiles = (v.qlen + tile_tok - 1) / tile_tok;
   v.chunks = v.qlen > 0 ? (v.len - v.begin + kChunk - 1) / kChunk : 0;
   return v;
 }
-__device__ __forceinline__ long long units_of(const TreeSeq &v) { return (long long)v.tiles * v.chunks; }
 
-__device__ __forceinline__ long long uniform64(const long long x) {
-  return (long long)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)x) |
-                     (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32);
-}
-
-// Units of all sequences, and those of the sequences before `upto`: by every wave for itself.
-__device__ __forceinline__ void count_units(const TreeParams &p, const int tile_tok, const int upto,
-                                            long long &total, long long &before) {
+// Place of one workgroup's range in the line of units.  Batches of up to 64 sequences are looked at
+// once, a lane per sequence; `lane_*` stay with the lanes.
+struct TreePlace {
+  int lane_row0, lane_row1, lane_len;
+  int per, u, u_end;  // units per range; this range's
+  int seq, before;    // the sequence that holds unit u, and the units before it
+};
+__device__ __forceinline__ int inclusive_scan(int x) {
   const int lane = threadIdx.x & 63;
-  long long a = 0, b = 0;
-  for (int s = lane; s < p.num_seqs; s += 64) {
-    const long long u = units_of(tree_seq(p, s, tile_tok));
-    a += u;
-    if (s < upto) b += u;
-  }
 #pragma unroll
-  for (int d = 32; d > 0; d >>= 1) {
-    a += __shfl_xor(a, d);
-    b += __shfl_xor(b, d);
+  for (int d = 1; d < 64; d <<= 1) {
+    const int o = __shfl_up(x, d);
+    if (lane >= d) x += o;
   }
-  total = uniform64(a);
-  before = uniform64(b);
+  return x;
 }
-
-// Sequence that holds unit u and the units before it.
-__device__ __forceinline__ int find_seq(const TreeParams &p, const int tile_tok, const long long u,
-                                        long long &before) {
+__device__ __forceinline__ TreePlace find_place(const TreeParams &p, const int range, const int tile_tok) {
   const int lane = threadIdx.x & 63;
-  long long base = 0;
-  for (int s0 = 0; s0 < p.num_seqs; s0 += 64) {
-    const int s = s0 + lane;
-    const long long n = s < p.num_seqs ? units_of(tree_seq(p, s, tile_tok)) : 0;
-    long long incl = n;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const long long o = __shfl_up(incl, d);
-      if (lane >= d) incl += o;
+  TreePlace w;
+  int total = 0, incl = 0, n = 0;
+  auto load = [&](const int s) {
+    w.lane_row0 = w.lane_row1 = w.lane_len = 0;
+    if (s < p.num_seqs) {
+      w.lane_row0 = p.cu_seqlens_q[s];
+      w.lane_row1 = p.cu_seqlens_q[s + 1];
+      w.lane_len = p.seq_lens[s];
     }
-    const unsigned long long hit = __ballot(base + incl > u);
-    if (hit) {
-      const int i = __builtin_ctzll(hit);
-      before = uniform64(base + __shfl(incl, i) - __shfl(n, i));
-      return s0 + i;
+    const TreeSeq v = tree_seq(p, w.lane_row0, w.lane_row1, w.lane_len, tile_tok);
+    n = v.tiles * v.chunks;
+    incl = inclusive_scan(n);
+    return __builtin_amdgcn_readlane(incl, 63);
+  };
+  for (int s0 = 0; s0 < p.num_seqs; s0 += 64) total += load(s0 + lane);
+  w.per = max((total + p.ranges - 1) / p.ranges, p.min_chunks);
+  w.u = range < (total + w.per - 1) / w.per ? range * w.per : total;
+  w.u_end = min(total - w.u, w.per) + w.u;
+  w.seq = w.before = 0;
+  for (int s0 = 0, base = 0; w.u < w.u_end; s0 += 64) {  // (the unit exists: some batch holds it)
+    const int sum = p.num_seqs <= 64 ? total : load(s0 + lane);
+    if (base + sum > w.u) {
+      const int i = __builtin_ctzll(__ballot(base + incl > w.u));
+      w.seq = s0 + i;
+      w.before = base + __builtin_amdgcn_readlane(incl, i) - __builtin_amdgcn_readlane(n, i);
+      break;
     }
-    base += uniform64(__shfl(incl, 63));
+    base += sum;
   }
-  before = base;
-  return p.num_seqs;
+  return w;
 }
-
-// Chunks per workgroup: equal contiguous ranges of the launch's units.
-__device__ __forceinline__ long long range_units(const TreeParams &p, const long long total) {
-  const long long q = (total + p.ranges - 1) / p.ranges;
-  return q > p.min_chunks ? q : p.min_chunks;
+__device__ __forceinline__ TreeSeq seq_at(const TreeParams &p, const TreePlace &w, const int s, const int tile_tok) {
+  if (p.num_seqs <= 64)
+    return tree_seq(p, __builtin_amdgcn_readlane(w.lane_row0, s), __builtin_amdgcn_readlane(w.lane_row1, s),
+                    __builtin_amdgcn_readlane(w.lane_len, s), tile_tok);
+  const const_i32_ptr cu = as_constant(p.cu_seqlens_q), sl = as_constant(p.seq_lens);
+  return tree_seq(p, cu[s], cu[s + 1], sl[s], tile_tok);
 }
 
 // 64 visibility bits of one drafted token for the keys tc .. tc + 63.
@@ -127,7 +125,7 @@ __device__ __forceinline__ uint64_t chunk_bits(const uint64_t *mask, const int l
 // K and V chunks stand in LDS as 64 rows of 128 bytes, read by all four waves; 16-byte segments
 // are permuted by the row (K: segment ^ (row / 2) % 8, V: pairs of segments by (row / 2) % 4),
 // which keeps the operand reads off each other's banks without padding.  bf16 caches: direct
-// global -> LDS loads, three stages, two chunks under way while one is computed.  fp8 caches:
+// global -> LDS loads, up to three chunks under way while one is computed.  fp8 caches:
 // through registers, where the bytes are widened once for the four waves, two stages.
 //
 // Chunks that some row does not see whole (the drafted tokens' own, a window's edge) differ in
@@ -157,13 +155,16 @@ __global__ __launch_bounds__(kTreeWaves * 64, NT == 1 ? 3 : 2) void tree_kernel(
   constexpr int kRows = kTok * kGroup;
   constexpr int kElt = FP8 ? 1 : 2;
   // Q operands of three and four tiles do not fit the registers beside the rest: LDS, in place of
-  // the third stage.
+  // more stages.
   constexpr bool QLDS = NT >= 3;
-  constexpr int ST = FP8 || QLDS ? 2 : 3;  // K/V stages
+  constexpr int ST = FP8 || QLDS ? 2 : 4;  // K/V stages
   constexpr bool DEEP8 = NT <= 3;          // fp8: two chunks under way
   // (separate arrays: the compiler can then tell the stage being filled from the one being read)
-  __shared__ __align__(1024) uint8_t k_st0[kTileBytes], k_st1[kTileBytes], k_st2[ST == 3 ? kTileBytes : 16];
-  __shared__ __align__(1024) uint8_t v_st0[kTileBytes], v_st1[kTileBytes], v_st2[ST == 3 ? kTileBytes : 16];
+  // one tile per tree: every chunk is read once, past the caches (non-temporal)
+  constexpr int kAux = NT <= 2 ? 2 : 0;
+  constexpr int kMore = ST == 4 ? kTileBytes : 16;
+  __shared__ __align__(1024) uint8_t k_st0[kTileBytes], k_st1[kTileBytes], k_st2[kMore], k_st3[kMore];
+  __shared__ __align__(1024) uint8_t v_st0[kTileBytes], v_st1[kTileBytes], v_st2[kMore], v_st3[kMore];
   __shared__ __align__(16) uint8_t lds_q[QLDS ? kTreeWaves * 2 * NT * 1024 : 16];
   __shared__ uint64_t lds_mask[kTok][kTreeWordsMax];
   __shared__ int lds_lo[kTok];
@@ -175,14 +176,9 @@ __global__ __launch_bounds__(kTreeWaves * 64, NT == 1 ? 3 : 2) void tree_kernel(
   const float c2 = p.softmax_scale * kLog2e * (FP8 ? p.k_scale[kvh] : 1.0f);
   const float vs = FP8 ? p.v_scale[kvh] : 1.0f;
 
-  long long total, ignored;
-  count_units(p, kTok, 0, total, ignored);
-  const long long per = range_units(p, total);
-  long long u = per * range;
-  const long long u_end = min(total, u + per);
+  const TreePlace place = find_place(p, range, kTok);
+  int u = place.u, s = place.seq, before = place.before;
   TreeRecord rec = {0, 0, 0, 0};  // what the merge has to join from this range on
-  long long before = 0;
-  int s = u < u_end ? find_seq(p, kTok, u, before) : 0;
 
   const uint32_t row_bytes = (uint32_t)Hkv * kHeadDim * kElt;
   const size_t page_bytes = (size_t)kBlock * row_bytes;
@@ -193,16 +189,16 @@ __global__ __launch_bounds__(kTreeWaves * 64, NT == 1 ? 3 : 2) void tree_kernel(
   const uint32_t v_off = (uint32_t)v_row * 128 + 8 * (i16 & 3);
   const int v_sw = 32 * ((v_row >> 1) & 3);
 
-  while (u < u_end) {
-    const TreeSeq v = tree_seq(p, s, kTok);
-    if (u - before >= units_of(v)) {  // next sequence (those without rows have no units)
-      before += units_of(v);
+  while (u < place.u_end) {
+    const TreeSeq v = seq_at(p, place, s, kTok);
+    const int units = v.tiles * v.chunks;
+    if (u - before >= units) {  // next sequence (those without rows have no units)
+      before += units;
       ++s;
       continue;
     }
-    const int tile = (int)((u - before) / v.chunks);
-    const int c0 = (int)((u - before) - (long long)tile * v.chunks);
-    const int n = (int)min((long long)(v.chunks - c0), u_end - u);
+    const int tile = (u - before) / v.chunks, c0 = (u - before) - tile * v.chunks;
+    const int n = min(v.chunks - c0, place.u_end - u);
     const int prefix = v.len - v.qlen;
     const int tok0 = tile * kTok;                   // first token of the tile, in the sequence
     const int ntok = min(kTok, v.qlen - tok0);
@@ -228,8 +224,8 @@ __global__ __launch_bounds__(kTreeWaves * 64, NT == 1 ? 3 : 2) void tree_kernel(
         const int tok = min(tc + 16 * wave + 8 * h + dr, v.len - 1);
         const uint32_t off = (uint32_t)(tok & 15) * row_bytes;
         const int kseg = sl ^ (4 * h + (dr >> 1)), vseg = sl ^ ((dr >> 1) << 1);
-        __builtin_amdgcn_global_load_lds((gptr_t *)(kp + off + kseg * 16), (lptr_t *)(kbuf + (2 * wave + h) * 1024), 16, 0, 0);
-        __builtin_amdgcn_global_load_lds((gptr_t *)(vp + off + vseg * 16), (lptr_t *)(vbuf + (2 * wave + h) * 1024), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((gptr_t *)(kp + off + kseg * 16), (lptr_t *)(kbuf + (2 * wave + h) * 1024), 16, 0, kAux);
+        __builtin_amdgcn_global_load_lds((gptr_t *)(vp + off + vseg * 16), (lptr_t *)(vbuf + (2 * wave + h) * 1024), 16, 0, kAux);
       }
     };
     const int fr = lane >> 2, fs = lane & 3;  // fp8: row of the page, 16-element segment
@@ -261,7 +257,10 @@ __global__ __launch_bounds__(kTreeWaves * 64, NT == 1 ? 3 : 2) void tree_kernel(
       if (DEEP8 && t_begin + kChunk < t_end) fetch8(t_begin + kChunk, page_next, kb, vb);
     } else {
       dma(k_st0, v_st0, t_begin, page);
-      if (ST == 3 && t_begin + kChunk < t_end) dma(k_st1, v_st1, t_begin + kChunk, page_next);
+      if constexpr (ST == 4) {
+        if (t_begin + kChunk < t_end) dma(k_st1, v_st1, t_begin + kChunk, page_next);
+        if (t_begin + 2 * kChunk < t_end) dma(k_st2, v_st2, t_begin + 2 * kChunk, page_at(t_begin + 2 * kChunk));
+      }
     }
 
     // ---- Q operands: row i16 of 16-row tile t is token 2 t + i16 / 8, head i16 % 8
@@ -479,18 +478,20 @@ __global__ __launch_bounds__(kTreeWaves * 64, NT == 1 ? 3 : 2) void tree_kernel(
           page = page_at(tc + ST * kChunk);
         }
         if (wave_active) step(kcur, vcur, tc);
-        // The next chunk has landed (three stages: its four loads are older than those just issued).
+        // The next chunk has landed: its four loads are older than those of the chunks behind it.
         // Not __syncthreads(): it would wait for all of them.
-        if (ST == 3 && more) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)" ::: "memory");
+        if (ST == 4 && tc + 3 * kChunk < t_end) asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
+        else if (ST == 4 && tc + 2 * kChunk < t_end) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)" ::: "memory");
         else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
       };
       for (int tc = t_begin; tc < t_end; tc += ST * kChunk) {
-        if constexpr (ST == 3) {
-          iter(k_st0, v_st0, k_st2, v_st2, tc);
+        if constexpr (ST == 4) {
+          iter(k_st0, v_st0, k_st3, v_st3, tc);
           if (tc + kChunk < t_end) iter(k_st1, v_st1, k_st0, v_st0, tc + kChunk);
           if (tc + 2 * kChunk < t_end) iter(k_st2, v_st2, k_st1, v_st1, tc + 2 * kChunk);
+          if (tc + 3 * kChunk < t_end) iter(k_st3, v_st3, k_st2, v_st2, tc + 3 * kChunk);
         } else {
           iter(k_st0, v_st0, k_st1, v_st1, tc);
           if (tc + kChunk < t_end) iter(k_st1, v_st1, k_st0, v_st0, tc + kChunk);
@@ -554,8 +555,8 @@ __global__ __launch_bounds__(kTreeWaves * 64, NT == 1 ? 3 : 2) void tree_kernel(
     float *ws_o = p.ws_o + ((size_t)(range * Hkv + kvh) * 2 + part) * (kRows * kHeadDim);
     float *ws_ml = p.ws_ml + ((size_t)(range * Hkv + kvh) * 2 + part) * (kRows * 2);
     if (!whole && c0 == 0) {
-      const long long last = u - c0 + v.chunks - 1;  // the tile's last unit
-      rec = {v.row0 + tok0, ntok, (int)(last / per) - range + 1, 0};
+      const int last = u - c0 + v.chunks - 1;  // the tile's last unit
+      rec = {v.row0 + tok0, ntok, last / place.per - range + 1, 0};
     }
     if (wave_active) {
 #pragma unroll
@@ -597,20 +598,15 @@ __global__ __launch_bounds__(kTreeWaves * 64, NT == 1 ? 3 : 2) void tree_kernel(
 }
 
 // Joins the pieces of a tile that range ends cut: out = sum 2^(m - M) o / (sum 2^(m - M) l + 2^(sink - M)).
-// At most one tile begins in a range without ending there (its record).  A workgroup takes two
-// tokens of it: 16 rows x 4 quarters of the dims x every fourth piece.
+// At most one tile begins in a range without ending there (its record).  A workgroup takes four
+// tokens of it: 32 rows x 4 quarters of the dims x every other piece, two pieces at a time.
 __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeParams p, const int tile_tok) {
-  const int Hkv = p.num_kv_heads;
-  int b = blockIdx.x;
-  const int pair = b % (tile_tok / 2);
-  b /= tile_tok / 2;
-  const int kvh = b % Hkv, range = b / Hkv;
+  const int Hkv = p.num_kv_heads, kvh = blockIdx.x % Hkv;
+  const int b = blockIdx.x / Hkv, range = b % p.ranges, tok = b / p.ranges * 4;
   const TreeRecord rec = p.ws_rec[range];
-  const int lane = threadIdx.x & 63;
-  // lane = (row of four, quarter, piece group): the piece groups of a row are four lanes of a wave
-  const int pg = lane & 3, quarter = (lane >> 2) & 3, row = (threadIdx.x >> 6) * 4 + (lane >> 4);
-  const int tl = 2 * pair + (row >> 3), h = row & 7;
-  if (2 * pair >= rec.ntok) return;
+  if (tok >= rec.ntok) return;
+  const int pg = threadIdx.x & 1, quarter = (threadIdx.x >> 1) & 3, row = threadIdx.x >> 3;
+  const int tl = tok + (row >> 3), h = row & 7;
   const int rows = tile_tok * kGroup;
   const size_t cell0 = (size_t)(range * Hkv + kvh) * 2 * rows + tl * kGroup + h;
   const int head = kvh * kGroup + h;
@@ -620,48 +616,53 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeParams p, con
   float M = kNegBig, den = 0.f;
   if (tl < rec.ntok) {
     for (int i = pg; i < rec.pieces; i += 4) {
-      const size_t c = cell0 + (size_t)i * Hkv * 2 * rows + (i == 0 ? rows : 0);
-      const float2 ml = *(const float2 *)(p.ws_ml + 2 * c);
-      const f32x4 *src = (const f32x4 *)(p.ws_o + c * kHeadDim + 16 * quarter);
-      const float M1 = max2(M, ml.x), a = fast_exp2(M - M1), w = fast_exp2(ml.x - M1);
-      den = den * a + ml.y * w;
+      float2 ml[2];
+      f32x4 x[2][4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const f32x4 x = src[k];
+      for (int e = 0; e < 2; ++e) {
+        const int j = min(i + 2 * e, rec.pieces - 1);  // (the last one again: its weight is taken away below)
+        const size_t c = cell0 + (size_t)j * Hkv * 2 * rows + (j == 0 ? rows : 0);
+        ml[e] = *(const float2 *)(p.ws_ml + 2 * c);
+        const f32x4 *src = (const f32x4 *)(p.ws_o + c * kHeadDim + 16 * quarter);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[k][r] = o[k][r] * a + x[r] * w;
+        for (int k = 0; k < 4; ++k) x[e][k] = src[k];
       }
+      const bool two = i + 2 < rec.pieces;
+      const float M1 = max2(M, two ? max2(ml[0].x, ml[1].x) : ml[0].x);
+      const float a = fast_exp2(M - M1), w0 = fast_exp2(ml[0].x - M1), w1 = fast_exp2(ml[1].x - M1);
+      den = den * a + ml[0].y * w0 + (two ? ml[1].y * w1 : 0.f);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[k][r] = o[k][r] * a + x[0][k][r] * w0 + (two ? x[1][k][r] * w1 : 0.f);
       M = M1;
     }
   }
   const float sink = p.sinks ? p.sinks[head] * kLog2e : -INFINITY;
-  float all = max2(M, __shfl_xor(M, 1));
-  all = max2(all, __shfl_xor(all, 2));
-  all = max2(all, sink);
+  const float all = max2(max2(M, __shfl_xor(M, 1)), sink);
   const float a = fast_exp2(M - all);
   den *= a;
   den += __shfl_xor(den, 1);
-  den += __shfl_xor(den, 2);
   den += fast_exp2(sink - all);
 #pragma unroll
   for (int k = 0; k < 4; ++k)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      float x = o[k][r] * a;
-      x += __shfl_xor(x, 1);
-      x += __shfl_xor(x, 2);
-      o[k][r] = x;
+      const float x = o[k][r] * a;
+      o[k][r] = x + __shfl_xor(x, 1);
     }
   if (tl >= rec.ntok) return;
   const float vs = p.v_scale ? p.v_scale[kvh] : 1.0f;
   const bool any = den > 0.f || den != den;
   const float f = any ? vs / den : 0.f;
   const size_t orow = (size_t)(rec.row + tl) * p.num_q_heads + head;
-  const f32x4 mine = pg == 0 ? o[0] : pg == 1 ? o[1] : pg == 2 ? o[2] : o[3];
-  u32x2 w;
-  w[0] = pack_bf16(mine[0] * f, mine[1] * f);
-  w[1] = pack_bf16(mine[2] * f, mine[3] * f);
-  *(u32x2 *)(p.out + orow * kHeadDim + 16 * quarter + 4 * pg) = w;
+  const f32x4 lo = pg ? o[2] : o[0], hi = pg ? o[3] : o[1];  // each of the two stores eight dims
+  u32x4 w;
+  w[0] = pack_bf16(lo[0] * f, lo[1] * f);
+  w[1] = pack_bf16(lo[2] * f, lo[3] * f);
+  w[2] = pack_bf16(hi[0] * f, hi[1] * f);
+  w[3] = pack_bf16(hi[2] * f, hi[3] * f);
+  *(u32x4 *)(p.out + orow * kHeadDim + 16 * quarter + 8 * pg) = w;
   if (p.lse && pg == 0 && quarter == 0) p.lse[orow] = any ? (all + __log2f(den)) * kLn2 : -INFINITY;
 }
 
@@ -692,7 +693,7 @@ hipError_t launch_tree(const TreeParams &p, const bool fp8, hipStream_t st) {
 
 hipError_t launch_tree_merge(const TreeParams &p, hipStream_t st) {
   const int tile = tree_tile_tokens(p.max_q_len);
-  tree_merge_kernel<<<(unsigned)(p.ranges * p.num_kv_heads * (tile / 2)), 256, 0, st>>>(p, tile);
+  tree_merge_kernel<<<(unsigned)(p.ranges * p.num_kv_heads * (tile / 4)), 256, 0, st>>>(p, tile);
   return hipGetLastError();
 }
 
