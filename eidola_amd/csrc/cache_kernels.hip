@@ -190,20 +190,29 @@ __global__ __launch_bounds__(kScoreWaves * 64) void score_rows_kernel(const Scor
 
 // ---------------------------------------------------------------------------------------
 // Rows to keep.  A workgroup per (sequence, KV head) finds the score of the last row that stays
-// by radix selection over order-preserving keys (8 bits a pass; sixteen copies of the histogram,
-// so that lanes with equal digits do not queue on one address), then writes the rows in order.
+// by radix selection over order-preserving keys, 8 bits a pass, then writes the rows in order: a
+// thread counts a run of consecutive rows, one scan over the workgroup gives it its places.
+//
+// Sequences of up to 32 rows per thread are read once, into LDS (four words of padding after every
+// 32 keep the threads' runs on different banks), and all passes work there; longer ones are read
+// again by every pass.  Eight copies of the histogram: lanes with equal digits, the usual case in
+// the first pass, do not queue on one address.
 // ---------------------------------------------------------------------------------------
-constexpr int kSelThreads = 1024;
 // larger = kept first; NaN lowest, -0 = +0
 __device__ __forceinline__ uint32_t order_key(const float x) {
   if (x != x) return 0u;
   const uint32_t u = __float_as_uint(x == 0.f ? 0.f : x);
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
+constexpr int kSelRun = 32;  // rows per thread of the LDS path
+constexpr int kSelCopies = 8;
 
-__global__ __launch_bounds__(kSelThreads) void select_kernel(const SelectParams p) {
-  __shared__ uint32_t hist[256 * 16];
-  __shared__ uint32_t wave_sum[kSelThreads / 64];
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void select_kernel(const SelectParams p) {
+  constexpr int kWaves = THREADS / 64, kCap = THREADS * kSelRun;
+  __shared__ __align__(16) uint32_t keys[kCap + kCap / 32 * 4];
+  __shared__ uint32_t hist[256 * kSelCopies];
+  __shared__ uint32_t wave_sum[kWaves];
   __shared__ uint32_t found[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int s = blockIdx.x / p.num_kv_heads, kvh = blockIdx.x % p.num_kv_heads;
@@ -212,31 +221,83 @@ __global__ __launch_bounds__(kSelThreads) void select_kernel(const SelectParams 
   int32_t *keep = p.keep + (size_t)blockIdx.x * budget;
   if (kvh == 0 && tid == 0) p.counts[s] = min(len, budget);
   if (len <= budget) {
-    for (int i = tid; i < budget; i += kSelThreads) keep[i] = i < len ? i : -1;
+    for (int i = tid; i < budget; i += THREADS) keep[i] = i < len ? i : -1;
     return;
   }
   const int32_t *bt = p.block_table + (size_t)s * p.max_blocks_per_seq;
   const int lo = p.keep_first, hi = len - p.keep_last;  // candidates: lo <= j < hi
-  auto key_at = [&](const int j) {
-    const int page = clamp_id(bt[j / kBlock], p.last_block);
-    return order_key(p.scores[((size_t)page * p.num_kv_heads + kvh) * kBlock + (j & 15)]);
+  const int quads = (len + 3) / 4;                      // four rows of one page
+  const bool in_lds = len <= kCap;
+  auto page_of = [&](const int q) { return clamp_id(bt[min(q, quads - 1) >> 2], p.last_block); };
+  auto quad_at = [&](const int page, const int q) {
+    return *(const f32x4 *)(p.scores + ((size_t)page * p.num_kv_heads + kvh) * kBlock + 4 * (q & 3));
   };
+  auto slot = [](const int q) { return 4 * q + (q >> 3) * 4; };
+  // f(j, key) for the rows of all quads q = tid, tid + THREADS, ... (any order of the workgroup)
+  auto for_rows = [&](auto f) {
+    if (in_lds) {
+      for (int q = tid; q < quads; q += THREADS) {
+        const u32x4 k = *(const u32x4 *)&keys[slot(q)];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f(4 * q + e, k[e]);
+      }
+    } else {
+      for (int q0 = tid; q0 < quads; q0 += 4 * THREADS) {
+        int page[4];
+        f32x4 x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) page[i] = page_of(q0 + i * THREADS);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = quad_at(page[i], q0 + i * THREADS);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (q0 + i * THREADS < quads)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f(4 * (q0 + i * THREADS) + e, order_key(x[i][e]));
+      }
+    }
+  };
+  if (in_lds) {
+    constexpr int kQ = kSelRun / 4;
+    int page[kQ];
+    f32x4 x[kQ];
+#pragma unroll
+    for (int i = 0; i < kQ; ++i)
+      if (i * THREADS < quads) page[i] = page_of(tid + i * THREADS);
+#pragma unroll
+    for (int i = 0; i < kQ; ++i)
+      if (i * THREADS < quads) x[i] = quad_at(page[i], tid + i * THREADS);
+#pragma unroll
+    for (int i = 0; i < kQ; ++i)
+      if (tid + i * THREADS < quads) {
+        u32x4 k;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) k[e] = order_key(x[i][e]);
+        *(u32x4 *)&keys[slot(tid + i * THREADS)] = k;
+      }
+  }
+  for (int i = tid; i < 256 * kSelCopies; i += THREADS) hist[i] = 0;
+  __syncthreads();
+
   uint32_t want = (uint32_t)(budget - p.keep_first - p.keep_last);  // candidates to keep
   uint32_t prefix = 0;
   if (want > 0) {
     for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256 * 16; i += kSelThreads) hist[i] = 0;
-      __syncthreads();
-      for (int j = lo + tid; j < hi; j += kSelThreads) {
-        const uint32_t k = key_at(j);
-        if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8)))
-          atomicAdd(&hist[(k >> shift & 255) * 16 + (lane & 15)], 1u);
-      }
+      for_rows([&](const int j, const uint32_t k) {
+        if (j >= lo && j < hi && (shift == 24 || ((k ^ prefix) >> (shift + 8)) == 0))
+          atomicAdd(&hist[(k >> shift & 255) * kSelCopies + (lane & (kSelCopies - 1))], 1u);
+      });
       __syncthreads();
       // counts of the digits from the highest down: thread d holds digit 255 - d
       uint32_t n = 0;
-      if (tid < 256)
-        for (int c = 0; c < 16; ++c) n += hist[(255 - tid) * 16 + ((c + tid) & 15)];
+      if (tid < 256) {
+        uint32_t *h = &hist[(255 - tid) * kSelCopies];
+#pragma unroll
+        for (int c = 0; c < kSelCopies; ++c) {
+          n += h[c];
+          h[c] = 0;  // for the next pass
+        }
+      }
       uint32_t incl = n;
 #pragma unroll
       for (int d = 1; d < 64; d <<= 1) {
@@ -257,32 +318,66 @@ __global__ __launch_bounds__(kSelThreads) void select_kernel(const SelectParams 
       want -= found[1];
     }
   }
-  // keys above `prefix` stay, and the first `want` of those equal to it
+  for (int i = tid; i < p.keep_first; i += THREADS) keep[i] = i;
+  for (int i = tid; i < p.keep_last; i += THREADS) keep[budget - p.keep_last + i] = hi + i;
+  if (budget == p.keep_first + p.keep_last) return;
+  // keys above `prefix` stay, and the first `want` of those equal to it.  Blocks of kCap rows (one,
+  // where the rows are in LDS), a run of consecutive rows per thread.
   uint32_t base = (uint32_t)p.keep_first, ties = 0;  // rows written, ties passed
-  for (int i = tid; i < p.keep_first; i += kSelThreads) keep[i] = i;
-  if (budget > p.keep_first + p.keep_last) {
-    for (int j0 = lo; j0 < hi; j0 += kSelThreads) {
-      const int j = j0 + tid;
-      const uint32_t k = j < hi ? key_at(j) : 0u;
-      const bool above = j < hi && k > prefix, tie = j < hi && k == prefix;
-      const uint64_t ba = __ballot(above), bt2 = __ballot(tie);
-      const uint64_t below = (1ull << lane) - 1;
-      __syncthreads();
-      if (lane == 0) wave_sum[wave] = (uint32_t)__popcll(ba) | (uint32_t)__popcll(bt2) << 16;
-      __syncthreads();
-      uint32_t mine = 0, all = 0;
-      for (int w = 0; w < kSelThreads / 64; ++w) {
-        if (w < wave) mine += wave_sum[w];
-        all += wave_sum[w];
+  for (int q_base = 0; q_base < quads; q_base += kCap / 4) {
+    const int here = min(quads - q_base, kCap / 4);
+    const int run = (here + THREADS - 1) / THREADS;  // quads per thread
+    const int q0 = min(tid * run, here), q1 = min(q0 + run, here);
+    auto keys_of = [&](const int q) {
+      u32x4 k;
+      if (in_lds) {
+        k = *(const u32x4 *)&keys[slot(q)];
+      } else {
+        const f32x4 x = quad_at(page_of(q_base + q), q_base + q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) k[e] = order_key(x[e]);
       }
-      const uint32_t a = (mine & 0xFFFF) + (uint32_t)__popcll(ba & below);
-      const uint32_t t = ties + (mine >> 16) + (uint32_t)__popcll(bt2 & below);  // ties before this row
-      if (above || (tie && t < want)) keep[base + a + (min(t, want) - min(ties, want))] = j;
-      base += (all & 0xFFFF) + (min(ties + (all >> 16), want) - min(ties, want));
-      ties += all >> 16;
+      return k;
+    };
+    uint32_t count = 0;  // rows above in the low half, ties in the high half (at most kCap <= 32768 each)
+    for (int q = q0; q < q1; ++q) {
+      const u32x4 k = keys_of(q);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int j = 4 * (q_base + q) + e;
+        if (j >= lo && j < hi) count += k[e] > prefix ? 1u : k[e] == prefix ? 0x10000u : 0u;
+      }
     }
+    uint32_t incl = count;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint32_t o = __shfl_up(incl, d);
+      if (lane >= d) incl += o;
+    }
+    __syncthreads();  // (the last use of wave_sum)
+    if (lane == 63) wave_sum[wave] = incl;
+    __syncthreads();
+    uint32_t mine = incl - count, all = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      if (w < wave) mine += wave_sum[w];
+      all += wave_sum[w];
+    }
+    uint32_t t = ties + (mine >> 16);  // ties before this thread's run
+    uint32_t at = base + (mine & 0xFFFFu) + (min(t, want) - min(ties, want));
+    for (int q = q0; q < q1; ++q) {
+      const u32x4 k = keys_of(q);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int j = 4 * (q_base + q) + e;
+        if (j < lo || j >= hi) continue;
+        if (k[e] > prefix || (k[e] == prefix && t < want)) keep[at++] = j;
+        t += k[e] == prefix ? 1u : 0u;
+      }
+    }
+    base += (all & 0xFFFFu) + (min(ties + (all >> 16), want) - min(ties, want));
+    ties += all >> 16;
   }
-  for (int i = tid; i < p.keep_last; i += kSelThreads) keep[budget - p.keep_last + i] = hi + i;
 }
 
 // ---------------------------------------------------------------------------------------
@@ -386,7 +481,10 @@ hipError_t launch_score(const ScoreParams &p, const bool fp8, const bool few, co
 int score_few_rows() { return kScoreFewRows; }
 
 hipError_t launch_select(const SelectParams &p, hipStream_t st) {
-  select_kernel<<<(unsigned)(p.num_seqs * p.num_kv_heads), kSelThreads, 0, st>>>(p);
+  // small workgroups while the longest sequence fits them: three share a CU's LDS
+  const unsigned grid = (unsigned)(p.num_seqs * p.num_kv_heads);
+  if (p.max_kv_len <= 256 * kSelRun) select_kernel<256><<<grid, 256, 0, st>>>(p);
+  else select_kernel<1024><<<grid, 1024, 0, st>>>(p);
   return hipGetLastError();
 }
 

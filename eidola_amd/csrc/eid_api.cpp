@@ -1339,6 +1339,7 @@ int32_t eid_kv_select(const eid_attn_desc *desc, const float *scores, const int3
   p.budget = budget;
   p.keep_first = keep_first;
   p.keep_last = keep_last;
+  p.max_kv_len = desc->max_kv_len;
   const hipError_t e = eid::launch_select(p, static_cast<hipStream_t>(hip_stream));
   if (e != hipSuccess) return hip_fail(e, "kv_select launch");
   return EID_OK;

@@ -55,6 +55,7 @@ struct SelectParams {
   int32_t *counts;  // [num_seqs]
   int32_t num_seqs, num_kv_heads, max_blocks_per_seq, last_block;
   int32_t budget, keep_first, keep_last;
+  int32_t max_kv_len;  // expected longest sequence: chooses the kernel
 };
 
 constexpr int kCompactLayers = 64;  // layers per launch

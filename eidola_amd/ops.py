@@ -508,10 +508,10 @@ def _scale(t, name, geom):
         raise ValueError(f"{name} must be [num_kv_heads]")
 
 
-def _rows_desc(geom, block_table, num_blocks):
+def _rows_desc(geom, block_table, num_blocks, max_kv_len=1):
     """Descriptor for the operators over cached rows."""
     S = block_table.shape[0]
-    return make_desc(geom, num_seqs=S, num_q_tokens=max(S, 1), max_q_len=1, max_kv_len=1,
+    return make_desc(geom, num_seqs=S, num_q_tokens=max(S, 1), max_q_len=1, max_kv_len=max_kv_len,
                      max_blocks_per_seq=block_table.shape[1], num_blocks=num_blocks)
 
 
@@ -661,7 +661,7 @@ def kv_select(geom, scores, block_table, seq_lens, *, budget, keep_first=0, keep
         if counts.shape[0] != S:
             raise ValueError("counts must be [S]")
     _same_device(scores, block_table=block_table, seq_lens=seq_lens, keep=keep, counts=counts)
-    desc = _rows_desc(geom, block_table, scores.shape[0])
+    desc = _rows_desc(geom, block_table, scores.shape[0], max_kv_len)
     on, stream = _on(scores.device)
     with on:
         check(load_library().eid_kv_select(

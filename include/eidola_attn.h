@@ -364,8 +364,9 @@ int32_t eid_kv_score(const eid_attn_desc *desc, const void *q, const float *lse,
  *   scores   as eid_kv_score leaves them
  *   keep     [num_seqs, num_kv_heads, budget] int32, rows in ascending order; -1 behind counts[s]
  *   counts   [num_seqs] int32 = min(seq_lens[s], budget): sequences within the budget keep all
- * keep_first + keep_last <= budget.  Of desc only the geometry, num_seqs, max_blocks_per_seq and
- * num_blocks are read.  Reference counterpart: none.
+ * keep_first + keep_last <= budget.  Of desc only the geometry, num_seqs, max_blocks_per_seq,
+ * num_blocks and max_kv_len are read, the last to choose the kernel alone (longer sequences are
+ * selected as well, slower).  Reference counterpart: none.
  */
 int32_t eid_kv_select(const eid_attn_desc *desc, const float *scores, const int32_t *block_table,
                       const int32_t *seq_lens, int32_t budget, int32_t keep_first,
