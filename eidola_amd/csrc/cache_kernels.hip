@@ -190,13 +190,13 @@ __global__ __launch_bounds__(kScoreWaves * 64) void score_rows_kernel(const Scor
 
 // ---------------------------------------------------------------------------------------
 // Rows to keep.  A workgroup per (sequence, KV head) finds the score of the last row that stays
-// by radix selection over order-preserving keys, 8 bits a pass, then writes the rows in order: a
-// thread counts a run of consecutive rows, one scan over the workgroup gives it its places.
-//
-// Sequences of up to 32 rows per thread are read once, into LDS (four words of padding after every
-// 32 keep the threads' runs on different banks), and all passes work there; longer ones are read
-// again by every pass.  Eight copies of the histogram: lanes with equal digits, the usual case in
-// the first pass, do not queue on one address.
+// by radix selection over order-preserving keys, eleven bits a pass, then writes the rows in
+// order.  A thread holds a run of RUN consecutive rows as keys in its registers: the scores are
+// read once, every pass works on registers, and one scan over the workgroup gives each thread the
+// places of its rows.  Sequences beyond 32 rows per thread are walked in blocks of that size and
+// read again by every pass.  Four copies of the histogram: lanes with equal digits, the
+// usual case in the first pass, queue less on one address.  A pass whose digit is kept whole ends
+// the search.
 // ---------------------------------------------------------------------------------------
 // larger = kept first; NaN lowest, -0 = +0
 __device__ __forceinline__ uint32_t order_key(const float x) {
@@ -204,16 +204,15 @@ __device__ __forceinline__ uint32_t order_key(const float x) {
   const uint32_t u = __float_as_uint(x == 0.f ? 0.f : x);
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
-constexpr int kSelRun = 32;  // rows per thread of the LDS path
-constexpr int kSelCopies = 8;
+constexpr int kSelThreads = 1024;
+constexpr int kSelBins = 2048, kSelCopies = 4;
 
-template <int THREADS>
-__global__ __launch_bounds__(THREADS) void select_kernel(const SelectParams p) {
-  constexpr int kWaves = THREADS / 64, kCap = THREADS * kSelRun;
-  __shared__ __align__(16) uint32_t keys[kCap + kCap / 32 * 4];
-  __shared__ uint32_t hist[256 * kSelCopies];
+template <int RUN>
+__global__ __launch_bounds__(kSelThreads) void select_kernel(const SelectParams p) {
+  constexpr int THREADS = kSelThreads, kWaves = THREADS / 64, kCap = THREADS * RUN, kBins = kSelBins / THREADS;
+  __shared__ __align__(16) uint32_t hist[kSelBins * kSelCopies];
   __shared__ uint32_t wave_sum[kWaves];
-  __shared__ uint32_t found[2];
+  __shared__ uint32_t found[3];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int s = blockIdx.x / p.num_kv_heads, kvh = blockIdx.x % p.num_kv_heads;
   const int len = max(0, min(p.seq_lens[s], p.max_blocks_per_seq * kBlock));
@@ -226,128 +225,111 @@ __global__ __launch_bounds__(THREADS) void select_kernel(const SelectParams p) {
   }
   const int32_t *bt = p.block_table + (size_t)s * p.max_blocks_per_seq;
   const int lo = p.keep_first, hi = len - p.keep_last;  // candidates: lo <= j < hi
-  const int quads = (len + 3) / 4;                      // four rows of one page
-  const bool in_lds = len <= kCap;
-  auto page_of = [&](const int q) { return clamp_id(bt[min(q, quads - 1) >> 2], p.last_block); };
-  auto quad_at = [&](const int page, const int q) {
-    return *(const f32x4 *)(p.scores + ((size_t)page * p.num_kv_heads + kvh) * kBlock + 4 * (q & 3));
-  };
-  auto slot = [](const int q) { return 4 * q + (q >> 3) * 4; };
-  // f(j, key) for the rows of all quads q = tid, tid + THREADS, ... (any order of the workgroup)
-  auto for_rows = [&](auto f) {
-    if (in_lds) {
-      for (int q = tid; q < quads; q += THREADS) {
-        const u32x4 k = *(const u32x4 *)&keys[slot(q)];
+  const int last_page = (len - 1) / kBlock;
+  uint32_t key[RUN];
+  uint32_t cand;  // bit i: key[i] is a candidate
+  // the thread's rows of the block that starts at row j0
+  auto load = [&](const int j0) {
+    const int j = j0 + tid * RUN;
+    cand = 0;
+    if (j < hi && j + RUN > lo) {
+      const int from = max(lo - j, 0), to = min(hi - j, RUN);
+      cand = (to >= 32 ? ~0u : (1u << to) - 1) & ~((1u << from) - 1);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) f(4 * q + e, k[e]);
-      }
-    } else {
-      for (int q0 = tid; q0 < quads; q0 += 4 * THREADS) {
-        int page[4];
-        f32x4 x[4];
+      for (int h = 0; h < (RUN + kBlock - 1) / kBlock; ++h) {
+        const int page = clamp_id(bt[min(j / kBlock + h, last_page)], p.last_block);
+        const f32x4 *src = (const f32x4 *)(p.scores + ((size_t)page * p.num_kv_heads + kvh) * kBlock + j % kBlock);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) page[i] = page_of(q0 + i * THREADS);
+        for (int q = 0; q < (RUN < kBlock ? RUN : kBlock) / 4; ++q) {
+          const f32x4 x = src[q];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = quad_at(page[i], q0 + i * THREADS);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (q0 + i * THREADS < quads)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) f(4 * (q0 + i * THREADS) + e, order_key(x[i][e]));
+          for (int e = 0; e < 4; ++e) key[kBlock * h + 4 * q + e] = order_key(x[e]);
+        }
       }
     }
   };
-  if (in_lds) {
-    constexpr int kQ = kSelRun / 4;
-    int page[kQ];
-    f32x4 x[kQ];
-#pragma unroll
-    for (int i = 0; i < kQ; ++i)
-      if (i * THREADS < quads) page[i] = page_of(tid + i * THREADS);
-#pragma unroll
-    for (int i = 0; i < kQ; ++i)
-      if (i * THREADS < quads) x[i] = quad_at(page[i], tid + i * THREADS);
-#pragma unroll
-    for (int i = 0; i < kQ; ++i)
-      if (tid + i * THREADS < quads) {
-        u32x4 k;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) k[e] = order_key(x[i][e]);
-        *(u32x4 *)&keys[slot(tid + i * THREADS)] = k;
-      }
-  }
-  for (int i = tid; i < 256 * kSelCopies; i += THREADS) hist[i] = 0;
+  const bool once = len <= kCap;
+  if (once) load(0);
+  for (int i = tid; i < kSelBins * kSelCopies; i += THREADS) hist[i] = 0;
   __syncthreads();
 
   uint32_t want = (uint32_t)(budget - p.keep_first - p.keep_last);  // candidates to keep
-  uint32_t prefix = 0;
+  uint32_t cut = 0;    // the digits found so far
+  bool whole = false;  // every key equal to `cut` in the bits searched stays
+  int shift = 21;
   if (want > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for_rows([&](const int j, const uint32_t k) {
-        if (j >= lo && j < hi && (shift == 24 || ((k ^ prefix) >> (shift + 8)) == 0))
-          atomicAdd(&hist[(k >> shift & 255) * kSelCopies + (lane & (kSelCopies - 1))], 1u);
-      });
-      __syncthreads();
-      // counts of the digits from the highest down: thread d holds digit 255 - d
-      uint32_t n = 0;
-      if (tid < 256) {
-        uint32_t *h = &hist[(255 - tid) * kSelCopies];
+    for (int pass = 0; pass < 3; ++pass) {
+      shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+      const uint32_t digits = pass < 2 ? 2047u : 1023u;
+      for (int j0 = 0; j0 < len; j0 += kCap) {
+        if (!once) load(j0);
 #pragma unroll
-        for (int c = 0; c < kSelCopies; ++c) {
-          n += h[c];
-          h[c] = 0;  // for the next pass
-        }
+        for (int i = 0; i < RUN; ++i)
+          if ((cand >> i & 1) && (pass == 0 || ((key[i] ^ cut) & ~(digits << shift)) >> shift == 0))
+            atomicAdd(&hist[(key[i] >> shift & digits) * kSelCopies + (lane & (kSelCopies - 1))], 1u);
       }
-      uint32_t incl = n;
+      __syncthreads();
+      // counts from the highest digit down: thread d holds digits (last - d kBins) .. of kBins bins
+      uint32_t n[kBins], sum = 0;
+#pragma unroll
+      for (int c = 0; c < kBins; ++c) {
+        u32x4 *h = (u32x4 *)&hist[(kSelBins - 1 - (tid * kBins + c)) * kSelCopies];
+        const u32x4 x = *h;
+        *h = u32x4{0, 0, 0, 0};  // for the next pass
+        n[c] = x[0] + x[1] + x[2] + x[3];
+        sum += n[c];
+      }
+      uint32_t incl = sum;
 #pragma unroll
       for (int d = 1; d < 64; d <<= 1) {
         const uint32_t o = __shfl_up(incl, d);
         if (lane >= d) incl += o;
       }
-      if (tid < 256 && lane == 63) wave_sum[wave] = incl;
+      if (lane == 63) wave_sum[wave] = incl;
       __syncthreads();
-      if (tid < 256) {
-        for (int w = 0; w < wave; ++w) incl += wave_sum[w];
-        if (incl >= want && incl - n < want) {
-          found[0] = (uint32_t)(255 - tid);
-          found[1] = incl - n;  // candidates above this digit
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w)
+        if (w < wave) incl += wave_sum[w];
+      uint32_t above = incl - sum;  // candidates with a higher digit
+#pragma unroll
+      for (int c = 0; c < kBins; ++c) {
+        if (above < want && above + n[c] >= want) {
+          found[0] = (uint32_t)(kSelBins - 1 - (tid * kBins + c));
+          found[1] = above;
+          found[2] = n[c];
         }
+        above += n[c];
       }
       __syncthreads();
-      prefix |= found[0] << shift;
+      cut |= found[0] << shift;
       want -= found[1];
+      whole = found[2] == want;
+      if (whole) break;
+      __syncthreads();  // (found is read before the next pass writes it)
     }
   }
   for (int i = tid; i < p.keep_first; i += THREADS) keep[i] = i;
   for (int i = tid; i < p.keep_last; i += THREADS) keep[budget - p.keep_last + i] = hi + i;
   if (budget == p.keep_first + p.keep_last) return;
-  // keys above `prefix` stay, and the first `want` of those equal to it.  Blocks of kCap rows (one,
-  // where the rows are in LDS), a run of consecutive rows per thread.
+  // Keys whose searched bits are above those of `cut` stay; of those equal to it all (`whole`), or
+  // the first `want`.
+  const uint32_t edge = cut >> shift;
   uint32_t base = (uint32_t)p.keep_first, ties = 0;  // rows written, ties passed
-  for (int q_base = 0; q_base < quads; q_base += kCap / 4) {
-    const int here = min(quads - q_base, kCap / 4);
-    const int run = (here + THREADS - 1) / THREADS;  // quads per thread
-    const int q0 = min(tid * run, here), q1 = min(q0 + run, here);
-    auto keys_of = [&](const int q) {
-      u32x4 k;
-      if (in_lds) {
-        k = *(const u32x4 *)&keys[slot(q)];
-      } else {
-        const f32x4 x = quad_at(page_of(q_base + q), q_base + q);
+  for (int j0 = 0; j0 < len; j0 += kCap) {
+    if (!once) load(j0);
+    uint32_t stay = 0, tie = 0;  // bits of the thread's rows
+    if (cand) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) k[e] = order_key(x[e]);
+      for (int i = 0; i < RUN; ++i) {
+        const uint32_t k = key[i] >> shift;
+        stay |= (k > edge || (whole && k == edge) ? 1u : 0u) << i;
+        tie |= (!whole && k == edge ? 1u : 0u) << i;
       }
-      return k;
-    };
-    uint32_t count = 0;  // rows above in the low half, ties in the high half (at most kCap <= 32768 each)
-    for (int q = q0; q < q1; ++q) {
-      const u32x4 k = keys_of(q);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int j = 4 * (q_base + q) + e;
-        if (j >= lo && j < hi) count += k[e] > prefix ? 1u : k[e] == prefix ? 0x10000u : 0u;
-      }
+      stay &= cand;
+      tie &= cand;
     }
+    // rows that stay in the low half, ties in the high half (at most kCap <= 32768 each)
+    const uint32_t count = (uint32_t)__popc(stay) | (uint32_t)__popc(tie) << 16;
     uint32_t incl = count;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -363,18 +345,13 @@ __global__ __launch_bounds__(THREADS) void select_kernel(const SelectParams p) {
       if (w < wave) mine += wave_sum[w];
       all += wave_sum[w];
     }
-    uint32_t t = ties + (mine >> 16);  // ties before this thread's run
+    const uint32_t t = ties + (mine >> 16);  // ties before this thread's run
     uint32_t at = base + (mine & 0xFFFFu) + (min(t, want) - min(ties, want));
-    for (int q = q0; q < q1; ++q) {
-      const u32x4 k = keys_of(q);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int j = 4 * (q_base + q) + e;
-        if (j < lo || j >= hi) continue;
-        if (k[e] > prefix || (k[e] == prefix && t < want)) keep[at++] = j;
-        t += k[e] == prefix ? 1u : 0u;
-      }
+    for (uint32_t room = want > t ? want - t : 0; tie && room; --room) {  // the run's first ties
+      stay |= tie & (0u - tie);
+      tie &= tie - 1;
     }
+    for (const int j = j0 + tid * RUN; stay; stay &= stay - 1) keep[at++] = j + __builtin_ctz(stay);
     base += (all & 0xFFFFu) + (min(ties + (all >> 16), want) - min(ties, want));
     ties += all >> 16;
   }
@@ -481,10 +458,11 @@ hipError_t launch_score(const ScoreParams &p, const bool fp8, const bool few, co
 int score_few_rows() { return kScoreFewRows; }
 
 hipError_t launch_select(const SelectParams &p, hipStream_t st) {
-  // small workgroups while the longest sequence fits them: three share a CU's LDS
+  // rows per thread: as few as hold the longest sequence
   const unsigned grid = (unsigned)(p.num_seqs * p.num_kv_heads);
-  if (p.max_kv_len <= 256 * kSelRun) select_kernel<256><<<grid, 256, 0, st>>>(p);
-  else select_kernel<1024><<<grid, 1024, 0, st>>>(p);
+  if (p.max_kv_len <= kSelThreads * 4) select_kernel<4><<<grid, kSelThreads, 0, st>>>(p);
+  else if (p.max_kv_len <= kSelThreads * 16) select_kernel<16><<<grid, kSelThreads, 0, st>>>(p);
+  else select_kernel<32><<<grid, kSelThreads, 0, st>>>(p);
   return hipGetLastError();
 }
 
