@@ -103,7 +103,8 @@ class BatchInfo(C.Structure):
 
 EXPORTS = ("eid_kv_write", "eid_rope_kv_write", "eid_qkv_rope_kv_write", "eid_attn_decode",
            "eid_attn_decode_noalloc", "eid_attn_varlen", "eid_lse_merge", "eid_o_proj",
-           "eid_attn_tree", "eid_attn_tree_workspace_bytes", "eid_kv_score", "eid_kv_select",
+           "eid_attn_tree", "eid_attn_tree_workspace_bytes", "eid_kv_score",
+           "eid_kv_score_workspace_bytes", "eid_kv_select",
            "eid_kv_compact", "eid_workspace_bytes", "eid_partition_size", "eid_last_error", "eid_version")
 # only in the measurement build (include/eidola_attn_measure.h)
 MEASURE_EXPORTS = ("eid_debug_set_timeline", "eid_debug_set_kernel_events",
@@ -173,8 +174,10 @@ def _bind(path, measure):
     lib.eid_attn_tree.restype = C.c_int32
     lib.eid_attn_tree_workspace_bytes.argtypes = [C.POINTER(AttnDesc)]
     lib.eid_attn_tree_workspace_bytes.restype = C.c_size_t
-    lib.eid_kv_score.argtypes = [C.POINTER(AttnDesc), P, P, P, P, P, P, P, P, P]
+    lib.eid_kv_score.argtypes = [C.POINTER(AttnDesc), P, P, P, P, P, P, P, P, P, C.c_size_t, P]
     lib.eid_kv_score.restype = C.c_int32
+    lib.eid_kv_score_workspace_bytes.argtypes = [C.POINTER(AttnDesc)]
+    lib.eid_kv_score_workspace_bytes.restype = C.c_size_t
     lib.eid_kv_select.argtypes = [C.POINTER(AttnDesc), P, P, P, C.c_int32, C.c_int32, C.c_int32, P, P, P]
     lib.eid_kv_select.restype = C.c_int32
     lib.eid_kv_compact.argtypes = [C.POINTER(AttnDesc), C.c_int32, P, P, P, P, P, P, C.c_int64, C.c_int64,

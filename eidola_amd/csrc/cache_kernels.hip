@@ -19,7 +19,7 @@ __device__ __forceinline__ ScoreSeq score_seq(const ScoreParams &p, const int s)
   const const_i32_ptr cu = as_constant(p.cu_seqlens_q), sl = as_constant(p.seq_lens);
   v.row0 = cu[s];
   v.qlen = cu[s + 1] - v.row0;
-  v.len = min(sl[s], p.max_blocks_per_seq * kBlock);
+  v.len = min(sl[s], p.max_kv_len);
   if (v.qlen < 0 || v.len < v.qlen || v.row0 < 0 || v.row0 + v.qlen > p.num_q_tokens) v.qlen = 0;
   return v;
 }
@@ -71,7 +71,14 @@ __device__ __forceinline__ float weights(const Frag8 (&qf)[2], const Frag8 (&kf)
   return see ? w : 0.f;
 }
 
-constexpr int kScoreFewRows = 2;  // q_len that the few-rows kernel takes
+// score of key j, new from `prefix` on
+__device__ __forceinline__ void add_score(const ScoreParams &p, const int s, const int kvh, const int j,
+                                          const int prefix, const float w) {
+  const int page = clamp_id(p.block_table[(size_t)s * p.max_blocks_per_seq + j / kBlock], p.last_block);
+  float *dst = p.scores + ((size_t)page * p.num_kv_heads + kvh) * kBlock + (j & 15);
+  *dst = (j >= prefix ? 0.f : *dst) + w;
+}
+
 
 // ---------------------------------------------------------------------------------------
 // score[j] = (key j is new ? 0 : score[j]) + sum over rows i and the group's heads of
@@ -120,72 +127,104 @@ __global__ __launch_bounds__(512) void score_few_kernel(const ScoreParams p) {
 }
 
 // ---------------------------------------------------------------------------------------
-// Sequences of more rows: bound by the products and exponentials.  A workgroup owns 64 KT keys of
-// one KV head (held as operands by every wave) and its waves share out the rows; no two
-// workgroups touch one key, so the sums need no atomics and have one order.
+// Sequences of more rows: bound by the exponentials and products.  A workgroup owns 128 keys of one
+// KV head (held as operands by each of its four waves) and every parts-th row pair per wave; one
+// lane adds up one key's weights, so the sums need no atomics and have one order.  With parts > 1
+// a workgroup's sums go to the workspace and score_join_kernel adds the parts up: a few key tiles
+// alone do not fill the device, and the tiles that see the causal edge have less to do.
+//
+// A stage is one 16-key page: its two matrix instructions are issued a stage ahead of its four
+// (multiply-add, exponential, add) per lane.
 // ---------------------------------------------------------------------------------------
-constexpr int kScoreWaves = 8;
-constexpr int kScorePages = 8;  // pages of keys per workgroup
 template <bool FP8>
-__global__ __launch_bounds__(kScoreWaves * 64) void score_rows_kernel(const ScoreParams p) {
+__global__ __launch_bounds__(kScoreWaves * 64, 3) void score_rows_kernel(const ScoreParams p) {
   const int lane = threadIdx.x & 63, i16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int kvh = blockIdx.x % p.num_kv_heads, tc = blockIdx.x / p.num_kv_heads * (kScorePages * kBlock);
-  const int s = blockIdx.y;
+  const int kvh = blockIdx.x % p.num_kv_heads, tc = blockIdx.x / p.num_kv_heads * kScoreKeys;
+  const int s = blockIdx.y, part = blockIdx.z;
   const ScoreSeq v = score_seq(p, s);
   if (v.qlen <= kScoreFewRows || tc >= v.len) return;
-  __shared__ float part[kScoreWaves][kScorePages * kBlock];
+  __shared__ float sums[kScoreWaves][kScoreKeys];
   const int prefix = v.len - v.qlen;
   const const_i32_ptr bt = as_constant(p.block_table + (size_t)s * p.max_blocks_per_seq);
   const int last_page = (v.len - 1) / kBlock;
   const uint32_t row_bytes = (uint32_t)p.num_kv_heads * kHeadDim * (FP8 ? 1 : 2);
   const float c2 = p.softmax_scale * kLog2e * (FP8 ? p.k_scale[kvh] : 1.0f);
-  Frag8 kf[kScorePages][2];
+  constexpr int kPages = kScoreKeys / kBlock;
+  // rows that see any of these keys: positions tc .. key_end - 1 + window - 1
+  const int key_end = min(tc + kScoreKeys, v.len);
+  const int i0 = max(0, tc - prefix) & ~1;
+  int i1 = v.qlen;
+  if (p.window > 0) i1 = (int)min((long long)i1, (long long)key_end - 1 + p.window - prefix);
+  const int stride = 2 * kScoreWaves * p.parts;
+  const int first = i0 + 2 * (wave + kScoreWaves * part);
+
+  Frag8 kf[kPages][2], qf[2], qn[2];
+  f32x4 off, off_n;
 #pragma unroll
-  for (int b = 0; b < kScorePages; ++b) {
+  for (int b = 0; b < kPages; ++b) {
     const int page = clamp_id(bt[min(tc / kBlock + b, last_page)], p.last_block);
     load_k<FP8>(p.k_cache + (size_t)page * kBlock * row_bytes + (size_t)kvh * kHeadDim * (FP8 ? 1 : 2), row_bytes, kf[b]);
   }
-  const int key_end = min(tc + kScorePages * kBlock, v.len);
-  // rows that see any of these keys: positions tc .. key_end - 1 + window - 1
-  int i0 = max(0, tc - prefix) & ~1;
-  int i1 = v.qlen;
-  if (p.window > 0) i1 = (int)min((long long)i1, (long long)key_end - 1 + p.window - prefix);
-  float sum[kScorePages];
+  load_rows(p, v, kvh, first, qf, off);
+  float sum[kPages];
 #pragma unroll
-  for (int b = 0; b < kScorePages; ++b) sum[b] = 0.f;
-  for (int i = i0 + 2 * wave; i < i1; i += 2 * kScoreWaves) {
-    Frag8 qf[2];
-    f32x4 off;
-    load_rows(p, v, kvh, i, qf, off);
+  for (int b = 0; b < kPages; ++b) sum[b] = 0.f;
+  for (int i = first; i < i1; i += stride) {
+    load_rows(p, v, kvh, i + stride, qn, off_n);  // (rows past the end: none)
     const int pos = prefix + i + (g >> 1);
     const bool edge = prefix + i < key_end - 1 || (p.window > 0 && prefix + i + 1 - tc >= p.window);
-    if (edge) {
+    f32x4 S[2];
+    S[0] = mfma16x32(qf[0], kf[0][0], f32x4{0.f, 0.f, 0.f, 0.f});
+    S[0] = mfma16x32(qf[1], kf[0][1], S[0]);
 #pragma unroll
-      for (int b = 0; b < kScorePages; ++b) {
-        const int j = tc + b * kBlock + i16;
-        sum[b] += weights(qf, kf[b], off, c2, j <= pos && (p.window <= 0 || pos - j < p.window));
+    for (int b = 0; b < kPages; ++b) {
+      if (b + 1 < kPages) {
+        S[(b + 1) & 1] = mfma16x32(qf[0], kf[b + 1][0], f32x4{0.f, 0.f, 0.f, 0.f});
+        S[(b + 1) & 1] = mfma16x32(qf[1], kf[b + 1][1], S[(b + 1) & 1]);
       }
-    } else {
+      float w[4];
 #pragma unroll
-      for (int b = 0; b < kScorePages; ++b) sum[b] += weights(qf, kf[b], off, c2, true);
+      for (int r = 0; r < 4; ++r) w[r] = fast_exp2(__builtin_fmaf(S[b & 1][r], c2, -off[r]));
+      float add = (w[0] + w[1]) + (w[2] + w[3]);
+      if (edge) {
+        const int j = tc + b * kBlock + i16;
+        add = j <= pos && (p.window <= 0 || pos - j < p.window) ? add : 0.f;
+      }
+      sum[b] += add;
     }
+    qf[0] = qn[0];
+    qf[1] = qn[1];
+    off = off_n;
   }
 #pragma unroll
-  for (int b = 0; b < kScorePages; ++b) {
+  for (int b = 0; b < kPages; ++b) {
     const float w = rowgroup_sum(sum[b]);
-    if (g == 0) part[wave][b * kBlock + i16] = w;
+    if (g == 0) sums[wave][b * kBlock + i16] = w;
   }
   __syncthreads();
   const int x = threadIdx.x;
-  if (x < kScorePages * kBlock && tc + x < v.len) {
+  if (x < kScoreKeys && tc + x < v.len) {
     float w = 0.f;
 #pragma unroll
-    for (int k = 0; k < kScoreWaves; ++k) w += part[k][x];
-    const int page = clamp_id(p.block_table[(size_t)s * p.max_blocks_per_seq + (tc + x) / kBlock], p.last_block);
-    float *dst = p.scores + ((size_t)page * p.num_kv_heads + kvh) * kBlock + (x & 15);
-    *dst = (tc + x >= prefix ? 0.f : *dst) + w;
+    for (int k = 0; k < kScoreWaves; ++k) w += sums[k][x];
+    if (p.parts > 1) {
+      p.ws[(((size_t)part * p.num_seqs + s) * p.num_kv_heads + kvh) * p.tile_keys + tc + x] = w;
+    } else {
+      add_score(p, s, kvh, tc + x, prefix, w);
+    }
   }
+}
+
+// Adds the parts of the rows kernel up, part after part.  grid = (keys / 256, KV heads, sequences).
+__global__ __launch_bounds__(256) void score_join_kernel(const ScoreParams p) {
+  const int s = blockIdx.z, kvh = blockIdx.y, j = blockIdx.x * 256 + threadIdx.x;
+  const ScoreSeq v = score_seq(p, s);
+  if (v.qlen <= kScoreFewRows || j >= v.len) return;
+  float w = 0.f;
+  for (int part = 0; part < p.parts; ++part)
+    w += p.ws[(((size_t)part * p.num_seqs + s) * p.num_kv_heads + kvh) * p.tile_keys + j];
+  add_score(p, s, kvh, j, v.len - v.qlen, w);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -446,16 +485,16 @@ hipError_t launch_score(const ScoreParams &p, const bool fp8, const bool few, co
     if (e != hipSuccess) return e;
   }
   if (many) {
-    constexpr int keys = kScorePages * kBlock;
-    const dim3 grid((unsigned)((p.max_kv_len + keys - 1) / keys) * (unsigned)p.num_kv_heads, (unsigned)p.num_seqs);
+    const dim3 grid((unsigned)(p.tile_keys / kScoreKeys) * (unsigned)p.num_kv_heads, (unsigned)p.num_seqs, (unsigned)p.parts);
     if (fp8) score_rows_kernel<true><<<grid, kScoreWaves * 64, 0, st>>>(p);
     else score_rows_kernel<false><<<grid, kScoreWaves * 64, 0, st>>>(p);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || p.parts == 1) return e;
+    score_join_kernel<<<dim3((unsigned)(p.max_kv_len + 255) / 256, (unsigned)p.num_kv_heads, (unsigned)p.num_seqs), 256, 0, st>>>(p);
     return hipGetLastError();
   }
   return hipSuccess;
 }
-
-int score_few_rows() { return kScoreFewRows; }
 
 hipError_t launch_select(const SelectParams &p, hipStream_t st) {
   // rows per thread: as few as hold the longest sequence

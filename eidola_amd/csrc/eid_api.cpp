@@ -57,7 +57,6 @@ hipError_t launch_kv_write(const uint16_t *k_new, const uint16_t *v_new, uint8_t
 int tree_tile_tokens(int max_q_len);
 hipError_t launch_tree(const TreeParams &p, bool fp8, hipStream_t st);
 hipError_t launch_tree_merge(const TreeParams &p, hipStream_t st);
-int score_few_rows();
 hipError_t launch_score(const ScoreParams &p, bool fp8, bool few, bool many, hipStream_t st);
 hipError_t launch_select(const SelectParams &p, hipStream_t st);
 hipError_t launch_compact(const CompactParams &p, int num_layers, hipStream_t st);
@@ -1194,6 +1193,38 @@ int32_t check_rows_desc(const eid_attn_desc *d) {
   return EID_OK;
 }
 
+int32_t check_score_desc(const eid_attn_desc *d) {
+  if (int32_t rc = check_attn_desc(d)) return rc;
+  if (((long long)d->max_kv_len / eid::kScoreKeys + 1) * d->num_kv_heads > 0x3fffffffLL)
+    return fail(EID_ERR_UNSUPPORTED, "max_kv_len %d with %d KV heads is too large", d->max_kv_len, d->num_kv_heads);
+  return EID_OK;
+}
+
+struct ScorePlan {
+  int32_t parts, tile_keys;
+  size_t ws_bytes;  // 0: none needed
+};
+
+// How many workgroups share the rows of a key tile.  A CU holds three workgroups; with two or
+// three times as many of them as places the tiles that see few rows even out.  A part keeps at least
+// eight row pairs per wave, so that loading the keys pays.
+ScorePlan make_score_plan(const eid_attn_desc *d) {
+  ScorePlan pl;
+  const long long tiles = ((long long)d->max_kv_len + eid::kScoreKeys - 1) / eid::kScoreKeys;
+  pl.tile_keys = (int32_t)(tiles * eid::kScoreKeys > 0x7fffffffLL ? 0x7fffffff : tiles * eid::kScoreKeys);
+  pl.parts = 1;
+  pl.ws_bytes = 0;
+  if (d->max_q_len <= eid::kScoreFewRows) return pl;
+  const long long keys = d->sum_kv_len ? d->sum_kv_len : (long long)d->num_seqs * d->max_kv_len;
+  const long long wgs = (keys / eid::kScoreKeys + d->num_seqs) * d->num_kv_heads;
+  const long long by_fill = 8LL * eid::device_cus() / std::max(1LL, wgs);
+  const long long by_rows = d->max_q_len / (2 * eid::kScoreWaves * 8);
+  pl.parts = (int32_t)std::max(1LL, std::min({by_fill, by_rows, (long long)eid::kScorePartsMax}));
+  if (pl.parts > 1)
+    pl.ws_bytes = (size_t)pl.parts * d->num_seqs * d->num_kv_heads * (size_t)pl.tile_keys * sizeof(float);
+  return pl;
+}
+
 int32_t last_block_of(const eid_attn_desc *d) { return (int32_t)std::min<int64_t>(d->num_blocks - 1, 0x7fffffff); }
 
 }  // namespace
@@ -1273,17 +1304,29 @@ int32_t eid_attn_tree(const eid_attn_desc *desc, const eid_attn_args *args, cons
 }
 
 // ---- thinning a cache out ------------------------------------------------------------------
+size_t eid_kv_score_workspace_bytes(const eid_attn_desc *desc) {
+  if (check_score_desc(desc)) return 0;
+  return make_score_plan(desc).ws_bytes;
+}
+
 int32_t eid_kv_score(const eid_attn_desc *desc, const void *q, const float *lse, const void *k_cache,
                      const int32_t *block_table, const int32_t *cu_seqlens_q, const int32_t *seq_lens,
-                     const float *k_scale, float *scores, void *hip_stream) {
+                     const float *k_scale, float *scores, void *workspace, size_t workspace_bytes,
+                     void *hip_stream) {
   g_err[0] = 0;
-  if (int32_t rc = check_attn_desc(desc)) return rc;
+  if (int32_t rc = check_score_desc(desc)) return rc;
   if (!q || !lse || !k_cache || !block_table || !cu_seqlens_q || !seq_lens || !scores)
     return fail(EID_ERR_INVALID_ARG, "q, lse, k_cache, block_table, cu_seqlens_q, seq_lens and scores must be non-NULL");
   if (!aligned16(q) || !aligned16(lse) || !aligned16(k_cache) || !aligned16(scores))
     return fail(EID_ERR_INVALID_ARG, "q, lse, k_cache and scores must be 16-byte aligned");
   const bool fp8 = desc->kv_dtype == EID_KV_FP8_E4M3;
   if (fp8 && !k_scale) return fail(EID_ERR_INVALID_ARG, "fp8 KV needs k_scale");
+  const ScorePlan pl = make_score_plan(desc);
+  if (pl.ws_bytes > 0 && (!workspace || workspace_bytes < pl.ws_bytes))
+    return fail(EID_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", pl.ws_bytes,
+                workspace ? workspace_bytes : (size_t)0);
+  if (pl.ws_bytes > 0 && (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
+    return fail(EID_ERR_WORKSPACE, "workspace must be 256-byte aligned");
   eid::ScoreParams p;
   std::memset(&p, 0, sizeof p);
   p.q = static_cast<const uint16_t *>(q);
@@ -1294,6 +1337,9 @@ int32_t eid_kv_score(const eid_attn_desc *desc, const void *q, const float *lse,
   p.seq_lens = seq_lens;
   p.k_scale = k_scale;
   p.scores = scores;
+  p.parts = pl.parts;
+  p.tile_keys = pl.tile_keys;
+  p.ws = static_cast<float *>(workspace);
   p.num_seqs = desc->num_seqs;
   p.num_q_heads = desc->num_q_heads;
   p.num_kv_heads = desc->num_kv_heads;
@@ -1307,7 +1353,7 @@ int32_t eid_kv_score(const eid_attn_desc *desc, const void *q, const float *lse,
   // Sequences are sorted into two classes by their rows on the device; when every sequence has
   // max_q_len rows (num_q_tokens says so) only one of them is populated.
   const bool uniform = (int64_t)desc->num_seqs * desc->max_q_len == desc->num_q_tokens;
-  const bool many = desc->max_q_len > eid::score_few_rows();
+  const bool many = desc->max_q_len > eid::kScoreFewRows;
   const hipError_t e = eid::launch_score(p, fp8, !many || !uniform, many, static_cast<hipStream_t>(hip_stream));
   if (e != hipSuccess) return hip_fail(e, "kv_score launch");
   return EID_OK;

@@ -36,6 +36,11 @@ struct TreeParams {
   float softmax_scale;
 };
 
+constexpr int kScoreFewRows = 2;   // q_len that the few-rows kernel takes
+constexpr int kScoreWaves = 4;     // of a workgroup of the rows kernel
+constexpr int kScoreKeys = 128;    // keys of a workgroup of the rows kernel
+constexpr int kScorePartsMax = 16;
+
 struct ScoreParams {
   const uint16_t *q;
   const float *lse;
@@ -45,6 +50,9 @@ struct ScoreParams {
   float *scores;         // [num_blocks][Hkv][16]
   int32_t num_seqs, num_q_heads, num_kv_heads, max_blocks_per_seq, last_block;
   int32_t num_q_tokens, window, max_q_len, max_kv_len;
+  int32_t parts;      // the rows kernel's rows are shared out over so many workgroups
+  int32_t tile_keys;  // max_kv_len, in whole key tiles
+  float *ws;          // [parts][num_seqs][Hkv][tile_keys], parts > 1 only
   float softmax_scale;
 };
 

@@ -598,10 +598,11 @@ def _scores_pool(t, name, geom, num_blocks):
 
 
 def kv_score(geom, q, lse, k_cache, block_table, seq_lens, cu_seqlens_q, scores, *, max_q_len, max_kv_len,
-             k_scale=None, sum_kv_len=0):
+             k_scale=None, sum_kv_len=0, workspace=None):
     """Adds the attention weight that every cached key receives from this step's rows to `scores`
     ([num_blocks, num_kv_heads, 16] fp32, paged like the caches; the step's own keys start from 0).
-    `lse` is what the step's attention call returned.  Returns `scores`."""
+    `lse` is what the step's attention call returned.  Returns `scores`.  `workspace`: a uint8
+    tensor of kv_score_workspace_bytes, for callers that keep one (one call at a time)."""
     _require(q, "q", torch.bfloat16, 3)
     _require(lse, "lse", torch.float32, 2)
     k_cache = _cache_view(k_cache, geom, "k_cache")
@@ -619,16 +620,28 @@ def kv_score(geom, q, lse, k_cache, block_table, seq_lens, cu_seqlens_q, scores,
     if geom.kv_dtype == KV_FP8_E4M3:
         _scale(k_scale, "k_scale", geom)
     _same_device(q, lse=lse, k_cache=k_cache, block_table=block_table, seq_lens=seq_lens, cu_seqlens_q=cu_seqlens_q,
-                 scores=scores, k_scale=k_scale)
+                 scores=scores, k_scale=k_scale, workspace=workspace)
     desc = make_desc(geom, num_seqs=S, num_q_tokens=T, max_q_len=max_q_len, max_kv_len=max_kv_len,
                      max_blocks_per_seq=block_table.shape[1], num_blocks=k_cache.shape[0], sum_kv_len=sum_kv_len)
+    lib = load_library()
     on, stream = _on(q.device)
     with on:
-        check(load_library().eid_kv_score(
+        if workspace is None:
+            need = lib.eid_kv_score_workspace_bytes(C.byref(desc))
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        elif not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous")
+        check(lib.eid_kv_score(
             C.byref(desc), q.data_ptr(), lse.data_ptr(), k_cache.data_ptr(), block_table.data_ptr(),
             cu_seqlens_q.data_ptr(), seq_lens.data_ptr(), k_scale.data_ptr() if k_scale is not None else None,
-            scores.data_ptr(), stream))
+            scores.data_ptr(), workspace.data_ptr() if workspace is not None else None,
+            workspace.numel() * workspace.element_size() if workspace is not None else 0, stream))
     return scores
+
+
+def kv_score_workspace_bytes(desc):
+    """Bytes of workspace kv_score needs (0: none)."""
+    return load_library().eid_kv_score_workspace_bytes(C.byref(desc))
 
 
 def kv_select(geom, scores, block_table, seq_lens, *, budget, keep_first=0, keep_last=0, max_kv_len, keep=None,

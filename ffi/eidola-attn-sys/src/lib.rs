@@ -199,8 +199,12 @@ unsafe extern "C" {
         seq_lens: *const i32,
         k_scale: *const f32,
         scores: *mut f32,
+        workspace: *mut c_void,
+        workspace_bytes: usize,
         hip_stream: *mut c_void,
     ) -> i32;
+
+    pub fn eid_kv_score_workspace_bytes(desc: *const eid_attn_desc) -> usize;
 
     pub fn eid_kv_select(
         desc: *const eid_attn_desc,

@@ -358,6 +358,8 @@ pub unsafe fn kv_score(
     seq_lens: *const i32,
     k_scale: Option<*const f32>,
     scores: *mut f32,
+    workspace: *mut c_void,
+    workspace_bytes: usize,
     stream: *mut c_void,
 ) -> Result<(), AttnError> {
     check(unsafe {
@@ -371,9 +373,17 @@ pub unsafe fn kv_score(
             seq_lens,
             k_scale.unwrap_or(ptr::null()),
             scores,
+            workspace,
+            workspace_bytes,
             stream,
         )
     })
+}
+
+/// Bytes of workspace `kv_score` needs (0: none; `workspace` may then be null).
+pub fn kv_score_workspace_bytes(desc: &sys::eid_attn_desc) -> usize {
+    // SAFETY: desc is a valid reference; planning touches no device memory.
+    unsafe { sys::eid_kv_score_workspace_bytes(desc) }
 }
 
 /// The rows that stay when caches are cut to `budget` rows per KV head.

@@ -355,7 +355,11 @@ size_t eid_attn_tree_workspace_bytes(const eid_attn_desc *desc);
 int32_t eid_kv_score(const eid_attn_desc *desc, const void *q, const float *lse,
                      const void *k_cache, const int32_t *block_table,
                      const int32_t *cu_seqlens_q, const int32_t *seq_lens, const float *k_scale,
-                     float *scores, void *hip_stream);
+                     float *scores, void *workspace, size_t workspace_bytes, void *hip_stream);
+
+/* Bytes of workspace eid_kv_score needs for desc; 0 when it needs none (workspace may then be
+ * NULL), or for an invalid desc. */
+size_t eid_kv_score_workspace_bytes(const eid_attn_desc *desc);
 
 /*
  * Which rows of a sequence stay when its cache is cut to `budget` rows, per KV head: the first

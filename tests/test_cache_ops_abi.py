@@ -80,14 +80,21 @@ def test_tree_workspace_follows_the_bounds():
 
 def test_score_refusals():
     lib, ok = ea.load_library(), 0x1000
-    call = lambda d, q=ok, lse=ok, k=ok, bt=ok, cu=ok, sl=ok, ks=None, w=ok: lib.eid_kv_score(
-        C.byref(d) if d else None, q, lse, k, bt, cu, sl, ks, w, None)
+    call = lambda d, q=ok, lse=ok, k=ok, bt=ok, cu=ok, sl=ok, ks=None, w=ok, ws=None, n=0: lib.eid_kv_score(
+        C.byref(d) if d else None, q, lse, k, bt, cu, sl, ks, w, ws, n, None)
     assert call(None) == BAD and call(desc(head_dim=32)) == UNSUP and call(desc(max_kv_len=0)) == BAD
     for f in ("q", "lse", "k", "bt", "cu", "sl", "w"):
         assert call(desc(), **{f: None}) == BAD
     for f in ("q", "lse", "k", "w"):
         assert call(desc(), **{f: 0x1004}) == BAD
     assert call(desc(kv_dtype=ea.KV_FP8_E4M3)) == BAD
+    # a long chunk whose rows are shared out needs a workspace; few rows do not
+    assert ea.kv_score_workspace_bytes(desc()) == 0 and ea.kv_score_workspace_bytes(desc(num_seqs=0)) == 0
+    long = desc(num_seqs=1, num_q_tokens=512, max_q_len=512)
+    need = ea.kv_score_workspace_bytes(long)
+    assert need > 0 and call(long) == WS and call(long, ws=0x2000, n=need - 1) == WS
+    assert call(long, ws=0x2010, n=need) == WS
+    assert ea.kv_score_workspace_bytes(desc(num_seqs=512, num_q_tokens=512 * 512, max_q_len=512)) == 0
 
 
 def test_select_refusals():
