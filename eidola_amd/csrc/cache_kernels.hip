@@ -3,6 +3,8 @@
 #include "eid_cache_params.h"
 #include "eid_device.h"
 
+#include <type_traits>
+
 namespace eid {
 
 namespace {
@@ -160,42 +162,66 @@ __global__ __launch_bounds__(kScoreWaves * 64, 3) void score_rows_kernel(const S
   const int first = i0 + 2 * (wave + kScoreWaves * part);
 
   Frag8 kf[kPages][2], qf[2], qn[2];
-  f32x4 off, off_n;
+  f32x4 e, en;  // lse of the rows, as they stand
 #pragma unroll
   for (int b = 0; b < kPages; ++b) {
     const int page = clamp_id(bt[min(tc / kBlock + b, last_page)], p.last_block);
     load_k<FP8>(p.k_cache + (size_t)page * kBlock * row_bytes + (size_t)kvh * kHeadDim * (FP8 ? 1 : 2), row_bytes, kf[b]);
   }
-  load_rows(p, v, kvh, first, qf, off);
+  // row pair from token i on; tokens past the end repeat the last (their weights are dropped)
+  const uint16_t *q_lane = p.q + ((size_t)v.row0 * p.num_q_heads + kvh * kGroup + (i16 & 7)) * kHeadDim + 16 * g;
+  const float *e_lane = p.lse + (size_t)v.row0 * p.num_q_heads + kvh * kGroup + 4 * (g & 1);
+  auto fetch = [&](const int i, Frag8 (&q)[2], f32x4 &x) {
+    const uint16_t *src = q_lane + (size_t)min(i + (i16 >> 3), v.qlen - 1) * p.num_q_heads * kHeadDim;
+    q[0].u = *(const u32x4 *)src;
+    q[1].u = *(const u32x4 *)(src + 8);
+    x = *(const f32x4 *)(e_lane + (size_t)min(i + (g >> 1), v.qlen - 1) * p.num_q_heads);
+  };
   float sum[kPages];
 #pragma unroll
   for (int b = 0; b < kPages; ++b) sum[b] = 0.f;
-  for (int i = first; i < i1; i += stride) {
-    load_rows(p, v, kvh, i + stride, qn, off_n);  // (rows past the end: none)
+  auto pair = [&](auto edge_c, const int i) {
+    constexpr bool EDGE = decltype(edge_c)::value;
+    // what the exponents take off, in log2 units; a row that saw nothing (-inf) has no weights
+    f32x4 off;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) off[r] = e[r] == -INFINITY ? -INFINITY : -kLog2e * e[r];
     const int pos = prefix + i + (g >> 1);
-    const bool edge = prefix + i < key_end - 1 || (p.window > 0 && prefix + i + 1 - tc >= p.window);
-    f32x4 S[2];
-    S[0] = mfma16x32(qf[0], kf[0][0], f32x4{0.f, 0.f, 0.f, 0.f});
-    S[0] = mfma16x32(qf[1], kf[0][1], S[0]);
+    if (EDGE && i + (g >> 1) >= v.qlen) off = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    f32x4 S[3];
+    auto first_half = [&](const int b) { S[b % 3] = mfma16x32(qf[0], kf[b][0], f32x4{0.f, 0.f, 0.f, 0.f}); };
+    auto second_half = [&](const int b) { S[b % 3] = mfma16x32(qf[1], kf[b][1], S[b % 3]); };
+    first_half(0);
+    first_half(1);
+    second_half(0);
 #pragma unroll
     for (int b = 0; b < kPages; ++b) {
-      if (b + 1 < kPages) {
-        S[(b + 1) & 1] = mfma16x32(qf[0], kf[b + 1][0], f32x4{0.f, 0.f, 0.f, 0.f});
-        S[(b + 1) & 1] = mfma16x32(qf[1], kf[b + 1][1], S[(b + 1) & 1]);
-      }
       float w[4];
+      __builtin_amdgcn_sched_barrier(0);
+      if (b + 1 < kPages) second_half(b + 1);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) w[r] = fast_exp2(__builtin_fmaf(S[b & 1][r], c2, -off[r]));
+      for (int r = 0; r < 2; ++r) w[r] = fast_exp2(__builtin_fmaf(S[b % 3][r], c2, off[r]));
+      __builtin_amdgcn_sched_barrier(0);
+      if (b + 2 < kPages) first_half(b + 2);
+#pragma unroll
+      for (int r = 2; r < 4; ++r) w[r] = fast_exp2(__builtin_fmaf(S[b % 3][r], c2, off[r]));
       float add = (w[0] + w[1]) + (w[2] + w[3]);
-      if (edge) {
+      if constexpr (EDGE) {
         const int j = tc + b * kBlock + i16;
         add = j <= pos && (p.window <= 0 || pos - j < p.window) ? add : 0.f;
       }
       sum[b] += add;
     }
+  };
+  if (first < i1) fetch(first, qf, e);
+  for (int i = first; i < i1; i += stride) {
+    fetch(i + stride, qn, en);
+    const bool edge = prefix + i < key_end - 1 || (p.window > 0 && prefix + i + 1 - tc >= p.window) || i + 1 >= v.qlen;
+    if (edge) pair(std::true_type{}, i);
+    else pair(std::false_type{}, i);
     qf[0] = qn[0];
     qf[1] = qn[1];
-    off = off_n;
+    e = en;
   }
 #pragma unroll
   for (int b = 0; b < kPages; ++b) {
