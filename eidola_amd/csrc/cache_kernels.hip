@@ -26,32 +26,35 @@ __device__ __forceinline__ ScoreSeq score_seq(const ScoreParams &p, const int s)
   return v;
 }
 
-// K operand of 16 keys (one page) of a head: lane (key i16, segment g) holds elements 16 g .. 16 g + 15
+// K operand of 16 keys (one page) of a head: lane (key i16, segment g) holds elements 8 g .. 8 g + 7
+// and 32 + 8 g .. 32 + 8 g + 7: a load instruction covers 64 consecutive bytes of each row.  An fp8
+// row is half as long, one load: elements 16 g .. 16 g + 15.  q is read in the same order.
 template <bool FP8>
 __device__ __forceinline__ void load_k(const uint8_t *base, const uint32_t row_bytes, Frag8 (&kf)[2]) {
   const int lane = threadIdx.x & 63, i16 = lane & 15, g = lane >> 4;
-  const uint8_t *src = base + (uint32_t)i16 * row_bytes + g * (FP8 ? 16 : 32);
+  const uint8_t *src = base + (uint32_t)i16 * row_bytes + g * 16;
   if constexpr (FP8) {
-    const u32x4 r = *(const u32x4 *)src;
+    const u32x4 r = __builtin_nontemporal_load((const u32x4 *)src);
     fp8x8_to_bf16x8(r[0], r[1], kf[0].w);
     fp8x8_to_bf16x8(r[2], r[3], kf[1].w);
   } else {
-    kf[0].u = *(const u32x4 *)src;
-    kf[1].u = *(const u32x4 *)(src + 16);
+    kf[0].u = __builtin_nontemporal_load((const u32x4 *)src);
+    kf[1].u = __builtin_nontemporal_load((const u32x4 *)(src + 64));
   }
 }
 
 // 16 rows of q (two tokens x 8 heads) from token `tok` of the sequence on, and what the rows'
 // exponents take off: lse in log2 units; +inf where there is no row (its weights are then 0).
+template <bool FP8>
 __device__ __forceinline__ void load_rows(const ScoreParams &p, const ScoreSeq &v, const int kvh, const int tok,
                                           Frag8 (&qf)[2], f32x4 &off) {
   const int lane = threadIdx.x & 63, i16 = lane & 15, g = lane >> 4;
   const int tq = tok + (i16 >> 3), tl = tok + (g >> 1);
   qf[0].u = qf[1].u = u32x4{0, 0, 0, 0};
   if (tq < v.qlen) {
-    const uint16_t *src = p.q + ((size_t)(v.row0 + tq) * p.num_q_heads + kvh * kGroup + (i16 & 7)) * kHeadDim + 16 * g;
+    const uint16_t *src = p.q + ((size_t)(v.row0 + tq) * p.num_q_heads + kvh * kGroup + (i16 & 7)) * kHeadDim + (FP8 ? 16 : 8) * g;
     qf[0].u = *(const u32x4 *)src;
-    qf[1].u = *(const u32x4 *)(src + 8);
+    qf[1].u = *(const u32x4 *)(src + (FP8 ? 8 : 32));
   }
   off = f32x4{INFINITY, INFINITY, INFINITY, INFINITY};
   if (tl < v.qlen) {
@@ -82,6 +85,11 @@ __device__ __forceinline__ void add_score(const ScoreParams &p, const int s, con
 }
 
 
+// Keys below `key_end` that no row of the sequence has in its window, none of them new: their scores stay.
+__device__ __forceinline__ bool below_window(const ScoreParams &p, const int prefix, const int key_end) {
+  return p.window > 0 && key_end <= prefix - p.window + 1;
+}
+
 // ---------------------------------------------------------------------------------------
 // score[j] = (key j is new ? 0 : score[j]) + sum over rows i and the group's heads of
 // vis(i, j) e^(c q.k_j - lse_i).
@@ -99,6 +107,7 @@ __global__ __launch_bounds__(512) void score_few_kernel(const ScoreParams p) {
   const int tc = blockIdx.x * kChunk;
   if (v.qlen < 1 || v.qlen > kScoreFewRows || tc >= v.len || kvh >= p.num_kv_heads) return;
   const int prefix = v.len - v.qlen;
+  if (below_window(p, prefix, tc + kChunk)) return;
   const const_i32_ptr bt = as_constant(p.block_table + (size_t)s * p.max_blocks_per_seq);
   const int last_page = (v.len - 1) / kBlock;
   const uint32_t row_bytes = (uint32_t)p.num_kv_heads * kHeadDim * (FP8 ? 1 : 2);
@@ -111,29 +120,30 @@ __global__ __launch_bounds__(512) void score_few_kernel(const ScoreParams p) {
 #pragma unroll
   for (int b = 0; b < 4; ++b)
     load_k<FP8>(p.k_cache + (size_t)page[b] * kBlock * row_bytes + (size_t)kvh * kHeadDim * (FP8 ? 1 : 2), row_bytes, kf[b]);
-  load_rows(p, v, kvh, 0, qf, off);
-  float mine = 0.f;
+  load_rows<FP8>(p, v, kvh, 0, qf, off);
+  // lane (i16, g) keeps key i16 of page g
+  const int mine = tc + g * kBlock + i16;
+  const int pg = g == 0 ? page[0] : g == 1 ? page[1] : g == 2 ? page[2] : page[3];
+  float *dst = p.scores + ((size_t)pg * p.num_kv_heads + kvh) * kBlock + i16;
+  const float old = mine < prefix ? *dst : 0.f;
+  float sum = 0.f;
 #pragma unroll
   for (int b = 0; b < 4; ++b) {
     const int j = tc + b * kBlock + i16, pos = prefix + (g >> 1);
     const bool see = j <= pos && (p.window <= 0 || pos - j < p.window);
     const float w = rowgroup_sum(weights(qf, kf[b], off, c2, see));
-    mine = g == b ? w : mine;  // lane (i16, g) keeps key i16 of page g
+    sum = g == b ? w : sum;
   }
-  const int j = tc + g * kBlock + i16;
-  if (j < v.len) {
-    const int pg = g == 0 ? page[0] : g == 1 ? page[1] : g == 2 ? page[2] : page[3];
-    float *dst = p.scores + ((size_t)pg * p.num_kv_heads + kvh) * kBlock + i16;
-    *dst = (j >= prefix ? 0.f : *dst) + mine;
-  }
+  if (mine < v.len) *dst = old + sum;
 }
 
 // ---------------------------------------------------------------------------------------
-// Sequences of more rows: bound by the exponentials and products.  A workgroup owns 128 keys of one
-// KV head (held as operands by each of its four waves) and every parts-th row pair per wave; one
-// lane adds up one key's weights, so the sums need no atomics and have one order.  With parts > 1
-// a workgroup's sums go to the workspace and score_join_kernel adds the parts up: a few key tiles
-// alone do not fill the device, and the tiles that see the causal edge have less to do.
+// Sequences of more rows: bound by the exponentials and products.  A wave holds 128 keys of one KV
+// head as operands and walks row pairs; one lane adds up one key's weights, so the sums need no
+// atomics and have one order.  The four waves of a workgroup hold neighbouring keys and walk the
+// same rows, which the CU's cache then reads once.  With parts > 1 a workgroup takes every
+// parts-th row pair, its sums go to the workspace and score_join_kernel adds the parts up: a few key
+// tiles alone do not fill the device, and the tiles that see the causal edge have less to do.
 //
 // A stage is one 16-key page: its two matrix instructions are issued a stage ahead of its four
 // (multiply-add, exponential, add) per lane.
@@ -142,12 +152,12 @@ template <bool FP8>
 __global__ __launch_bounds__(kScoreWaves * 64, 3) void score_rows_kernel(const ScoreParams p) {
   const int lane = threadIdx.x & 63, i16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int kvh = blockIdx.x % p.num_kv_heads, tc = blockIdx.x / p.num_kv_heads * kScoreKeys;
+  const int kvh = blockIdx.x % p.num_kv_heads;
+  const int tc = (blockIdx.x / p.num_kv_heads * kScoreWaves + wave) * kScoreKeys;
   const int s = blockIdx.y, part = blockIdx.z;
   const ScoreSeq v = score_seq(p, s);
-  if (v.qlen <= kScoreFewRows || tc >= v.len) return;
-  __shared__ float sums[kScoreWaves][kScoreKeys];
   const int prefix = v.len - v.qlen;
+  if (v.qlen <= kScoreFewRows || tc >= v.len || below_window(p, prefix, tc + kScoreKeys)) return;
   const const_i32_ptr bt = as_constant(p.block_table + (size_t)s * p.max_blocks_per_seq);
   const int last_page = (v.len - 1) / kBlock;
   const uint32_t row_bytes = (uint32_t)p.num_kv_heads * kHeadDim * (FP8 ? 1 : 2);
@@ -158,8 +168,8 @@ __global__ __launch_bounds__(kScoreWaves * 64, 3) void score_rows_kernel(const S
   const int i0 = max(0, tc - prefix) & ~1;
   int i1 = v.qlen;
   if (p.window > 0) i1 = (int)min((long long)i1, (long long)key_end - 1 + p.window - prefix);
-  const int stride = 2 * kScoreWaves * p.parts;
-  const int first = i0 + 2 * (wave + kScoreWaves * part);
+  const int stride = 2 * p.parts;
+  const int first = i0 + 2 * part;
 
   Frag8 kf[kPages][2], qf[2], qn[2];
   f32x4 e, en;  // lse of the rows, as they stand
@@ -169,12 +179,12 @@ __global__ __launch_bounds__(kScoreWaves * 64, 3) void score_rows_kernel(const S
     load_k<FP8>(p.k_cache + (size_t)page * kBlock * row_bytes + (size_t)kvh * kHeadDim * (FP8 ? 1 : 2), row_bytes, kf[b]);
   }
   // row pair from token i on; tokens past the end repeat the last (their weights are dropped)
-  const uint16_t *q_lane = p.q + ((size_t)v.row0 * p.num_q_heads + kvh * kGroup + (i16 & 7)) * kHeadDim + 16 * g;
+  const uint16_t *q_lane = p.q + ((size_t)v.row0 * p.num_q_heads + kvh * kGroup + (i16 & 7)) * kHeadDim + (FP8 ? 16 : 8) * g;
   const float *e_lane = p.lse + (size_t)v.row0 * p.num_q_heads + kvh * kGroup + 4 * (g & 1);
   auto fetch = [&](const int i, Frag8 (&q)[2], f32x4 &x) {
     const uint16_t *src = q_lane + (size_t)min(i + (i16 >> 3), v.qlen - 1) * p.num_q_heads * kHeadDim;
     q[0].u = *(const u32x4 *)src;
-    q[1].u = *(const u32x4 *)(src + 8);
+    q[1].u = *(const u32x4 *)(src + (FP8 ? 8 : 32));
     x = *(const f32x4 *)(e_lane + (size_t)min(i + (g >> 1), v.qlen - 1) * p.num_q_heads);
   };
   float sum[kPages];
@@ -223,22 +233,19 @@ __global__ __launch_bounds__(kScoreWaves * 64, 3) void score_rows_kernel(const S
     qf[1] = qn[1];
     e = en;
   }
+  // lane (i16, g) keeps key i16 of pages g and 4 + g
 #pragma unroll
-  for (int b = 0; b < kPages; ++b) {
-    const float w = rowgroup_sum(sum[b]);
-    if (g == 0) sums[wave][b * kBlock + i16] = w;
-  }
-  __syncthreads();
-  const int x = threadIdx.x;
-  if (x < kScoreKeys && tc + x < v.len) {
+  for (int h = 0; h < 2; ++h) {
     float w = 0.f;
 #pragma unroll
-    for (int k = 0; k < kScoreWaves; ++k) w += sums[k][x];
-    if (p.parts > 1) {
-      p.ws[(((size_t)part * p.num_seqs + s) * p.num_kv_heads + kvh) * p.tile_keys + tc + x] = w;
-    } else {
-      add_score(p, s, kvh, tc + x, prefix, w);
+    for (int b = 0; b < 4; ++b) {
+      const float x = rowgroup_sum(sum[4 * h + b]);
+      w = g == b ? x : w;
     }
+    const int j = tc + (4 * h + g) * kBlock + i16;
+    if (j >= v.len) continue;
+    if (p.parts > 1) p.ws[(((size_t)part * p.num_seqs + s) * p.num_kv_heads + kvh) * p.tile_keys + j] = w;
+    else add_score(p, s, kvh, j, prefix, w);
   }
 }
 
@@ -246,10 +253,17 @@ __global__ __launch_bounds__(kScoreWaves * 64, 3) void score_rows_kernel(const S
 __global__ __launch_bounds__(256) void score_join_kernel(const ScoreParams p) {
   const int s = blockIdx.z, kvh = blockIdx.y, j = blockIdx.x * 256 + threadIdx.x;
   const ScoreSeq v = score_seq(p, s);
-  if (v.qlen <= kScoreFewRows || j >= v.len) return;
+  if (v.qlen <= kScoreFewRows || j >= v.len || below_window(p, v.len - v.qlen, j + 1)) return;
+  const float *src = p.ws + ((size_t)s * p.num_kv_heads + kvh) * p.tile_keys + j;
+  const size_t step = (size_t)p.num_seqs * p.num_kv_heads * p.tile_keys;
   float w = 0.f;
-  for (int part = 0; part < p.parts; ++part)
-    w += p.ws[(((size_t)part * p.num_seqs + s) * p.num_kv_heads + kvh) * p.tile_keys + j];
+  for (int part = 0; part < p.parts; part += 8) {  // eight loads under way, added in order
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = src[min(part + i, p.parts - 1) * step];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w += part + i < p.parts ? x[i] : 0.f;
+  }
   add_score(p, s, kvh, j, v.len - v.qlen, w);
 }
 
@@ -511,7 +525,8 @@ hipError_t launch_score(const ScoreParams &p, const bool fp8, const bool few, co
     if (e != hipSuccess) return e;
   }
   if (many) {
-    const dim3 grid((unsigned)(p.tile_keys / kScoreKeys) * (unsigned)p.num_kv_heads, (unsigned)p.num_seqs, (unsigned)p.parts);
+    const dim3 grid((unsigned)(p.tile_keys / (kScoreWaves * kScoreKeys)) * (unsigned)p.num_kv_heads, (unsigned)p.num_seqs,
+                    (unsigned)p.parts);
     if (fp8) score_rows_kernel<true><<<grid, kScoreWaves * 64, 0, st>>>(p);
     else score_rows_kernel<false><<<grid, kScoreWaves * 64, 0, st>>>(p);
     const hipError_t e = hipGetLastError();

@@ -1195,30 +1195,33 @@ int32_t check_rows_desc(const eid_attn_desc *d) {
 
 int32_t check_score_desc(const eid_attn_desc *d) {
   if (int32_t rc = check_attn_desc(d)) return rc;
-  if (((long long)d->max_kv_len / eid::kScoreKeys + 1) * d->num_kv_heads > 0x3fffffffLL)
+  if (d->max_kv_len > 0x7fff0000 || ((long long)d->max_kv_len / eid::kScoreKeys + 1) * d->num_kv_heads > 0x3fffffffLL)
     return fail(EID_ERR_UNSUPPORTED, "max_kv_len %d with %d KV heads is too large", d->max_kv_len, d->num_kv_heads);
   return EID_OK;
 }
+
+constexpr long long kScoreFill = 8;  // workgroups per CU that the parts aim at
 
 struct ScorePlan {
   int32_t parts, tile_keys;
   size_t ws_bytes;  // 0: none needed
 };
 
-// How many workgroups share the rows of a key tile.  A CU holds three workgroups; with two or
-// three times as many of them as places the tiles that see few rows even out.  A part keeps at least
-// eight row pairs per wave, so that loading the keys pays.
+// How many workgroups share the rows of a key tile.  A CU holds three workgroups; with several
+// times as many of them as places the tiles that see few rows even out.  A part keeps at least eight
+// row pairs, so that loading the keys pays.
 ScorePlan make_score_plan(const eid_attn_desc *d) {
   ScorePlan pl;
-  const long long tiles = ((long long)d->max_kv_len + eid::kScoreKeys - 1) / eid::kScoreKeys;
-  pl.tile_keys = (int32_t)(tiles * eid::kScoreKeys > 0x7fffffffLL ? 0x7fffffff : tiles * eid::kScoreKeys);
+  constexpr long long wg_keys = eid::kScoreWaves * eid::kScoreKeys;
+  const long long tiles = (d->max_kv_len + wg_keys - 1) / wg_keys;
+  pl.tile_keys = (int32_t)std::min(tiles * wg_keys, 0x7fffffffLL / wg_keys * wg_keys);
   pl.parts = 1;
   pl.ws_bytes = 0;
   if (d->max_q_len <= eid::kScoreFewRows) return pl;
   const long long keys = d->sum_kv_len ? d->sum_kv_len : (long long)d->num_seqs * d->max_kv_len;
-  const long long wgs = (keys / eid::kScoreKeys + d->num_seqs) * d->num_kv_heads;
-  const long long by_fill = 8LL * eid::device_cus() / std::max(1LL, wgs);
-  const long long by_rows = d->max_q_len / (2 * eid::kScoreWaves * 8);
+  const long long wgs = (keys / wg_keys + d->num_seqs) * d->num_kv_heads;
+  const long long by_fill = kScoreFill * eid::device_cus() / std::max(1LL, wgs);
+  const long long by_rows = d->max_q_len / 16;
   pl.parts = (int32_t)std::max(1LL, std::min({by_fill, by_rows, (long long)eid::kScorePartsMax}));
   if (pl.parts > 1)
     pl.ws_bytes = (size_t)pl.parts * d->num_seqs * d->num_kv_heads * (size_t)pl.tile_keys * sizeof(float);

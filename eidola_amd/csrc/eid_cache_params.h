@@ -38,8 +38,8 @@ struct TreeParams {
 
 constexpr int kScoreFewRows = 2;   // q_len that the few-rows kernel takes
 constexpr int kScoreWaves = 4;     // of a workgroup of the rows kernel
-constexpr int kScoreKeys = 128;    // keys of a workgroup of the rows kernel
-constexpr int kScorePartsMax = 16;
+constexpr int kScoreKeys = 128;    // keys of a wave of the rows kernel
+constexpr int kScorePartsMax = 64;
 
 struct ScoreParams {
   const uint16_t *q;
@@ -51,7 +51,7 @@ struct ScoreParams {
   int32_t num_seqs, num_q_heads, num_kv_heads, max_blocks_per_seq, last_block;
   int32_t num_q_tokens, window, max_q_len, max_kv_len;
   int32_t parts;      // the rows kernel's rows are shared out over so many workgroups
-  int32_t tile_keys;  // max_kv_len, in whole key tiles
+  int32_t tile_keys;  // max_kv_len, in whole workgroups' keys
   float *ws;          // [parts][num_seqs][Hkv][tile_keys], parts > 1 only
   float softmax_scale;
 };
