@@ -491,28 +491,63 @@ def lse_merge(geom, workspace, seq_lens, cu_seqlens_q, *, num_q_tokens, max_q_le
     return out
 
 
-def _on(device):
-    """The device's current stream, with the device made current for the launch."""
-    return torch.cuda.device(device), C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+# The operators below check their tensors in one expression each (a Python check of its own for every
+# property of every tensor would cost more than the kernels of a small batch); what fails there is looked
+# at property by property to name it.
+
+def _fits(t, dtype, device, shape):
+    return t.dtype is dtype and t.get_device() == device and t.shape == shape and t.is_contiguous()
 
 
-def _same_device(first, **others):
-    for name, t in others.items():
-        if t is not None and t.device != first.device:
-            raise ValueError(f"{name} is on {t.device}, not on {first.device}")
+def _need(t, name, dtype, device, shape):
+    """Raises unless `t` is a contiguous tensor of that type and shape on that GPU."""
+    if t is not None and _fits(t, dtype, device, shape):
+        return
+    _require(t, name, dtype, len(shape))
+    if t.get_device() != device:
+        raise ValueError(f"{name} is on {t.device}, not on GPU {device}")
+    raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
 
 
-def _scale(t, name, geom):
-    _require(t, name, torch.float32, 1)
-    if t.shape[0] != geom.num_kv_heads:
-        raise ValueError(f"{name} must be [num_kv_heads]")
+def _device_of(t, name):
+    """Index of the GPU that holds `t`: every other tensor of the call has to be there."""
+    if t is None or not t.is_cuda:
+        raise ValueError(f"{name} must be a GPU tensor")
+    return t.get_device()
 
 
-def _rows_desc(geom, block_table, num_blocks, max_kv_len=1):
+def _cache_shape(t, geom, name):
+    """(type, shape) that the caches of a call must have, from the first of them."""
+    if t is None or t.dim() != 4 or t.shape[1:] != (geom.block_size, geom.num_kv_heads, geom.head_dim):
+        _cache_view(t, geom, name)
+    dtype = torch.float8_e4m3fn if geom.kv_dtype == KV_FP8_E4M3 and t.dtype == torch.float8_e4m3fn \
+        else _kv_torch_dtype(geom.kv_dtype)
+    return dtype, t.shape
+
+
+def _launch(device, call):
+    """call(stream) on the device's current stream, with the device made current."""
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if torch.cuda.current_device() == device:
+        check(call(stream))
+    else:
+        with torch.cuda.device(device):
+            check(call(stream))
+
+
+def _workspace(t, need, device):
+    """The caller's workspace, checked, or one from the allocator; None where none is needed."""
+    if t is None:
+        return torch.empty(need, dtype=torch.uint8, device=f"cuda:{device}") if need else None
+    if t.get_device() != device or not t.is_contiguous():
+        raise ValueError(f"workspace must be a contiguous tensor on GPU {device}")
+    return t
+
+
+def _rows_desc(geom, S, max_blocks, num_blocks, max_kv_len=1):
     """Descriptor for the operators over cached rows."""
-    S = block_table.shape[0]
     return make_desc(geom, num_seqs=S, num_q_tokens=max(S, 1), max_q_len=1, max_kv_len=max_kv_len,
-                     max_blocks_per_seq=block_table.shape[1], num_blocks=num_blocks)
+                     max_blocks_per_seq=max_blocks, num_blocks=num_blocks)
 
 
 def attn_tree_workspace_bytes(desc):
@@ -527,74 +562,52 @@ def attn_tree(geom, q, k_cache, v_cache, block_table, seq_lens, cu_seqlens_q, tr
     the same sequence, at most 256 tokens).  The tokens' K/V rows stand in the cache behind the
     context (seq_lens counts them).  geom.window is measured in depths.  `workspace`: a uint8
     tensor of attn_tree_workspace_bytes, for callers that keep one (one call at a time)."""
-    _require(q, "q", torch.bfloat16, 3)
-    k_cache = _cache_view(k_cache, geom, "k_cache")
-    v_cache = _cache_view(v_cache, geom, "v_cache")
-    if k_cache.shape != v_cache.shape:
-        raise ValueError("k_cache and v_cache shapes differ")
-    _require(block_table, "block_table", torch.int32, 2)
-    _require(seq_lens, "seq_lens", torch.int32, 1)
-    _require(cu_seqlens_q, "cu_seqlens_q", torch.int32, 1)
-    _require(tree_mask, "tree_mask", torch.int64, 2)
-    S, T = seq_lens.shape[0], q.shape[0]
-    if tuple(q.shape[1:]) != (geom.num_q_heads, geom.head_dim):
-        raise ValueError("q must be [T, num_q_heads, head_dim]")
-    if block_table.shape[0] != S or cu_seqlens_q.shape[0] != S + 1:
-        raise ValueError("block_table must have one row per sequence, cu_seqlens_q one entry more")
-    if tree_mask.shape[0] != T:
-        raise ValueError("tree_mask must have one row per query token")
+    dev = _device_of(q, "q")
+    kv, cache_shape = _cache_shape(k_cache, geom, "k_cache")
+    if seq_lens is None or block_table is None or block_table.dim() != 2 or tree_mask is None or tree_mask.dim() != 2:
+        raise ValueError("seq_lens must be [S], block_table [S, max_blocks], tree_mask [T, words]")
+    T, S, f32, i32 = q.shape[0], seq_lens.shape[0], torch.float32, torch.int32
+    blocks, words = block_table.shape[1], tree_mask.shape[1]
+    Hq, Hkv = geom.num_q_heads, geom.num_kv_heads
+    q_shape = (T, Hq, geom.head_dim)
+    _need(q, "q", torch.bfloat16, dev, q_shape)
+    _need(k_cache, "k_cache", kv, dev, cache_shape)
+    _need(v_cache, "v_cache", kv, dev, cache_shape)
+    _need(block_table, "block_table", i32, dev, (S, blocks))
+    _need(seq_lens, "seq_lens", i32, dev, (S,))
+    _need(cu_seqlens_q, "cu_seqlens_q", i32, dev, (S + 1,))
+    _need(tree_mask, "tree_mask", torch.int64, dev, (T, words))
     if sinks is not None:
-        _require(sinks, "sinks", torch.float32, 1)
-        if sinks.shape[0] != geom.num_q_heads:
-            raise ValueError("sinks must be [num_q_heads]")
-    if geom.kv_dtype == KV_FP8_E4M3:
-        _scale(k_scale, "k_scale", geom)
-        _scale(v_scale, "v_scale", geom)
+        _need(sinks, "sinks", f32, dev, (Hq,))
+    fp8 = geom.kv_dtype == KV_FP8_E4M3
+    if fp8:
+        _need(k_scale, "k_scale", f32, dev, (Hkv,))
+        _need(v_scale, "v_scale", f32, dev, (Hkv,))
     if out is None:
         out = torch.empty_like(q)
     else:
-        _require(out, "out", torch.bfloat16, 3)
-        if out.shape != q.shape:
-            raise ValueError("out must have the shape of q")
-    if lse is None and return_lse:
-        lse = torch.empty((T, geom.num_q_heads), dtype=torch.float32, device=q.device)
-    elif lse is not None:
-        _require(lse, "lse", torch.float32, 2)
-        if tuple(lse.shape) != (T, geom.num_q_heads):
-            raise ValueError("lse must be [T, num_q_heads]")
-    _same_device(q, k_cache=k_cache, v_cache=v_cache, block_table=block_table, seq_lens=seq_lens,
-                 cu_seqlens_q=cu_seqlens_q, tree_mask=tree_mask, sinks=sinks, k_scale=k_scale, v_scale=v_scale,
-                 out=out, lse=lse, workspace=workspace)
+        _need(out, "out", torch.bfloat16, dev, q_shape)
+    if lse is not None:
+        _need(lse, "lse", f32, dev, (T, Hq))
+    elif return_lse:
+        lse = torch.empty((T, Hq), dtype=f32, device=q.device)
     desc = make_desc(geom, num_seqs=S, num_q_tokens=T, max_q_len=max_q_len, max_kv_len=max_kv_len,
-                     max_blocks_per_seq=block_table.shape[1], num_blocks=k_cache.shape[0], sum_kv_len=sum_kv_len)
-    lib = load_library()
-    on, stream = _on(q.device)
-    with on:
-        if workspace is None:
-            need = lib.eid_attn_tree_workspace_bytes(C.byref(desc))
-            workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-        args = AttnArgs()
-        args.q, args.out = q.data_ptr(), out.data_ptr()
-        args.lse = lse.data_ptr() if lse is not None else None
-        args.k_cache, args.v_cache = k_cache.data_ptr(), v_cache.data_ptr()
-        args.block_table, args.seq_lens = block_table.data_ptr(), seq_lens.data_ptr()
-        args.cu_seqlens_q = cu_seqlens_q.data_ptr()
-        args.sinks = sinks.data_ptr() if sinks is not None else None
-        args.k_scale = k_scale.data_ptr() if k_scale is not None else None
-        args.v_scale = v_scale.data_ptr() if v_scale is not None else None
-        if workspace is not None:
-            if not workspace.is_contiguous():
-                raise ValueError("workspace must be contiguous")
-            args.workspace = workspace.data_ptr()
-            args.workspace_bytes = workspace.numel() * workspace.element_size()
-        check(lib.eid_attn_tree(C.byref(desc), C.byref(args), tree_mask.data_ptr(), tree_mask.shape[1], stream))
+                     max_blocks_per_seq=blocks, num_blocks=cache_shape[0], sum_kv_len=sum_kv_len)
+    lib, ref = load_library(), C.byref(desc)
+    workspace = _workspace(workspace, lib.eid_attn_tree_workspace_bytes(ref), dev)
+    args = AttnArgs(q=q.data_ptr(), out=out.data_ptr(), k_cache=k_cache.data_ptr(), v_cache=v_cache.data_ptr(),
+                    block_table=block_table.data_ptr(), cu_seqlens_q=cu_seqlens_q.data_ptr(),
+                    seq_lens=seq_lens.data_ptr())
+    if lse is not None:
+        args.lse = lse.data_ptr()
+    if sinks is not None:
+        args.sinks = sinks.data_ptr()
+    if fp8:
+        args.k_scale, args.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
+    if workspace is not None:
+        args.workspace, args.workspace_bytes = workspace.data_ptr(), workspace.nbytes
+    _launch(dev, lambda stream: lib.eid_attn_tree(ref, C.byref(args), tree_mask.data_ptr(), words, stream))
     return (out, lse) if return_lse else out
-
-
-def _scores_pool(t, name, geom, num_blocks):
-    _require(t, name, torch.float32, 3)
-    if tuple(t.shape) != (num_blocks, geom.num_kv_heads, geom.block_size):
-        raise ValueError(f"{name} must be [{num_blocks}, {geom.num_kv_heads}, {geom.block_size}], got {tuple(t.shape)}")
 
 
 def kv_score(geom, q, lse, k_cache, block_table, seq_lens, cu_seqlens_q, scores, *, max_q_len, max_kv_len,
@@ -603,39 +616,31 @@ def kv_score(geom, q, lse, k_cache, block_table, seq_lens, cu_seqlens_q, scores,
     ([num_blocks, num_kv_heads, 16] fp32, paged like the caches; the step's own keys start from 0).
     `lse` is what the step's attention call returned.  Returns `scores`.  `workspace`: a uint8
     tensor of kv_score_workspace_bytes, for callers that keep one (one call at a time)."""
-    _require(q, "q", torch.bfloat16, 3)
-    _require(lse, "lse", torch.float32, 2)
-    k_cache = _cache_view(k_cache, geom, "k_cache")
-    _require(block_table, "block_table", torch.int32, 2)
-    _require(seq_lens, "seq_lens", torch.int32, 1)
-    _require(cu_seqlens_q, "cu_seqlens_q", torch.int32, 1)
-    _scores_pool(scores, "scores", geom, k_cache.shape[0])
-    S, T = seq_lens.shape[0], q.shape[0]
-    if tuple(q.shape[1:]) != (geom.num_q_heads, geom.head_dim):
-        raise ValueError("q must be [T, num_q_heads, head_dim]")
-    if tuple(lse.shape) != (T, geom.num_q_heads):
-        raise ValueError("lse must be [T, num_q_heads]")
-    if block_table.shape[0] != S or cu_seqlens_q.shape[0] != S + 1:
-        raise ValueError("block_table must have one row per sequence, cu_seqlens_q one entry more")
+    dev = _device_of(q, "q")
+    kv, cache_shape = _cache_shape(k_cache, geom, "k_cache")
+    if seq_lens is None or block_table is None or block_table.dim() != 2:
+        raise ValueError("seq_lens must be [S], block_table [S, max_blocks]")
+    T, S, f32, i32 = q.shape[0], seq_lens.shape[0], torch.float32, torch.int32
+    blocks = block_table.shape[1]
+    _need(q, "q", torch.bfloat16, dev, (T, geom.num_q_heads, geom.head_dim))
+    _need(lse, "lse", f32, dev, (T, geom.num_q_heads))
+    _need(k_cache, "k_cache", kv, dev, cache_shape)
+    _need(block_table, "block_table", i32, dev, (S, blocks))
+    _need(seq_lens, "seq_lens", i32, dev, (S,))
+    _need(cu_seqlens_q, "cu_seqlens_q", i32, dev, (S + 1,))
+    _need(scores, "scores", f32, dev, (cache_shape[0], geom.num_kv_heads, geom.block_size))
+    scale = None
     if geom.kv_dtype == KV_FP8_E4M3:
-        _scale(k_scale, "k_scale", geom)
-    _same_device(q, lse=lse, k_cache=k_cache, block_table=block_table, seq_lens=seq_lens, cu_seqlens_q=cu_seqlens_q,
-                 scores=scores, k_scale=k_scale, workspace=workspace)
+        _need(k_scale, "k_scale", f32, dev, (geom.num_kv_heads,))
+        scale = k_scale.data_ptr()
     desc = make_desc(geom, num_seqs=S, num_q_tokens=T, max_q_len=max_q_len, max_kv_len=max_kv_len,
-                     max_blocks_per_seq=block_table.shape[1], num_blocks=k_cache.shape[0], sum_kv_len=sum_kv_len)
-    lib = load_library()
-    on, stream = _on(q.device)
-    with on:
-        if workspace is None:
-            need = lib.eid_kv_score_workspace_bytes(C.byref(desc))
-            workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-        elif not workspace.is_contiguous():
-            raise ValueError("workspace must be contiguous")
-        check(lib.eid_kv_score(
-            C.byref(desc), q.data_ptr(), lse.data_ptr(), k_cache.data_ptr(), block_table.data_ptr(),
-            cu_seqlens_q.data_ptr(), seq_lens.data_ptr(), k_scale.data_ptr() if k_scale is not None else None,
-            scores.data_ptr(), workspace.data_ptr() if workspace is not None else None,
-            workspace.numel() * workspace.element_size() if workspace is not None else 0, stream))
+                     max_blocks_per_seq=blocks, num_blocks=cache_shape[0], sum_kv_len=sum_kv_len)
+    lib, ref = load_library(), C.byref(desc)
+    workspace = _workspace(workspace, lib.eid_kv_score_workspace_bytes(ref), dev)
+    ws, n = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.nbytes)
+    _launch(dev, lambda stream: lib.eid_kv_score(
+        ref, q.data_ptr(), lse.data_ptr(), k_cache.data_ptr(), block_table.data_ptr(), cu_seqlens_q.data_ptr(),
+        seq_lens.data_ptr(), scale, scores.data_ptr(), ws, n, stream))
     return scores
 
 
@@ -650,37 +655,42 @@ def kv_select(geom, scores, block_table, seq_lens, *, budget, keep_first=0, keep
     first keep_first, the last keep_last and the highest scores between them (ties: the lower
     row).  Returns (keep [S, num_kv_heads, budget] int32, ascending, -1 behind the count; counts
     [S] int32)."""
-    _require(block_table, "block_table", torch.int32, 2)
-    _require(seq_lens, "seq_lens", torch.int32, 1)
-    _require(scores, "scores", torch.float32, 3)
-    _scores_pool(scores, "scores", geom, scores.shape[0])
-    S = seq_lens.shape[0]
-    if block_table.shape[0] != S:
-        raise ValueError("block_table must have one row per sequence")
-    if max_kv_len > block_table.shape[1] * geom.block_size:
+    dev = _device_of(scores, "scores")
+    if seq_lens is None or block_table is None or block_table.dim() != 2 or scores.dim() != 3:
+        raise ValueError("seq_lens must be [S], block_table [S, max_blocks], scores [num_blocks, num_kv_heads, 16]")
+    S, f32, i32 = seq_lens.shape[0], torch.float32, torch.int32
+    blocks, num_blocks = block_table.shape[1], scores.shape[0]
+    if max_kv_len > blocks * geom.block_size:
         raise ValueError(f"block_table cannot hold max_kv_len {max_kv_len}")
     if budget <= 0:
         raise ValueError("budget must be positive")
+    _need(scores, "scores", f32, dev, (num_blocks, geom.num_kv_heads, geom.block_size))
+    _need(block_table, "block_table", i32, dev, (S, blocks))
+    _need(seq_lens, "seq_lens", i32, dev, (S,))
     if keep is None:
-        keep = torch.empty((S, geom.num_kv_heads, budget), dtype=torch.int32, device=scores.device)
+        keep = torch.empty((S, geom.num_kv_heads, budget), dtype=i32, device=scores.device)
     else:
-        _require(keep, "keep", torch.int32, 3)
-        if tuple(keep.shape) != (S, geom.num_kv_heads, budget):
-            raise ValueError("keep must be [S, num_kv_heads, budget]")
+        _need(keep, "keep", i32, dev, (S, geom.num_kv_heads, budget))
     if counts is None:
-        counts = torch.empty((S,), dtype=torch.int32, device=scores.device)
+        counts = torch.empty((S,), dtype=i32, device=scores.device)
     else:
-        _require(counts, "counts", torch.int32, 1)
-        if counts.shape[0] != S:
-            raise ValueError("counts must be [S]")
-    _same_device(scores, block_table=block_table, seq_lens=seq_lens, keep=keep, counts=counts)
-    desc = _rows_desc(geom, block_table, scores.shape[0], max_kv_len)
-    on, stream = _on(scores.device)
-    with on:
-        check(load_library().eid_kv_select(
-            C.byref(desc), scores.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), budget, keep_first,
-            keep_last, keep.data_ptr(), counts.data_ptr(), stream))
+        _need(counts, "counts", i32, dev, (S,))
+    desc = _rows_desc(geom, S, blocks, num_blocks, max_kv_len)
+    lib = load_library()
+    _launch(dev, lambda stream: lib.eid_kv_select(
+        C.byref(desc), scores.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), budget, keep_first, keep_last,
+        keep.data_ptr(), counts.data_ptr(), stream))
     return keep, counts
+
+
+def _layers(tensors, name, dtype, device, shape):
+    """Addresses of one tensor per layer, all of them of that type and shape."""
+    T = torch.Tensor
+    if not (set(map(T.get_device, tensors)) == {device} and all([t.shape == shape for t in tensors])
+            and all([t.dtype is dtype for t in tensors]) and all(map(T.is_contiguous, tensors))):
+        for i, t in enumerate(tensors):
+            _need(t, f"{name}[{i}]", dtype, device, shape)
+    return list(map(T.data_ptr, tensors))
 
 
 def kv_compact(geom, k_caches, v_caches, block_table, seq_lens, keep, counts, *, starts=None, scores=None):
@@ -689,52 +699,37 @@ def kv_compact(geom, k_caches, v_caches, block_table, seq_lens, keep, counts, *,
     (list, optional).  keep is int32 and ascending, keep[..., i] >= starts[s] + i: [S, N] (the same
     rows in every layer and head), [S, Hkv, N] (in every layer) or [layers, S, Hkv, N]; seq_lens is
     the length before the move.  The sequence's length afterwards is starts[s] + counts[s]."""
-    n_layers = len(k_caches)
-    if n_layers == 0 or len(v_caches) != n_layers or (scores is not None and len(scores) != n_layers):
+    n = len(k_caches)
+    if n == 0 or len(v_caches) != n or (scores is not None and len(scores) != n):
         raise ValueError("k_caches, v_caches (and scores) must be lists with one tensor per layer")
-    k_caches = [_cache_view(t, geom, f"k_caches[{i}]") for i, t in enumerate(k_caches)]
-    v_caches = [_cache_view(t, geom, f"v_caches[{i}]") for i, t in enumerate(v_caches)]
-    num_blocks = k_caches[0].shape[0]
-    pointers = [t.data_ptr() for t in k_caches] + [t.data_ptr() for t in v_caches]
+    dev = _device_of(keep, "keep")
+    kv, cache_shape = _cache_shape(k_caches[0], geom, "k_caches[0]")
+    if seq_lens is None or block_table is None or block_table.dim() != 2 or not 2 <= keep.dim() <= 4:
+        raise ValueError("keep must be [S, N], [S, num_kv_heads, N] or [layers, S, num_kv_heads, N]; seq_lens [S]; "
+                         "block_table [S, max_blocks]")
+    S, i32, H = seq_lens.shape[0], torch.int32, geom.num_kv_heads
+    blocks, N, dims = block_table.shape[1], keep.shape[-1], keep.dim()
+    at = _layers(k_caches, "k_caches", kv, dev, cache_shape) + _layers(v_caches, "v_caches", kv, dev, cache_shape)
     if scores is not None:
-        for i, t in enumerate(scores):
-            _scores_pool(t, f"scores[{i}]", geom, num_blocks)
-        pointers += [t.data_ptr() for t in scores]
-    if len(set(pointers)) != len(pointers):
+        at += _layers(scores, "scores", torch.float32, dev, (cache_shape[0], H, geom.block_size))
+    if len(set(at)) != len(at):
         raise ValueError("a tensor is given twice")
-    _require(block_table, "block_table", torch.int32, 2)
-    _require(seq_lens, "seq_lens", torch.int32, 1)
-    _require(counts, "counts", torch.int32, 1)
-    S = seq_lens.shape[0]
-    if block_table.shape[0] != S or counts.shape[0] != S:
-        raise ValueError("block_table and counts must have one row per sequence")
+    _need(block_table, "block_table", i32, dev, (S, blocks))
+    _need(seq_lens, "seq_lens", i32, dev, (S,))
+    _need(counts, "counts", i32, dev, (S,))
+    _need(keep, "keep", i32, dev, (S, N) if dims == 2 else (S, H, N) if dims == 3 else (n, S, H, N))
+    first = None
     if starts is not None:
-        _require(starts, "starts", torch.int32, 1)
-        if starts.shape[0] != S:
-            raise ValueError("starts must be [S]")
-    _require(keep, "keep", torch.int32)
-    N = keep.shape[-1] if keep.dim() else 0
-    shapes = {2: (S, N), 3: (S, geom.num_kv_heads, N), 4: (n_layers, S, geom.num_kv_heads, N)}
-    if tuple(keep.shape) != shapes.get(keep.dim()):
-        raise ValueError("keep must be [S, N], [S, num_kv_heads, N] or [layers, S, num_kv_heads, N]")
-    per_head = keep.dim() > 2
-    for name, group in (("k_caches", k_caches), ("v_caches", v_caches), ("scores", scores or [])):
-        for t in group:
-            if t.shape[0] != num_blocks:
-                raise ValueError(f"{name}: every layer must have {num_blocks} blocks")
-            _same_device(keep, **{name: t})
-    _same_device(keep, block_table=block_table, seq_lens=seq_lens, counts=counts, starts=starts)
-    desc = _rows_desc(geom, block_table, num_blocks)
-    at = (C.c_int64 * len(pointers))(*pointers)
-    off = C.sizeof(C.c_int64) * n_layers
-    base = C.addressof(at)
-    on, stream = _on(keep.device)
-    with on:
-        check(load_library().eid_kv_compact(
-            C.byref(desc), n_layers, base, base + off, base + 2 * off if scores is not None else None,
-            block_table.data_ptr(), seq_lens.data_ptr(), keep.data_ptr(),
-            S * geom.num_kv_heads * N if keep.dim() == 4 else 0, (geom.num_kv_heads if per_head else 1) * N,
-            N if per_head else 0, N, counts.data_ptr(), starts.data_ptr() if starts is not None else None, stream))
+        _need(starts, "starts", i32, dev, (S,))
+        first = starts.data_ptr()
+    desc = _rows_desc(geom, S, blocks, cache_shape[0])
+    host = (C.c_int64 * len(at))(*at)
+    base = C.addressof(host)
+    lib = load_library()
+    _launch(dev, lambda stream: lib.eid_kv_compact(
+        C.byref(desc), n, base, base + 8 * n, base + 16 * n if scores is not None else None, block_table.data_ptr(),
+        seq_lens.data_ptr(), keep.data_ptr(), S * H * N if dims == 4 else 0, N if dims == 2 else H * N,
+        0 if dims == 2 else N, N, counts.data_ptr(), first, stream))
 
 
 def workspace_layout(desc):
