@@ -440,7 +440,10 @@ __global__ __launch_bounds__(kSelThreads) void select_kernel(const SelectParams 
 // row start + i <- row keep[i], i ascending, keep[i] >= start + i.  In place: a workgroup owns a
 // column of the sequence (one KV head, or eight where all heads keep the same rows) in one tensor
 // of one layer and moves it in steps; a step's rows are all in registers before its first
-// store, and later steps read only rows behind everything that this one overwrites.
+// store, and later steps read only rows behind everything that this one overwrites.  What bounds
+// long moves is the caches' layout: a head's row is 128 bytes of a token's 1 KiB and every head keeps
+// other tokens, so memory sees lone lines (8 sequences cut from 16k to 4k: 40 us for 137 MB; two
+// workgroups per column, 64 bytes of a row each: 49 us).
 // ---------------------------------------------------------------------------------------
 __device__ __forceinline__ void step_loaded() {
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's rows are in registers
@@ -463,52 +466,57 @@ __global__ __launch_bounds__(THREADS) void compact_kernel(const CompactParams p,
   if (start < 0 || n <= 0) return;
   const int32_t *keep = p.keep + (size_t)layer * p.keep_layer + (size_t)s * p.keep_seq + (size_t)hg * heads * p.keep_head;
   const int32_t *bt = p.block_table + (size_t)s * p.max_blocks_per_seq;
+  auto page_of = [&](const int row) { return clamp_id(bt[row / kBlock], p.last_block); };
+  // Addresses are found a step ahead, and loads are issued for all R rows of a lane at once (one
+  // that does not move loads the sequence's row `start` and stores nothing).
+  auto move_all = [&](auto zero, auto *base, const int lanes, auto at) {
+    using T = decltype(zero);
+    const int per = THREADS / lanes, r0 = tid / lanes;
+    int src[R], from[R], to[R];  // source row (its own place: no move), pages of both
+    auto find = [&](const int i0) {
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        const int i = i0 + k * per + r0, row = start + min(i, n - 1);
+        const int x = keep[min(i, n - 1)];
+        src[k] = i < n && x > row && x < len ? x : row;
+      }
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        from[k] = page_of(src[k]);
+        to[k] = page_of(start + min(i0 + k * per + r0, n - 1));
+      }
+    };
+    find(0);
+    for (int i0 = 0; i0 < n; i0 += per * R) {
+      T x[R];
+      T *dst[R];
+      bool move[R];
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        const int row = start + min(i0 + k * per + r0, n - 1);
+        move[k] = i0 + k * per + r0 < n && src[k] != row;
+        x[k] = *(const T *)at(base, from[k], src[k]);
+        dst[k] = (T *)at(base, to[k], row);
+      }
+      if (i0 + per * R < n) find(i0 + per * R);
+      step_loaded();
+#pragma unroll
+      for (int k = 0; k < R; ++k)
+        if (move[k]) *dst[k] = x[k];
+    }
+  };
   if (what < 2) {
-    uint8_t *base = what ? p.v[layer] : p.k[layer];
     const int lanes = heads * kHeadDim * p.elt / 16;  // 16-byte lanes of a row: 4 .. 64
     const uint32_t row_bytes = (uint32_t)p.num_kv_heads * kHeadDim * p.elt;
     const uint32_t col = (uint32_t)hg * heads * kHeadDim * p.elt + (tid % lanes) * 16;
-    const int per = THREADS / lanes, r0 = tid / lanes;
-    auto addr = [&](const int row) {
-      const int page = clamp_id(bt[row / kBlock], p.last_block);
-      return (size_t)page * kBlock * row_bytes + (size_t)(row & 15) * row_bytes + col;
-    };
-    for (int i0 = 0; i0 < n; i0 += per * R) {
-      u32x4 x[R];
-      bool move[R];
-#pragma unroll
-      for (int k = 0; k < R; ++k) {
-        const int i = i0 + k * per + r0;
-        const int src = i < n ? keep[i] : -1;
-        move[k] = src > start + i && src < len;  // (a row that stays in place is not touched)
-        if (move[k]) x[k] = *(const u32x4 *)(base + addr(src));
-      }
-      step_loaded();
-#pragma unroll
-      for (int k = 0; k < R; ++k)
-        if (move[k]) *(u32x4 *)(base + addr(start + i0 + k * per + r0)) = x[k];
-    }
+    move_all(u32x4{}, what ? p.v[layer] : p.k[layer], lanes, [=](uint8_t *base, const int page, const int row) {
+      return base + (size_t)page * kBlock * row_bytes + (uint32_t)(row & 15) * row_bytes + col;
+    });
   } else {
-    float *base = p.scores[layer];
-    for (int i0 = 0; i0 < n; i0 += THREADS / heads * R) {
-      const int per = THREADS / heads, h = hg * heads + tid % heads, r0 = tid / heads;
-      auto addr = [&](const int row) {
-        return ((size_t)clamp_id(bt[row / kBlock], p.last_block) * p.num_kv_heads + h) * kBlock + (row & 15);
-      };
-      float x[R];
-      bool move[R];
-#pragma unroll
-      for (int k = 0; k < R; ++k) {
-        const int i = i0 + k * per + r0;
-        const int src = i < n ? keep[i] : -1;
-        move[k] = src > start + i && src < len;
-        if (move[k]) x[k] = base[addr(src)];
-      }
-      step_loaded();
-#pragma unroll
-      for (int k = 0; k < R; ++k)
-        if (move[k]) base[addr(start + i0 + k * per + r0)] = x[k];
-    }
+    const int h = hg * heads + tid % heads, Hkv = p.num_kv_heads;
+    move_all(0.f, p.scores[layer], heads, [=](float *base, const int page, const int row) {
+      return base + ((size_t)page * Hkv + h) * kBlock + (row & 15);
+    });
   }
 }
 
