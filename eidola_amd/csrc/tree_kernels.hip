@@ -13,6 +13,7 @@ __device__ __forceinline__ const_i32_ptr as_constant(const int32_t *p) { return 
 __device__ __forceinline__ int clamp_id(const int id, const int last) { return min(max(id, 0), last); }
 
 constexpr float kLazyLog2 = 8.0f;  // a row's reference moves when a score outgrows it by this
+constexpr float kRowSumGuard = 1152921504606846976.0f;  // 2^60
 
 // What one sequence gives the kernel: `chunks` 64-key chunks from key `begin` on for each of
 // `tiles` tiles of drafted tokens.
@@ -149,8 +150,8 @@ template <int I>
 using IC = std::integral_constant<int, I>;
 #define EID_SB() __builtin_amdgcn_sched_barrier(0)
 
-template <int NT, bool FP8>
-__global__ __launch_bounds__(kTreeWaves * 64, NT == 1 ? 3 : 2) void tree_kernel(const TreeParams p) {
+template <int NT, bool FP8, bool LSE>
+__global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_kernel(const TreeParams p) {
   constexpr int kTok = 2 * NT * kTreeWaves;  // tokens of a tile
   constexpr int kRows = kTok * kGroup;
   constexpr int kElt = FP8 ? 1 : 2;
@@ -177,6 +178,9 @@ __global__ __launch_bounds__(kTreeWaves * 64, NT == 1 ? 3 : 2) void tree_kernel(
   const float vs = FP8 ? p.v_scale[kvh] : 1.0f;
 
   const TreePlace place = find_place(p, range, kTok);
+  Frag8 ones;
+  ones.u = u32x4{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
+  asm volatile("" : "+v"(ones.u));  // (kept in registers)
   int u = place.u, s = place.seq, before = place.before;
   TreeRecord rec = {0, 0, 0, 0};  // what the merge has to join from this range on
 
@@ -333,12 +337,17 @@ __global__ __launch_bounds__(kTreeWaves * 64, NT == 1 ? 3 : 2) void tree_kernel(
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) acc[t][mt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
+    bool fresh = true;  // no row has a reference from a chunk that it sees whole
     bool odd = false;  // this lane took a value that is not finite out of a masked chunk
 
     // One chunk.  Its tiles overlap: while tile t's exponentials run, the matrix unit works on the
-    // scores of tile t + 1 and the output of tile t - 1.
+    // scores of tile t + 1 and the output of tile t - 1.  A row's reference is the maximum of its first
+    // chunks (those that are masked and the first that is not) and then stays: a weight may grow far
+    // beyond 1, which costs nothing in fp32 and bf16 until its row's sum reaches 2^60 (see guard).
+    // Row sums: products of the rounded weights with ones; exact fp32 sums where lse is asked for.
     auto step = [&](const uint8_t *kbuf, const uint8_t *vbuf, const int tc) {
       const bool need_mask = masked(tc);  // (one stream for both kinds: two would not share registers)
+      const bool track = need_mask || fresh;
       Frag8 kf[4][2], vf[4][2];
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
@@ -370,8 +379,9 @@ __global__ __launch_bounds__(kTreeWaves * 64, NT == 1 ? 3 : 2) void tree_kernel(
               x &= (hi ? 0xFFFFu : ~0u) & (lo ? 0xFFFF0000u : ~0u);
             }
       }
-      f32x4 S[2][4];
+      f32x4 S[2][4], lt;
       Frag8 P[2][2];
+      float sum = 0.f;  // LSE: of a tile's weights, this lane's keys
       auto load_q = [&](auto t_c) {
         constexpr int t = t_c;
         if constexpr (QLDS && t < NT) {
@@ -389,63 +399,128 @@ __global__ __launch_bounds__(kTreeWaves * 64, NT == 1 ? 3 : 2) void tree_kernel(
         constexpr int t = t_c, j = j_c, mt = j & 3, pr = j >> 2;
         acc[t][mt] = mfma16x32(vf[mt][pr], P[t & 1][pr], acc[t][mt]);
       };
+      auto row_sum = [&](auto t_c, auto j_c) {  // every lane of a row receives its sum over the chunk
+        constexpr int t = t_c, j = j_c;
+        if constexpr (j == 0) lt = mfma16x32(ones, P[t & 1][0], f32x4{0.f, 0.f, 0.f, 0.f});
+        else lt = mfma16x32(ones, P[t & 1][1], lt);
+      };
+      auto lane_max = [&](const f32x4(&Sx)[4]) {
+        float mx = max3(Sx[0][0], Sx[0][1], Sx[0][2]);
+#pragma unroll
+        for (int o = 1; o < 7; ++o)
+          mx = max3(mx, Sx[(2 * o + 1) >> 2][(2 * o + 1) & 3], Sx[(2 * o + 2) >> 2][(2 * o + 2) & 3]);
+        return max2(mx, Sx[3][3]) * c2;
+      };
+      auto move_ref = [&](auto t_c, const float m_new) {
+        constexpr int t = t_c;
+        const float alpha = fast_exp2(m[t] - m_new);
+        l[t] *= alpha;
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[t][mt][r] *= alpha;
+        m[t] = m_new;
+      };
+      // After tile t's weights: a row whose sum is not below 2^60 (inf and NaN among that) has outgrown
+      // its reference.  Its scores are computed again and the reference moves to their maximum.  (In a
+      // masked chunk the reference has just followed the maximum: only a NaN could be found there.)
+      auto guard = [&](auto t_c) {
+        constexpr int t = t_c;
+        float got = LSE ? sum : lt[0];
+        if (!need_mask && __any(!(got < kRowSumGuard))) {
+          f32x4(&Sx)[4] = S[t & 1];
+          Frag8 q2[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if constexpr (QLDS) q2[h].u = *(const u32x4 *)(q_lds + (2 * t + h) * 1024);
+            else q2[h] = qf[QLDS ? 0 : t][h];
+          }
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            Sx[b] = mfma16x32(kf[b][0], q2[0], f32x4{0.f, 0.f, 0.f, 0.f});
+            Sx[b] = mfma16x32(kf[b][1], q2[1], Sx[b]);
+          }
+          move_ref(t_c, max2(m[t], rowgroup_max(lane_max(Sx))));  // (a plain chunk: every key is seen)
+          got = 0.f;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float p0 = fast_exp2(__builtin_fmaf(Sx[(2 * k) >> 2][(2 * k) & 3], c2, -m[t]));
+            const float p1 = fast_exp2(__builtin_fmaf(Sx[(2 * k + 1) >> 2][(2 * k + 1) & 3], c2, -m[t]));
+            got += p0 + p1;
+            P[t & 1][k >> 2].w[k & 3] = pack_bf16(p0, p1);
+          }
+          if constexpr (!LSE) got = rowgroup_sum(got);
+        }
+        l[t] += got;
+      };
       load_q(IC<0>{});
       load_q(IC<1>{});
       static_for<8>([&](auto j) { score(IC<0>{}, j); });
       static_for<NT>([&](auto t_c) {
         constexpr int t = t_c;
         f32x4(&Sx)[4] = S[t & 1];
-        if (need_mask) {
-          const int tl = wtok + 2 * t + (i16 >> 3);
-          const uint64_t w = chunk_bits(lds_mask[tl], lds_lo[tl], prefix, tc) >> (4 * g);
+        if constexpr (t > 0) guard(IC<t - 1>{});
+        if (track) {
+          if (need_mask) {
+            const int tl = wtok + 2 * t + (i16 >> 3);
+            const uint64_t w = chunk_bits(lds_mask[tl], lds_lo[tl], prefix, tc) >> (4 * g);
 #pragma unroll
-          for (int b = 0; b < 4; ++b)
+            for (int b = 0; b < 4; ++b)
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (!((w >> (16 * b + r)) & 1)) Sx[b][r] = -INFINITY;
-        }
-        float mx = max3(Sx[0][0], Sx[0][1], Sx[0][2]);
-#pragma unroll
-        for (int o = 1; o < 7; ++o)
-          mx = max3(mx, Sx[(2 * o + 1) >> 2][(2 * o + 1) & 3], Sx[(2 * o + 2) >> 2][(2 * o + 2) & 3]);
-        mx = max2(mx, Sx[3][3]) * c2;
-        if (__any(mx > m[t] + kLazyLog2)) {
-          const float mrow = rowgroup_max(mx);
-          const float m_new = mrow > m[t] + kLazyLog2 ? mrow : m[t];
-          const float alpha = fast_exp2(m[t] - m_new);
-          l[t] *= alpha;
-#pragma unroll
-          for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) acc[t][mt][r] *= alpha;
-          m[t] = m_new;
+              for (int r = 0; r < 4; ++r)
+                if (!((w >> (16 * b + r)) & 1)) Sx[b][r] = -INFINITY;
+          }
+          const float mx = lane_max(Sx);
+          if (__any(mx > m[t] + kLazyLog2)) {
+            const float mrow = rowgroup_max(mx);
+            move_ref(t_c, mrow > m[t] + kLazyLog2 ? mrow : m[t]);
+          }
         }
         EID_SB();
-        // 16 scores of a lane, spread over the stage's matrix instructions
+        // The stage: output of tile t - 1, scores of tile t + 1, and between them the 16 scores of a
+        // lane; the row sums two matrix instructions before the end, so that they are there for the guard.
         constexpr int n_value = t > 0 ? 8 : 0, n_score = t + 1 < NT ? 8 : 0, n_mfma = n_value + n_score;
-        constexpr int per_slot = n_mfma == 16 ? 1 : 2, slots = 16 / per_slot;
+        constexpr int slots = n_mfma > 0 ? n_mfma : 1, spread = n_mfma > 2 ? n_mfma - 2 : 1;
         static_for<slots>([&](auto i_c) {
           constexpr int i = i_c;
+          if constexpr (!LSE && i == spread) {
+            row_sum(t_c, IC<0>{});
+            row_sum(t_c, IC<1>{});
+          }
           if constexpr (i < n_value) value(IC<(t > 0 ? t - 1 : 0)>{}, i_c);
           else if constexpr (i < n_mfma) score(IC<(t + 1 < NT ? t + 1 : 0)>{}, IC<i - n_value>{});
           if constexpr (i == n_mfma - 1) load_q(IC<t + 2>{});
-          static_for<per_slot>([&](auto e_c) {
-            constexpr int e = i * per_slot + e_c;
-            const float x = fast_exp2(__builtin_fmaf(Sx[e >> 2][e & 3], c2, -m[t]));
-            Sx[e >> 2][e & 3] = x;
-            if constexpr (e % 2 == 1) {
-              l[t] += Sx[(e - 1) >> 2][(e - 1) & 3];
-              l[t] += x;
-              uint32_t w = pack_bf16(Sx[(e - 1) >> 2][(e - 1) & 3], x);
-              asm volatile("" : "+v"(w), "+v"(l[t]));  // (pinned here: they would be sunk to where they are used)
-              P[t & 1][e >> 3].w[(e >> 1) & 3] = w;
+          static_for<16>([&](auto e_c) {
+            constexpr int e = e_c;
+            if constexpr (e * spread / 16 == i) {
+              const float x = fast_exp2(__builtin_fmaf(Sx[e >> 2][e & 3], c2, -m[t]));
+              Sx[e >> 2][e & 3] = x;
+              if constexpr (e % 2 == 1) {
+                const float y = Sx[(e - 1) >> 2][(e - 1) & 3];
+                uint32_t w = pack_bf16(y, x);
+                // (pinned here: they would be sunk to where they are used)
+                if constexpr (LSE) {
+                  sum = e == 1 ? y + x : sum + y + x;
+                  asm volatile("" : "+v"(w), "+v"(sum));
+                } else {
+                  asm volatile("" : "+v"(w));
+                }
+                P[t & 1][e >> 3].w[(e >> 1) & 3] = w;
+              }
             }
           });
           EID_SB();
         });
+        if constexpr (!LSE && spread >= slots) {
+          row_sum(t_c, IC<0>{});
+          row_sum(t_c, IC<1>{});
+        }
       });
+      guard(IC<NT - 1>{});
       static_for<8>([&](auto j) { value(IC<NT - 1>{}, j); });
+      if (!need_mask) fresh = false;
     };
+
     if constexpr (FP8) {
       // chunk c is in stage c % 2, chunk c + 1 in registers; with registers to spare chunk c + 2 is
       // requested as well
@@ -562,7 +637,7 @@ __global__ __launch_bounds__(kTreeWaves * 64, NT == 1 ? 3 : 2) void tree_kernel(
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const int tl = wtok + 2 * t + (i16 >> 3);
-        const float lt = rowgroup_sum(l[t]);
+        const float lt = LSE ? rowgroup_sum(l[t]) : l[t];
         if (tl >= ntok) continue;
         if (whole) {
           const int head = kvh * kGroup + (i16 & 7);
@@ -675,19 +750,19 @@ int tree_tiles(const int max_q_len) {
 }
 int tree_tile_tokens(const int max_q_len) { return 2 * tree_tiles(max_q_len) * kTreeWaves; }
 
-template <bool FP8>
+template <bool FP8, bool LSE>
 static void launch_tree_tiles(const TreeParams &p, const int nt, hipStream_t st) {
   const dim3 grid((unsigned)(p.ranges * p.num_kv_heads)), block(kTreeWaves * 64);
-  if (nt == 1) tree_kernel<1, FP8><<<grid, block, 0, st>>>(p);
-  else if (nt == 2) tree_kernel<2, FP8><<<grid, block, 0, st>>>(p);
-  else if (nt == 3) tree_kernel<3, FP8><<<grid, block, 0, st>>>(p);
-  else tree_kernel<4, FP8><<<grid, block, 0, st>>>(p);
+  if (nt == 1) tree_kernel<1, FP8, LSE><<<grid, block, 0, st>>>(p);
+  else if (nt == 2) tree_kernel<2, FP8, LSE><<<grid, block, 0, st>>>(p);
+  else if (nt == 3) tree_kernel<3, FP8, LSE><<<grid, block, 0, st>>>(p);
+  else tree_kernel<4, FP8, LSE><<<grid, block, 0, st>>>(p);
 }
 
 hipError_t launch_tree(const TreeParams &p, const bool fp8, hipStream_t st) {
   const int nt = tree_tiles(p.max_q_len);
-  if (fp8) launch_tree_tiles<true>(p, nt, st);
-  else launch_tree_tiles<false>(p, nt, st);
+  if (fp8) p.lse ? launch_tree_tiles<true, true>(p, nt, st) : launch_tree_tiles<true, false>(p, nt, st);
+  else p.lse ? launch_tree_tiles<false, true>(p, nt, st) : launch_tree_tiles<false, false>(p, nt, st);
   return hipGetLastError();
 }
 
