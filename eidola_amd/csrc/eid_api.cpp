@@ -1145,7 +1145,7 @@ int32_t eid_o_proj(const void *attn_out, const void *weight, const void *bias,
 namespace {
 
 struct TreePlan {
-  int32_t ranges;  // workgroups per KV head
+  int32_t ranges, max_tiles;  // workgroups per KV head, tiles of the longest tree
   size_t rec_bytes, o_bytes, ml_bytes;
   size_t total() const { return rec_bytes + o_bytes + ml_bytes; }
 };
@@ -1154,7 +1154,8 @@ TreePlan make_tree_plan(const eid_attn_desc *d) {
   TreePlan pl;
   const long long tile = eid::tree_tile_tokens(d->max_q_len);
   // an upper bound of the launch's 64-key chunks, by what the descriptor says of the lengths
-  const long long tiles = std::min<long long>((d->max_q_len + tile - 1) / tile, d->num_q_tokens);
+  const long long tiles = (d->max_q_len + tile - 1) / tile;
+  pl.max_tiles = (int32_t)tiles;
   long long keys = d->sum_kv_len ? d->sum_kv_len : (long long)d->num_seqs * d->max_kv_len;
   if (d->window > 0) {
     const long long span = (long long)d->window + d->max_q_len + eid::kBlock;
@@ -1165,8 +1166,8 @@ TreePlan make_tree_plan(const eid_attn_desc *d) {
   const long long most = (chunks + eid::kTreeMinChunks - 1) / eid::kTreeMinChunks;
   pl.ranges = (int32_t)std::max(1LL, std::min(fill, most));
   const size_t rows = (size_t)pl.ranges * d->num_kv_heads * 2 * tile * eid::kGroup;
-  pl.rec_bytes = ((size_t)pl.ranges * sizeof(eid::TreeRecord) + 255) / 256 * 256;
-  pl.o_bytes = rows * eid::kHeadDim * sizeof(float);
+  pl.rec_bytes = ((size_t)d->num_seqs * tiles * sizeof(eid::TreeRecord) + 255) / 256 * 256;
+  pl.o_bytes = rows * eid::kHeadDim * sizeof(_Float16);
   pl.ml_bytes = rows * 2 * sizeof(float);
   return pl;
 }
@@ -1251,8 +1252,8 @@ int32_t eid_attn_tree(const eid_attn_desc *desc, const eid_attn_args *args, cons
   if (mask_words < (desc->max_q_len + 63) / 64 || mask_words > eid::kTreeWordsMax)
     return fail(EID_ERR_INVALID_ARG, "mask_words %d: max_q_len %d needs %d to %d", mask_words, desc->max_q_len,
                 (desc->max_q_len + 63) / 64, eid::kTreeWordsMax);
-  if ((long long)desc->num_q_tokens * desc->num_kv_heads > 0x7fffffffLL)
-    return fail(EID_ERR_UNSUPPORTED, "num_q_tokens %d too large", desc->num_q_tokens);
+  if ((long long)desc->num_seqs * ((desc->max_q_len + 31) / 32 * 32) * desc->num_kv_heads > 0x3fffffffLL)
+    return fail(EID_ERR_UNSUPPORTED, "batch of %d trees with %d KV heads is too large", desc->num_seqs, desc->num_kv_heads);
   const TreePlan pl = make_tree_plan(desc);
   const size_t need = pl.total();
   if (!args->workspace || args->workspace_bytes < need)
@@ -1277,7 +1278,7 @@ int32_t eid_attn_tree(const eid_attn_desc *desc, const eid_attn_args *args, cons
   p.mask = reinterpret_cast<const uint64_t *>(tree_mask);
   uint8_t *ws = static_cast<uint8_t *>(args->workspace);
   p.ws_rec = reinterpret_cast<eid::TreeRecord *>(ws);
-  p.ws_o = reinterpret_cast<float *>(ws + pl.rec_bytes);
+  p.ws_o = reinterpret_cast<_Float16 *>(ws + pl.rec_bytes);
   p.ws_ml = reinterpret_cast<float *>(ws + pl.rec_bytes + pl.o_bytes);
   p.num_seqs = desc->num_seqs;
   p.num_q_heads = desc->num_q_heads;
@@ -1289,6 +1290,7 @@ int32_t eid_attn_tree(const eid_attn_desc *desc, const eid_attn_args *args, cons
   p.window = desc->window;
   p.max_q_len = desc->max_q_len;
   p.max_kv_len = desc->max_kv_len;
+  p.max_tiles = pl.max_tiles;
   p.ranges = pl.ranges;
   p.min_chunks = eid::kTreeMinChunks;
   p.softmax_scale = desc->softmax_scale;

@@ -10,11 +10,9 @@ constexpr int kTreeMax = 64 * kTreeWordsMax;  // drafted tokens per sequence
 constexpr int kTreeWaves = 4;
 constexpr int kTreeMinChunks = 2;             // 64-key chunks per workgroup of a range, at least
 
-// Tile of drafted tokens that begins in a range and ends in a later one (ntok == 0: none).
+// Where the pieces of a tile of drafted tokens are.
 struct TreeRecord {
-  int32_t row, ntok;  // first row of q / out, number of tokens
-  int32_t pieces;     // ranges that hold some of it
-  int32_t unused;
+  int32_t range, pieces;  // first range that holds some of it, and how many do
 };
 
 struct TreeParams {
@@ -26,11 +24,12 @@ struct TreeParams {
   const float *sinks;             // may be null
   const float *k_scale, *v_scale; // fp8 only
   const uint64_t *mask;           // [num_q_tokens][mask_words]
-  TreeRecord *ws_rec;  // [ranges]
-  float *ws_o;   // [ranges][Hkv][2][tile rows][64]  sum of e^(s-m) v of a piece, not normalised
+  TreeRecord *ws_rec;  // [num_seqs][max_tiles]
+  _Float16 *ws_o;  // [ranges][Hkv][2][tile rows][64]  sum of 2^(s-m) v of a piece, not normalised
   float *ws_ml;  // [ranges][Hkv][2][tile rows][2]   m (log2 units), l
   int32_t num_seqs, num_q_heads, num_kv_heads, max_blocks_per_seq, last_block;
   int32_t num_q_tokens, mask_words, window, max_q_len, max_kv_len;
+  int32_t max_tiles;  // tiles of the longest tree
   int32_t ranges;     // workgroups per KV head
   int32_t min_chunks; // smallest range
   float softmax_scale;

@@ -138,6 +138,13 @@ typedef __attribute__((address_space(1))) const void gptr_t;
 typedef __attribute__((address_space(3))) void lptr_t;
 constexpr int kTileBytes = kChunk * 128;
 
+typedef __attribute__((ext_vector_type(4))) _Float16 f16x4;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+// e with |x| in [2^(e-1), 2^e); 0 for 0
+__device__ __forceinline__ int top_exponent(const float x) {
+  return x > 0.f ? __builtin_amdgcn_frexp_expf(x) : 0;
+}
+
 template <int... Is, typename F>
 __device__ __forceinline__ void static_for_impl(std::integer_sequence<int, Is...>, F &&f) {
   (f(std::integral_constant<int, Is>{}), ...);
@@ -182,7 +189,6 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_kernel(const TreePara
   ones.u = u32x4{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
   asm volatile("" : "+v"(ones.u));  // (kept in registers)
   int u = place.u, s = place.seq, before = place.before;
-  TreeRecord rec = {0, 0, 0, 0};  // what the merge has to join from this range on
 
   const uint32_t row_bytes = (uint32_t)Hkv * kHeadDim * kElt;
   const size_t page_bytes = (size_t)kBlock * row_bytes;
@@ -627,11 +633,11 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_kernel(const TreePara
     // ---- this piece's rows: the answer, or a partial
     const bool whole = n == v.chunks;
     const int part = c0 == 0 ? 1 : 0;  // a range holds at most one piece of each kind that is not whole
-    float *ws_o = p.ws_o + ((size_t)(range * Hkv + kvh) * 2 + part) * (kRows * kHeadDim);
+    _Float16 *ws_o = p.ws_o + ((size_t)(range * Hkv + kvh) * 2 + part) * (kRows * kHeadDim);
     float *ws_ml = p.ws_ml + ((size_t)(range * Hkv + kvh) * 2 + part) * (kRows * 2);
-    if (!whole && c0 == 0) {
-      const int last = u - c0 + v.chunks - 1;  // the tile's last unit
-      rec = {v.row0 + tok0, ntok, last / place.per - range + 1, 0};
+    if (c0 == 0 && kvh == 0 && tid == 0) {  // the tile begins here: where its pieces are
+      const int last = u + v.chunks - 1;    // its last unit
+      p.ws_rec[s * p.max_tiles + tile] = {range, last / place.per - range + 1};
     }
     if (wave_active) {
 #pragma unroll
@@ -657,88 +663,117 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_kernel(const TreePara
           }
           if (p.lse && g == 0) p.lse[orow] = any ? (M + __log2f(den)) * kLn2 : -INFINITY;
         } else {
+          // The outputs go out as fp16 beside a power of two of the row's own, which brings its largest
+          // (finite) one to [1/2, 1): a rounding of 2^-12 there, one of 2^-25 of that one for those
+          // that are far smaller, against the 2^-9 of the bf16 that the answer is rounded to; and half
+          // the bytes of fp32.  The power moves into m and l: (m + e, l 2^-e, o 2^-e) is the same piece.
           const int row = tl * kGroup + (i16 & 7);
+          float top = 0.f;
 #pragma unroll
-          for (int mt = 0; mt < 4; ++mt) *(f32x4 *)(ws_o + (size_t)row * kHeadDim + 16 * mt + 4 * g) = acc[t][mt];
+          for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const float x = fabsf(acc[t][mt][r]);
+              top = fmaxf(top, x < INFINITY ? x : 0.f);
+            }
+          const int e = top_exponent(rowgroup_max(top));
+#pragma unroll
+          for (int mt = 0; mt < 4; ++mt) {
+            f16x4 h;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) h[r] = (_Float16)ldexpf(acc[t][mt][r], -e);
+            *(f16x4 *)(ws_o + (size_t)row * kHeadDim + 16 * mt + 4 * g) = h;
+          }
           if (g == 0) {
-            ws_ml[2 * row] = m[t];
-            ws_ml[2 * row + 1] = lt;
+            ws_ml[2 * row] = m[t] + (float)e;
+            ws_ml[2 * row + 1] = ldexpf(lt, -e);
           }
         }
       }
     }
     u += n;
   }
-  if (kvh == 0 && tid == 0) p.ws_rec[range] = rec;
 }
 
 // Joins the pieces of a tile that range ends cut: out = sum 2^(m - M) o / (sum 2^(m - M) l + 2^(sink - M)).
-// At most one tile begins in a range without ending there (its record).  A workgroup takes four
-// tokens of it: 32 rows x 4 quarters of the dims x every other piece, two pieces at a time.
+// Eight lanes take a row, PG lane groups every PG-th of its pieces, four at a time; a workgroup holds
+// 32 / PG rows of one tile.
+template <int PG>
 __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeParams p, const int tile_tok) {
+  constexpr int kTokens = 4 / PG;  // of a workgroup (PG 1: four, PG 4: one)
   const int Hkv = p.num_kv_heads, kvh = blockIdx.x % Hkv;
-  const int b = blockIdx.x / Hkv, range = b % p.ranges, tok = b / p.ranges * 4;
-  const TreeRecord rec = p.ws_rec[range];
-  if (tok >= rec.ntok) return;
-  const int pg = threadIdx.x & 1, quarter = (threadIdx.x >> 1) & 3, row = threadIdx.x >> 3;
+  const int b = blockIdx.x / Hkv, tiles = p.num_seqs * p.max_tiles, at = b % tiles, tok = b / tiles * kTokens;
+  const int s = at / p.max_tiles, tok0 = at % p.max_tiles * tile_tok;
+  const const_i32_ptr cu = as_constant(p.cu_seqlens_q), sl = as_constant(p.seq_lens);
+  const TreeSeq v = tree_seq(p, cu[s], cu[s + 1], sl[s], tile_tok);
+  const int ntok = min(v.qlen - tok0, tile_tok);
+  if (tok >= ntok) return;
+  const TreeRecord rec = p.ws_rec[at];
+  if (rec.pieces < 2) return;  // a range held it whole
+  // lane = 8 pg + eighth, so that a row's piece groups are lanes of one wave
+  const int eighth = threadIdx.x & 7, pg = (threadIdx.x >> 3) % PG, row = threadIdx.x / (8 * PG);
   const int tl = tok + (row >> 3), h = row & 7;
   const int rows = tile_tok * kGroup;
-  const size_t cell0 = (size_t)(range * Hkv + kvh) * 2 * rows + tl * kGroup + h;
+  const size_t cell0 = (size_t)(rec.range * Hkv + kvh) * 2 * rows + tl * kGroup + h;
   const int head = kvh * kGroup + h;
-  f32x4 o[4];
+  float o[8], M = kNegBig, den = 0.f;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) o[k] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float M = kNegBig, den = 0.f;
-  if (tl < rec.ntok) {
-    for (int i = pg; i < rec.pieces; i += 4) {
-      float2 ml[2];
-      f32x4 x[2][4];
+  for (int k = 0; k < 8; ++k) o[k] = 0.f;
+  if (tl < ntok) {
+    for (int i = pg; i < rec.pieces; i += 4 * PG) {
+      float2 ml[4];
+      f16x8 x[4];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int j = min(i + 2 * e, rec.pieces - 1);  // (the last one again: its weight is taken away below)
+      for (int e = 0; e < 4; ++e) {
+        const int j = min(i + e * PG, rec.pieces - 1);  // (past the end the last one again, without weight)
         const size_t c = cell0 + (size_t)j * Hkv * 2 * rows + (j == 0 ? rows : 0);
         ml[e] = *(const float2 *)(p.ws_ml + 2 * c);
-        const f32x4 *src = (const f32x4 *)(p.ws_o + c * kHeadDim + 16 * quarter);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) x[e][k] = src[k];
+        x[e] = *(const f16x8 *)(p.ws_o + c * kHeadDim + 8 * eighth);
       }
-      const bool two = i + 2 < rec.pieces;
-      const float M1 = max2(M, two ? max2(ml[0].x, ml[1].x) : ml[0].x);
-      const float a = fast_exp2(M - M1), w0 = fast_exp2(ml[0].x - M1), w1 = fast_exp2(ml[1].x - M1);
-      den = den * a + ml[0].y * w0 + (two ? ml[1].y * w1 : 0.f);
+      float M1 = M;
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
+      for (int e = 0; e < 4; ++e) M1 = i + e * PG < rec.pieces ? max2(M1, ml[e].x) : M1;
+      const float a = fast_exp2(M - M1);
+      den *= a;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[k][r] = o[k][r] * a + x[0][k][r] * w0 + (two ? x[1][k][r] * w1 : 0.f);
+      for (int k = 0; k < 8; ++k) o[k] *= a;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (i + e * PG < rec.pieces) {
+          const float w = fast_exp2(ml[e].x - M1);
+          den += ml[e].y * w;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) o[k] += (float)x[e][k] * w;
+        }
       M = M1;
     }
   }
   const float sink = p.sinks ? p.sinks[head] * kLog2e : -INFINITY;
-  const float all = max2(max2(M, __shfl_xor(M, 1)), sink);
+  float all = M;
+#pragma unroll
+  for (int d = 8; d < 8 * PG; d <<= 1) all = max2(all, __shfl_xor(all, d));
+  all = max2(all, sink);
   const float a = fast_exp2(M - all);
   den *= a;
-  den += __shfl_xor(den, 1);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) o[k] *= a;
+#pragma unroll
+  for (int d = 8; d < 8 * PG; d <<= 1) {
+    den += __shfl_xor(den, d);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) o[k] += __shfl_xor(o[k], d);
+  }
   den += fast_exp2(sink - all);
-#pragma unroll
-  for (int k = 0; k < 4; ++k)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const float x = o[k][r] * a;
-      o[k][r] = x + __shfl_xor(x, 1);
-    }
-  if (tl >= rec.ntok) return;
+  if (tl >= ntok || pg > 0) return;
   const float vs = p.v_scale ? p.v_scale[kvh] : 1.0f;
   const bool any = den > 0.f || den != den;
   const float f = any ? vs / den : 0.f;
-  const size_t orow = (size_t)(rec.row + tl) * p.num_q_heads + head;
-  const f32x4 lo = pg ? o[2] : o[0], hi = pg ? o[3] : o[1];  // each of the two stores eight dims
+  const size_t orow = (size_t)(v.row0 + tok0 + tl) * p.num_q_heads + head;
   u32x4 w;
-  w[0] = pack_bf16(lo[0] * f, lo[1] * f);
-  w[1] = pack_bf16(lo[2] * f, lo[3] * f);
-  w[2] = pack_bf16(hi[0] * f, hi[1] * f);
-  w[3] = pack_bf16(hi[2] * f, hi[3] * f);
-  *(u32x4 *)(p.out + orow * kHeadDim + 16 * quarter + 8 * pg) = w;
-  if (p.lse && pg == 0 && quarter == 0) p.lse[orow] = any ? (all + __log2f(den)) * kLn2 : -INFINITY;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) w[k] = pack_bf16(o[2 * k] * f, o[2 * k + 1] * f);
+  *(u32x4 *)(p.out + orow * kHeadDim + 8 * eighth) = w;
+  if (p.lse && eighth == 0) p.lse[orow] = any ? (all + __log2f(den)) * kLn2 : -INFINITY;
 }
 
 }  // namespace
@@ -767,8 +802,11 @@ hipError_t launch_tree(const TreeParams &p, const bool fp8, hipStream_t st) {
 }
 
 hipError_t launch_tree_merge(const TreeParams &p, hipStream_t st) {
+  // many pieces of few tiles: their pieces side by side
   const int tile = tree_tile_tokens(p.max_q_len);
-  tree_merge_kernel<<<(unsigned)(p.ranges * p.num_kv_heads * (tile / 4)), 256, 0, st>>>(p, tile);
+  const unsigned tiles = (unsigned)(p.num_seqs * p.max_tiles), cells = tiles * (unsigned)p.num_kv_heads;
+  if ((unsigned)p.ranges > 4 * tiles) tree_merge_kernel<4><<<cells * tile, 256, 0, st>>>(p, tile);
+  else tree_merge_kernel<1><<<cells * (tile / 4), 256, 0, st>>>(p, tile);
   return hipGetLastError();
 }
 

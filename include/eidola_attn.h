@@ -325,7 +325,8 @@ int32_t eid_qkv_rope_kv_write(const eid_attn_desc *desc, const void *hidden, con
  * host copies of the lengths, k_new / v_new (must be NULL) and desc->partition_size play no part.
  * split_done_event is recorded behind the first of the two launches.  `out` rows of no sequence
  * (behind cu_seqlens_q[num_seqs]) are left as they were.
- * Partial results are kept in fp32; the softmax weights enter the value product as bf16.
+ * Sums are fp32; the softmax weights enter the value product as bf16, and the outputs of pieces of a
+ * long context are kept as fp16 beside a power of two per row.
  * Reference counterpart: none.  Engine call site: per layer of a verification step, in place of
  * eid_attn_varlen.
  */
