@@ -1146,6 +1146,7 @@ namespace {
 
 struct TreePlan {
   int32_t ranges, max_tiles;  // workgroups per KV head, tiles of the longest tree
+  bool whole;                 // a workgroup per tile: nothing is cut, nothing is joined
   size_t rec_bytes, o_bytes, ml_bytes;
   size_t total() const { return rec_bytes + o_bytes + ml_bytes; }
 };
@@ -1165,6 +1166,17 @@ TreePlan make_tree_plan(const eid_attn_desc *d) {
   const long long fill = std::max(1, 2 * eid::device_cus() / d->num_kv_heads);
   const long long most = (chunks + eid::kTreeMinChunks - 1) / eid::kTreeMinChunks;
   pl.ranges = (int32_t)std::max(1LL, std::min(fill, most));
+  // Short spans (windows among them): cutting a tile costs a piece written, read and joined by a second
+  // launch, which is more than eight chunks take (32 x 24 tokens in a window of 128: 26 us cut).
+  long long span = d->max_kv_len;
+  if (d->window > 0) span = std::min(span, (long long)d->window + d->max_q_len + eid::kBlock);
+  pl.whole = span <= eid::kTreeWholeChunks * eid::kChunk;
+  if (pl.whole) {
+    pl.ranges = (int32_t)(d->num_seqs * tiles);
+    pl.rec_bytes = 256;  // (a workspace has to be somewhere)
+    pl.o_bytes = pl.ml_bytes = 0;
+    return pl;
+  }
   const size_t rows = (size_t)pl.ranges * d->num_kv_heads * 2 * tile * eid::kGroup;
   pl.rec_bytes = ((size_t)d->num_seqs * tiles * sizeof(eid::TreeRecord) + 255) / 256 * 256;
   pl.o_bytes = rows * eid::kHeadDim * sizeof(_Float16);
@@ -1293,6 +1305,7 @@ int32_t eid_attn_tree(const eid_attn_desc *desc, const eid_attn_args *args, cons
   p.max_tiles = pl.max_tiles;
   p.ranges = pl.ranges;
   p.min_chunks = eid::kTreeMinChunks;
+  p.whole = pl.whole ? 1 : 0;
   p.softmax_scale = desc->softmax_scale;
   hipStream_t st = static_cast<hipStream_t>(hip_stream);
   hipError_t e = eid::launch_tree(p, fp8, st);
@@ -1301,7 +1314,7 @@ int32_t eid_attn_tree(const eid_attn_desc *desc, const eid_attn_args *args, cons
     e = hipEventRecord(static_cast<hipEvent_t>(args->split_done_event), st);
     if (e != hipSuccess) return hip_fail(e, "split_done_event record");
   }
-  if (pl.ranges > 1) {  // (one range holds every row whole)
+  if (!pl.whole && pl.ranges > 1) {  // (else every row is whole)
     e = eid::launch_tree_merge(p, st);
     if (e != hipSuccess) return hip_fail(e, "tree merge launch");
   }

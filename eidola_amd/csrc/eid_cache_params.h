@@ -9,6 +9,7 @@ constexpr int kTreeWordsMax = 4;              // mask words per drafted token
 constexpr int kTreeMax = 64 * kTreeWordsMax;  // drafted tokens per sequence
 constexpr int kTreeWaves = 4;
 constexpr int kTreeMinChunks = 2;             // 64-key chunks per workgroup of a range, at least
+constexpr int kTreeWholeChunks = 8;           // sequences of up to so many chunks are not cut
 
 // Where the pieces of a tile of drafted tokens are.
 struct TreeRecord {
@@ -31,6 +32,7 @@ struct TreeParams {
   int32_t num_q_tokens, mask_words, window, max_q_len, max_kv_len;
   int32_t max_tiles;  // tiles of the longest tree
   int32_t ranges;     // workgroups per KV head
+  int32_t whole;      // 1: a range per (sequence, tile), nothing is cut
   int32_t min_chunks; // smallest range
   float softmax_scale;
 };

@@ -87,7 +87,7 @@ __device__ __forceinline__ TreePlace find_place(const TreeParams &p, const int r
   return w;
 }
 __device__ __forceinline__ TreeSeq seq_at(const TreeParams &p, const TreePlace &w, const int s, const int tile_tok) {
-  if (p.num_seqs <= 64)
+  if (!p.whole && p.num_seqs <= 64)
     return tree_seq(p, __builtin_amdgcn_readlane(w.lane_row0, s), __builtin_amdgcn_readlane(w.lane_row1, s),
                     __builtin_amdgcn_readlane(w.lane_len, s), tile_tok);
   const const_i32_ptr cu = as_constant(p.cu_seqlens_q), sl = as_constant(p.seq_lens);
@@ -138,7 +138,6 @@ typedef __attribute__((address_space(1))) const void gptr_t;
 typedef __attribute__((address_space(3))) void lptr_t;
 constexpr int kTileBytes = kChunk * 128;
 
-typedef __attribute__((ext_vector_type(4))) _Float16 f16x4;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 // e with |x| in [2^(e-1), 2^e); 0 for 0
 __device__ __forceinline__ int top_exponent(const float x) {
@@ -176,6 +175,8 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_kernel(const TreePara
   __shared__ __align__(16) uint8_t lds_q[QLDS ? kTreeWaves * 2 * NT * 1024 : 16];
   __shared__ uint64_t lds_mask[kTok][kTreeWordsMax];
   __shared__ int lds_lo[kTok];
+  __shared__ int lds_depth[kTreeMax];
+  static_assert(kTreeMax == kTreeWaves * 64, "a thread per token of the longest tree");
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i16 = lane & 15, g = lane >> 4;
@@ -184,7 +185,17 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_kernel(const TreePara
   const float c2 = p.softmax_scale * kLog2e * (FP8 ? p.k_scale[kvh] : 1.0f);
   const float vs = FP8 ? p.v_scale[kvh] : 1.0f;
 
-  const TreePlace place = find_place(p, range, kTok);
+  TreePlace place;
+  if (p.whole) {  // a range is one tile of one sequence
+    place.seq = range / p.max_tiles;
+    place.per = 0x7fffffff;
+    const TreeSeq v = seq_at(p, place, place.seq, kTok);
+    place.before = 0;
+    place.u = range % p.max_tiles * v.chunks;
+    place.u_end = range % p.max_tiles < v.tiles ? place.u + v.chunks : place.u;
+  } else {
+    place = find_place(p, range, kTok);
+  }
   Frag8 ones;
   ones.u = u32x4{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
   asm volatile("" : "+v"(ones.u));  // (kept in registers)
@@ -259,56 +270,64 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_kernel(const TreePara
     };
 
     __syncthreads();  // (the last piece's readers are done)
-    // the first two chunks are requested before anything else of the piece is looked at
+    // Requested together: the first chunks' pages, the rows of q (row i16 of 16-row tile t is token
+    // 2 t + i16 / 8, head i16 % 8; tokens past the end repeat the last), the masks; then the chunks.
+    int pages[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) pages[i] = page_at(t_begin + i * kChunk);
+    Frag8 qx[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int tok = tok0 + min(wtok + 2 * t + (i16 >> 3), ntok - 1);
+      const uint16_t *src = p.q + ((size_t)(v.row0 + tok) * p.num_q_heads + kvh * kGroup + (i16 & 7)) * kHeadDim + 16 * g;
+      qx[t][0].u = *(const u32x4 *)src;
+      qx[t][1].u = *(const u32x4 *)(src + 8);
+    }
+    // bits of tokens of this sequence in word w of a row's mask
+    auto mask_word = [&](const int tok, const int w) {
+      const uint64_t m = p.mask[(size_t)(v.row0 + min(tok, v.qlen - 1)) * p.mask_words + min(w, p.mask_words - 1)];
+      const int left = tok < v.qlen ? v.qlen - 64 * w : 0;
+      return left <= 0 ? 0 : left < 64 ? m & ((1ull << left) - 1) : m;
+    };
+    uint64_t mine[kTreeWordsMax];
+    if (tid < kTok) {
+#pragma unroll
+      for (int w = 0; w < kTreeWordsMax; ++w) mine[w] = mask_word(tok0 + tid, w);
+    }
     u32x4 ka, va, kb, vb;  // fp8: two chunks under way
-    int page = page_at(t_begin), page_next = page_at(t_begin + kChunk);
+    int page = pages[0];
     if constexpr (FP8) {
-      fetch8(t_begin, page, ka, va);
-      if (DEEP8 && t_begin + kChunk < t_end) fetch8(t_begin + kChunk, page_next, kb, vb);
+      fetch8(t_begin, pages[0], ka, va);
+      if (DEEP8 && t_begin + kChunk < t_end) fetch8(t_begin + kChunk, pages[1], kb, vb);
     } else {
-      dma(k_st0, v_st0, t_begin, page);
+      dma(k_st0, v_st0, t_begin, pages[0]);
       if constexpr (ST == 4) {
-        if (t_begin + kChunk < t_end) dma(k_st1, v_st1, t_begin + kChunk, page_next);
-        if (t_begin + 2 * kChunk < t_end) dma(k_st2, v_st2, t_begin + 2 * kChunk, page_at(t_begin + 2 * kChunk));
+        if (t_begin + kChunk < t_end) dma(k_st1, v_st1, t_begin + kChunk, pages[1]);
+        if (t_begin + 2 * kChunk < t_end) dma(k_st2, v_st2, t_begin + 2 * kChunk, pages[2]);
       }
     }
-
-    // ---- Q operands: row i16 of 16-row tile t is token 2 t + i16 / 8, head i16 % 8
     Frag8 qf[QLDS ? 2 : NT][2];
     uint8_t *q_lds = lds_q + (QLDS ? wave * (2 * NT * 1024) + lane * 16 : 0);
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int tl = wtok + 2 * t + (i16 >> 3);
-      Frag8 x[2];
-      x[0].u = x[1].u = u32x4{0, 0, 0, 0};
-      if (tl < ntok) {
-        const uint16_t *src = p.q + ((size_t)(v.row0 + tok0 + tl) * p.num_q_heads + kvh * kGroup + (i16 & 7)) * kHeadDim + 16 * g;
-        x[0].u = *(const u32x4 *)src;
-        x[1].u = *(const u32x4 *)(src + 8);
-      }
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        if constexpr (QLDS) *(u32x4 *)(q_lds + (2 * t + h) * 1024) = x[h].u;  // (read by this lane alone)
-        else qf[t][h] = x[h];
+        if constexpr (QLDS) *(u32x4 *)(q_lds + (2 * t + h) * 1024) = qx[t][h].u;  // (read by this lane alone)
+        else qf[t][h] = qx[t][h];
       }
-    }
-    // ---- the tile's masks: bits of tokens of this sequence, those outside the window taken out
     if (tid < kTok) {
-      const int tok = tok0 + tid;
       int depth = -1;
 #pragma unroll
       for (int w = 0; w < kTreeWordsMax; ++w) {
-        uint64_t m = 0;
-        if (tok < v.qlen && w < p.mask_words) m = p.mask[(size_t)(v.row0 + tok) * p.mask_words + w];
-        const int left = v.qlen - 64 * w;
-        if (left <= 0) m = 0;
-        else if (left < 64) m &= (1ull << left) - 1;
-        lds_mask[tid][w] = m;
-        depth += __popcll(m);
+        lds_mask[tid][w] = mine[w];
+        depth += __popcll(mine[w]);
       }
       lds_lo[tid] = p.window > 0 ? prefix + depth - p.window + 1 : 0;
     }
     if (p.window > 0 && p.window < v.qlen) {  // an ancestor may lie outside the window
+      int depth = -1;  // of token tid of the tree
+      for (int w = 0; w < p.mask_words; ++w) depth += __popcll(mask_word(tid, w));
+      lds_depth[tid] = depth;
       __syncthreads();
       uint64_t keep = 0;
       const int tl = tid / kTreeWordsMax, w = tid % kTreeWordsMax;
@@ -318,16 +337,7 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_kernel(const TreePara
         while (m) {
           const int b = __builtin_ctzll(m);
           m &= m - 1;
-          const int j = 64 * w + b;  // an ancestor: its depth comes from its own mask
-          int dj = -1;
-          for (int x = 0; x < p.mask_words; ++x) {
-            uint64_t a = p.mask[(size_t)(v.row0 + j) * p.mask_words + x];
-            const int left = v.qlen - 64 * x;
-            if (left <= 0) a = 0;
-            else if (left < 64) a &= (1ull << left) - 1;
-            dj += __popcll(a);
-          }
-          if (prefix + dj < lds_lo[tl]) keep &= ~(1ull << b);
+          if (prefix + lds_depth[64 * w + b] < lds_lo[tl]) keep &= ~(1ull << b);
         }
       }
       __syncthreads();
@@ -548,7 +558,7 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_kernel(const TreePara
         if (tc + kChunk < t_end) iter(k_st1, v_st1, k_st0, v_st0, ka, va, kb, vb, tc + kChunk);
       }
     } else {
-      page = page_at(t_begin + (ST - 1) * kChunk);
+      page = ST == 2 ? pages[1] : page_at(t_begin + (ST - 1) * kChunk);
       // (the first chunk's loads are the oldest; the rows of q behind them have to be here as well)
       __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
       __syncthreads();
@@ -635,7 +645,7 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_kernel(const TreePara
     const int part = c0 == 0 ? 1 : 0;  // a range holds at most one piece of each kind that is not whole
     _Float16 *ws_o = p.ws_o + ((size_t)(range * Hkv + kvh) * 2 + part) * (kRows * kHeadDim);
     float *ws_ml = p.ws_ml + ((size_t)(range * Hkv + kvh) * 2 + part) * (kRows * 2);
-    if (c0 == 0 && kvh == 0 && tid == 0) {  // the tile begins here: where its pieces are
+    if (c0 == 0 && kvh == 0 && tid == 0 && !p.whole) {  // the tile begins here: where its pieces are
       const int last = u + v.chunks - 1;    // its last unit
       p.ws_rec[s * p.max_tiles + tile] = {range, last / place.per - range + 1};
     }
@@ -678,11 +688,11 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_kernel(const TreePara
             }
           const int e = top_exponent(rowgroup_max(top));
 #pragma unroll
-          for (int mt = 0; mt < 4; ++mt) {
-            f16x4 h;
+          for (int h = 0; h < 2; ++h) {  // (a lane's 16 dims next to each other: 16 mt + 4 g + r at 16 g + 4 mt + r)
+            f16x8 x;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) h[r] = (_Float16)ldexpf(acc[t][mt][r], -e);
-            *(f16x4 *)(ws_o + (size_t)row * kHeadDim + 16 * mt + 4 * g) = h;
+            for (int i = 0; i < 8; ++i) x[i] = (_Float16)ldexpf(acc[t][2 * h + i / 4][i & 3], -e);
+            *(f16x8 *)(ws_o + (size_t)row * kHeadDim + 16 * g + 8 * h) = x;
           }
           if (g == 0) {
             ws_ml[2 * row] = m[t] + (float)e;
@@ -769,10 +779,11 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeParams p, con
   const bool any = den > 0.f || den != den;
   const float f = any ? vs / den : 0.f;
   const size_t orow = (size_t)(v.row0 + tok0 + tl) * p.num_q_heads + head;
-  u32x4 w;
+  // value 16 g + 4 mt + r of a piece is dim 16 mt + 4 g + r
+  uint16_t *dst = p.out + orow * kHeadDim + 4 * (eighth >> 1) + 32 * (eighth & 1);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) w[k] = pack_bf16(o[2 * k] * f, o[2 * k + 1] * f);
-  *(u32x4 *)(p.out + orow * kHeadDim + 8 * eighth) = w;
+  for (int k = 0; k < 2; ++k)
+    *(u32x2 *)(dst + 16 * k) = u32x2{pack_bf16(o[4 * k] * f, o[4 * k + 1] * f), pack_bf16(o[4 * k + 2] * f, o[4 * k + 3] * f)};
   if (p.lse && eighth == 0) p.lse[orow] = any ? (all + __log2f(den)) * kLn2 : -INFINITY;
 }
 
