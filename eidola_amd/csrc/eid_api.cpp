@@ -1167,10 +1167,15 @@ TreePlan make_tree_plan(const eid_attn_desc *d) {
   const long long most = (chunks + eid::kTreeMinChunks - 1) / eid::kTreeMinChunks;
   pl.ranges = (int32_t)std::max(1LL, std::min(fill, most));
   // Short spans (windows among them): cutting a tile costs a piece written, read and joined by a second
-  // launch, which is more than eight chunks take (32 x 24 tokens in a window of 128: 26 us cut).
+  // launch, which is more than a few chunks take: 1 x 8 tokens behind 500, 8 chunks, 14 us whole and
+  // 17 us cut, behind 1,000 20 and 17; with 17 and more tokens a chunk takes longer: 1 x 30 behind
+  // 500 23 whole, 17 cut; 32 x 24 in a window of 128, 3 chunks, 16 and 26.  When the tiles fill the device
+  // by themselves cutting gains nothing for longer: 64 x 8 behind 1,000 31 and 34, 64 x 24 behind 500 33 and 36.
   long long span = d->max_kv_len;
   if (d->window > 0) span = std::min(span, (long long)d->window + d->max_q_len + eid::kBlock);
-  pl.whole = span <= eid::kTreeWholeChunks * eid::kChunk;
+  const bool full = d->num_seqs * tiles * d->num_kv_heads >= 2 * eid::device_cus();
+  const int most_whole = full ? 16 : tile <= 16 ? 8 : 4;
+  pl.whole = span <= most_whole * eid::kChunk;
   if (pl.whole) {
     pl.ranges = (int32_t)(d->num_seqs * tiles);
     pl.rec_bytes = 256;  // (a workspace has to be somewhere)

@@ -9,7 +9,6 @@ constexpr int kTreeWordsMax = 4;              // mask words per drafted token
 constexpr int kTreeMax = 64 * kTreeWordsMax;  // drafted tokens per sequence
 constexpr int kTreeWaves = 4;
 constexpr int kTreeMinChunks = 2;             // 64-key chunks per workgroup of a range, at least
-constexpr int kTreeWholeChunks = 8;           // sequences of up to so many chunks are not cut
 
 // Where the pieces of a tile of drafted tokens are.
 struct TreeRecord {
