@@ -138,6 +138,215 @@ __global__ __launch_bounds__(512) void score_few_kernel(const ScoreParams p) {
 }
 
 // ---------------------------------------------------------------------------------------
+// The same with KV heads in groups of eight, as a stream.  The launch's 64-key chunks (from the first a
+// window reaches) stand in a line, cut into equal ranges, and a wave walks a range for one head (two of
+// an fp8 cache, whose rows are half a line) with two chunks under way through direct global -> LDS
+// loads, whole 128-byte rows at a time, without barriers: its tiles are its own.
+// 64 sequences of one row behind 8192 bf16 keys, 8 KV heads: 102 us, 5.6 TB/s (117 us from the kernel
+// above, which picks every row up in halves; 116 us here without the non-temporal hint); fp8 63 us
+// (72).  A window of 128 behind 128 x 4096 keys: 8.4 us (47: most workgroups of a grid over all
+// chunks find nothing to do).  One sequence of 500: 4.1 us (4.7); fp8 8 x 8192 alone loses, 13.1 (12.3).
+// ---------------------------------------------------------------------------------------
+typedef __attribute__((address_space(1))) const void gptr_t;
+typedef __attribute__((address_space(3))) void lptr_t;
+constexpr int kStreamTile = kChunk * 128;      // K rows of a chunk
+
+// One cursor of a stream: a chunk of a sequence.
+struct StreamPos {
+  int s, chunk, chunks, begin;
+  ScoreSeq v;
+};
+struct Pages {
+  int a, b, c, d;
+};
+__device__ __forceinline__ int stream_chunks(const ScoreParams &p, const ScoreSeq &v, int &begin) {
+  begin = p.window > 0 ? max(0, v.len - v.qlen - p.window + 1) & ~(kChunk - 1) : 0;
+  return v.qlen >= 1 && v.qlen <= kScoreFewRows ? (v.len - begin + kChunk - 1) / kChunk : 0;
+}
+
+template <bool FP8>
+__global__ __launch_bounds__(FP8 ? 256 : 512, 2) void score_stream_kernel(const ScoreParams p) {
+  constexpr int kHeads = FP8 ? 2 : 1, kWaves = 8 / kHeads;
+  constexpr int kWave = kStreamTile + kHeads * 256;  // a wave's tile: the rows, and the old scores
+  __shared__ __align__(1024) uint8_t tile0[kWaves * kWave], tile1[kWaves * kWave];
+  const int lane = threadIdx.x & 63, i16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int groups = p.num_kv_heads / 8;
+  const int kvh = blockIdx.x % groups * 8 + wave * kHeads, range = blockIdx.x / groups;
+  const uint32_t row_bytes = (uint32_t)p.num_kv_heads * (128 / kHeads);
+  const size_t page_bytes = (size_t)kBlock * row_bytes;
+  float c2[kHeads];
+#pragma unroll
+  for (int h = 0; h < kHeads; ++h) c2[h] = p.softmax_scale * kLog2e * (FP8 ? p.k_scale[kvh + h] : 1.0f);
+
+  // this range of the line
+  int total = 0;
+  auto units_at = [&](const int s) {
+    ScoreSeq v;
+    v.row0 = v.qlen = v.len = 0;
+    if (s < p.num_seqs) {
+      v.row0 = p.cu_seqlens_q[s];
+      v.qlen = p.cu_seqlens_q[s + 1] - v.row0;
+      v.len = min(p.seq_lens[s], p.max_kv_len);
+      if (v.qlen < 0 || v.len < v.qlen || v.row0 < 0 || v.row0 + v.qlen > p.num_q_tokens) v.qlen = 0;
+    }
+    int begin;
+    return stream_chunks(p, v, begin);
+  };
+  auto scan = [&](const int n) {
+    int incl = n;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(incl, d);
+      if (lane >= d) incl += o;
+    }
+    return incl;
+  };
+  int n = 0, incl = 0;
+  for (int s0 = 0; s0 < p.num_seqs; s0 += 64) {
+    n = units_at(s0 + lane);
+    incl = scan(n);
+    total += __builtin_amdgcn_readlane(incl, 63);
+  }
+  const int per = (total + p.ranges - 1) / p.ranges;
+  int left = min(total - range * per, per);  // units of this range (per > 0 where total > 0)
+  if (left <= 0) return;
+  StreamPos at;  // the next chunk to be requested
+  for (int s0 = 0, base = 0;; s0 += 64) {
+    if (p.num_seqs > 64) {
+      n = units_at(s0 + lane);
+      incl = scan(n);
+    }
+    const int sum = __builtin_amdgcn_readlane(incl, 63);
+    if (base + sum > range * per) {  // (the unit exists: some batch holds it)
+      const int i = __builtin_ctzll(__ballot(base + incl > range * per));
+      at.s = s0 + i;
+      at.chunk = range * per - (base + __builtin_amdgcn_readlane(incl, i) - __builtin_amdgcn_readlane(n, i));
+      break;
+    }
+    base += sum;
+  }
+  at.v = score_seq(p, at.s);
+  at.chunks = stream_chunks(p, at.v, at.begin);
+  auto advance = [&](StreamPos &c) {  // (called only while units are left in the range)
+    if (++c.chunk < c.chunks) return;
+    c.chunk = 0;
+    do {
+      c.v = score_seq(p, ++c.s);
+      c.chunks = stream_chunks(p, c.v, c.begin);
+    } while (c.chunks == 0);
+  };
+  auto pages_of = [&](const StreamPos &c, Pages &pg) {
+    const const_i32_ptr bt = as_constant(p.block_table + (size_t)c.s * p.max_blocks_per_seq);
+    const int first = (c.begin + c.chunk * kChunk) / kBlock, last = (c.v.len - 1) / kBlock;
+    pg.a = clamp_id(bt[min(first, last)], p.last_block);
+    pg.b = clamp_id(bt[min(first + 1, last)], p.last_block);
+    pg.c = clamp_id(bt[min(first + 2, last)], p.last_block);
+    pg.d = clamp_id(bt[min(first + 3, last)], p.last_block);
+  };
+  // the lane's page of four
+  const int m1 = g == 1 ? -1 : 0, m2 = g == 2 ? -1 : 0, m3 = g == 3 ? -1 : 0, m0 = ~(m1 | m2 | m3);
+  auto of_lane = [&](const Pages &pg) {
+    return (uint32_t)((pg.a & m0) | (pg.b & m1) | (pg.c & m2) | (pg.d & m3));
+  };
+  const int dr = lane >> 3, sl = lane & 7;
+  auto request = [&](const Pages &pg, uint8_t *tile) {
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const int page = b == 0 ? pg.a : b == 1 ? pg.b : b == 2 ? pg.c : pg.d;
+      const uint8_t *base = p.k_cache + (size_t)page * page_bytes + (uint32_t)kvh * (128 / kHeads);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {  // (rows past the end are some page's rows: their weights are not stored)
+        const uint32_t off = (uint32_t)(8 * h + dr) * row_bytes + (uint32_t)(sl ^ (4 * h + (dr >> 1))) * 16;
+        __builtin_amdgcn_global_load_lds((gptr_t *)(base + off), (lptr_t *)(tile + (2 * b + h) * 1024), 16, 0, 2);
+      }
+    }
+    const float *src = p.scores + ((size_t)of_lane(pg) * p.num_kv_heads + kvh) * kBlock + i16;
+#pragma unroll
+    for (int h = 0; h < kHeads; ++h)
+      __builtin_amdgcn_global_load_lds((gptr_t *)(src + h * kBlock), (lptr_t *)(tile + kStreamTile + h * 256), 4, 0, 0);
+  };
+  uint8_t *t0 = tile0 + wave * kWave, *t1 = tile1 + wave * kWave;
+  const uint32_t k_off = (uint32_t)i16 * 128 + (uint32_t)(g ^ ((i16 >> 1) & 7)) * 16;
+
+  StreamPos cur = at;  // the chunk that is computed
+  int asked = 1;       // chunks requested so far
+  Pages pg0, pg1;
+  pages_of(at, pg0);
+  request(pg0, t0);
+  if (asked < left) {
+    advance(at);
+    pages_of(at, pg1);
+    request(pg1, t1);
+    ++asked;
+  }
+  Frag8 qf[kHeads][2];
+  f32x4 off[kHeads];
+  int have = -1;  // sequence of qf and off
+  auto step = [&](uint8_t *tile, Pages &pg, const int u) {
+    if (have != cur.s) {
+#pragma unroll
+      for (int h = 0; h < kHeads; ++h) load_rows<FP8>(p, cur.v, kvh + h, 0, qf[h], off[h]);
+      __builtin_amdgcn_s_waitcnt(0xF70);  // vmcnt(0): no wait for them below
+      have = cur.s;
+    }
+    // younger than this chunk's loads: the next one's, and the stores of the last one
+    if (u + 1 >= left) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    else if (u > 0) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(8 + 2 * kHeads) : "memory");
+    else asm volatile("s_waitcnt vmcnt(%0)" ::"i"(8 + kHeads) : "memory");
+    // (read by hand: the compiler would wait for every load under way before it reads a tile)
+    u32x4 raw[4][2];
+    float old[kHeads];
+    const uint32_t lo = (uint32_t)(uintptr_t)(lptr_t *)tile + k_off, hi = lo ^ 64;
+    const uint32_t at_old = (uint32_t)(uintptr_t)(lptr_t *)tile + kStreamTile + 4 * lane;
+    asm volatile(
+        "ds_read_b128 %0, %10\n ds_read_b128 %1, %11\n ds_read_b128 %2, %10 offset:2048\n"
+        "ds_read_b128 %3, %11 offset:2048\n ds_read_b128 %4, %10 offset:4096\n"
+        "ds_read_b128 %5, %11 offset:4096\n ds_read_b128 %6, %10 offset:6144\n"
+        "ds_read_b128 %7, %11 offset:6144\n ds_read_b32 %8, %12\n ds_read_b32 %9, %12 offset:%13\n"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(raw[0][0]), "=&v"(raw[0][1]), "=&v"(raw[1][0]), "=&v"(raw[1][1]), "=&v"(raw[2][0]),
+          "=&v"(raw[2][1]), "=&v"(raw[3][0]), "=&v"(raw[3][1]), "=&v"(old[0]), "=&v"(old[kHeads - 1])
+        : "v"(lo), "v"(hi), "v"(at_old), "i"((kHeads - 1) * 256)
+        : "memory");  // the operands are in registers: the tile is free
+    const int prefix = cur.v.len - cur.v.qlen, tc = cur.begin + cur.chunk * kChunk;
+    const int mine = tc + g * kBlock + i16;
+    float *dst = p.scores + ((size_t)of_lane(pg) * p.num_kv_heads + kvh) * kBlock + i16;
+    if (asked < left) {
+      advance(at);
+      pages_of(at, pg);
+      request(pg, tile);
+      ++asked;
+    }
+#pragma unroll
+    for (int h = 0; h < kHeads; ++h) {
+      float sum = 0.f;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        Frag8 kf[2];
+        if constexpr (FP8) {
+          fp8x8_to_bf16x8(raw[b][h][0], raw[b][h][1], kf[0].w);
+          fp8x8_to_bf16x8(raw[b][h][2], raw[b][h][3], kf[1].w);
+        } else {
+          kf[0].u = raw[b][0];
+          kf[1].u = raw[b][1];
+        }
+        const int j = tc + b * kBlock + i16, pos = prefix + (g >> 1);
+        const bool see = j <= pos && (p.window <= 0 || pos - j < p.window);
+        const float w = rowgroup_sum(weights(qf[h], kf, off[h], c2[h], see));
+        sum = g == b ? w : sum;
+      }
+      if (mine < cur.v.len) dst[h * kBlock] = (mine < prefix ? old[h] : 0.f) + sum;
+    }
+    if (u + 1 < left) advance(cur);
+  };
+  for (int u = 0; u < left; u += 2) {
+    step(t0, pg0, u);
+    if (u + 1 < left) step(t1, pg1, u + 1);
+  }
+}
+
+// ---------------------------------------------------------------------------------------
 // Sequences of more rows: bound by the exponentials and products.  A wave holds 128 keys of one KV
 // head as operands and walks row pairs; one lane adds up one key's weights, so the sums need no
 // atomics and have one order.  The four waves of a workgroup hold neighbouring keys and walk the
@@ -523,7 +732,13 @@ __global__ __launch_bounds__(THREADS) void compact_kernel(const CompactParams p,
 }  // namespace
 
 hipError_t launch_score(const ScoreParams &p, const bool fp8, const bool few, const bool many, hipStream_t st) {
-  if (few) {
+  if (few && p.num_kv_heads % 8 == 0) {
+    const unsigned grid = (unsigned)(p.ranges * (p.num_kv_heads / 8));
+    if (fp8) score_stream_kernel<true><<<grid, 256, 0, st>>>(p);
+    else score_stream_kernel<false><<<grid, 512, 0, st>>>(p);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  } else if (few) {
     const int waves = p.num_kv_heads < 8 ? p.num_kv_heads : 8;
     const dim3 grid((unsigned)((p.max_kv_len + kChunk - 1) / kChunk), (unsigned)p.num_seqs,
                     (unsigned)((p.num_kv_heads + waves - 1) / waves));

@@ -1213,7 +1213,8 @@ int32_t check_rows_desc(const eid_attn_desc *d) {
 
 int32_t check_score_desc(const eid_attn_desc *d) {
   if (int32_t rc = check_attn_desc(d)) return rc;
-  if (d->max_kv_len > 0x7fff0000 || ((long long)d->max_kv_len / eid::kScoreKeys + 1) * d->num_kv_heads > 0x3fffffffLL)
+  if (d->max_kv_len > 0x7fff0000 || ((long long)d->max_kv_len / eid::kScoreKeys + 1) * d->num_kv_heads > 0x3fffffffLL ||
+      (d->max_kv_len / eid::kChunk + 2LL) * d->num_seqs > 0x3fffffffLL)
     return fail(EID_ERR_UNSUPPORTED, "max_kv_len %d with %d KV heads is too large", d->max_kv_len, d->num_kv_heads);
   return EID_OK;
 }
@@ -1361,6 +1362,12 @@ int32_t eid_kv_score(const eid_attn_desc *desc, const void *q, const float *lse,
   p.k_scale = k_scale;
   p.scores = scores;
   p.parts = pl.parts;
+  {
+    const long long keys = desc->sum_kv_len ? desc->sum_kv_len : (long long)desc->num_seqs * desc->max_kv_len;
+    const long long chunks = keys / eid::kChunk + desc->num_seqs;
+    const long long fill = std::max(1, eid::device_cus() * 8 / std::max(8, desc->num_kv_heads) * (fp8 ? 2 : 1));
+    p.ranges = (int32_t)std::max(1LL, std::min(fill, chunks));
+  }
   p.tile_keys = pl.tile_keys;
   p.ws = static_cast<float *>(workspace);
   p.num_seqs = desc->num_seqs;

@@ -50,6 +50,7 @@ struct ScoreParams {
   float *scores;         // [num_blocks][Hkv][16]
   int32_t num_seqs, num_q_heads, num_kv_heads, max_blocks_per_seq, last_block;
   int32_t num_q_tokens, window, max_q_len, max_kv_len;
+  int32_t ranges;     // workgroups per eight KV heads of the stream kernel
   int32_t parts;      // the rows kernel's rows are shared out over so many workgroups
   int32_t tile_keys;  // max_kv_len, in whole workgroups' keys
   float *ws;          // [parts][num_seqs][Hkv][tile_keys], parts > 1 only

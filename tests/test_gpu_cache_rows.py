@@ -277,3 +277,70 @@ def test_captured_selection_and_move_serve_other_lengths(G):
         assert np.array_equal(keep.cpu().numpy(), rk) and np.array_equal(counts.cpu().numpy(), rc)
         assert np.array_equal(G.cache_host(kd), R.kv_compact(b2, ks, rk, rc, [0, 0], True))
         assert np.array_equal(G.cache_host(vd), R.kv_compact(b2, vs, rk, rc, [0, 0], True))
+
+
+@pytest.mark.parametrize("kv_dtype", [KV_BF16, KV_FP8_E4M3])
+@pytest.mark.parametrize("heads,window", [(8, 0), (8, 100), (16, 0), (16, 33)])
+def test_scores_of_many_sequences(G, heads, window, kv_dtype):
+    # more sequences than lanes, some of more rows than the single-token kernel takes, some of one chunk
+    rng = np.random.default_rng(heads + window)
+    q_lens = [int(n) for n in rng.choice([1, 1, 1, 2, 2, 5], 90)]
+    seq_lens = [int(rng.choice([n, 63, 64, 65, 128, int(rng.integers(n, 500))])) for n in q_lens]
+    seq_lens[40], q_lens[40] = 3000, 1
+    b, q, kc, vc, ks, vs, sinks = R.filled(seq_lens, q_lens, num_kv_heads=heads, window=window, kv_dtype=kv_dtype)
+    lse = lse_of(b, q, kc, vc, sinks, ks, vs)
+    w = pool(b, rng)
+    ref = R.kv_score(b, q, lse, kc, w, ks)
+    for kw in ({}, dict(sum_kv_len=int(b.seq_lens.sum())), dict(max_kv_len=3008)):
+        got = score(G, b, q, lse, kc, w, ks, **kw)
+        assert (np.abs(got - ref) <= REL * ref + 1e-7).all()
+
+
+def test_captured_scores_serve_other_lengths(G):
+    for q_lens in ([1, 2, 1], [70, 3, 1]):
+        b, q, kc, vc, ks, vs, sinks = R.filled([700, 1200, 300], q_lens)
+        w = pool(b, np.random.default_rng(4))
+        cases = []
+        from eidola_amd import synth
+        for lens in (b.seq_lens, np.array([90, 1190, 65]), np.array([70, 600, 1])):
+            n = np.array(lens, np.int32)
+            b2 = synth.Batch("other", b.geom, n, b.q_lens, b.block_table, b.num_blocks, b.seed)
+            lse = lse_of(b2, q, kc, vc, sinks, ks, vs)
+            cases.append((n, lse, R.kv_score(b2, q, lse, kc, w)))
+        w_d, lens_d, lse_d = G.dev(w), G.dev(b.seq_lens), G.dev(cases[0][1])
+        q_d, k_d, bt, cu = G.bf16_dev(q), G.cache_dev(kc), G.dev(b.block_table), G.dev(b.cu_seqlens_q)
+        desc = ea.make_desc(b.geom, num_seqs=3, num_q_tokens=len(q), max_q_len=max(q_lens), max_kv_len=1200,
+                            max_blocks_per_seq=bt.shape[1], num_blocks=k_d.shape[0])
+        ws = torch.empty(max(1, ea.kv_score_workspace_bytes(desc)), dtype=torch.uint8, device="cuda")
+        run = lambda: ea.kv_score(b.geom, q_d, lse_d, k_d, bt, lens_d, cu, w_d, max_q_len=max(q_lens),
+                                  max_kv_len=1200, workspace=ws)
+        run()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            run()
+        for turn in range(5):
+            n, lse, ref = cases[turn % 3]
+            lens_d.copy_(G.dev(n))
+            lse_d.copy_(G.dev(lse))
+            w_d.copy_(G.dev(w))
+            ws.fill_(255)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            got = w_d.cpu().numpy()
+            assert (np.abs(got - ref) <= REL * ref + 1e-7).all()
+            w_d.copy_(G.dev(w))
+            run()
+            assert np.array_equal(got, w_d.cpu().numpy())
+
+
+def test_selection_of_sequences_longer_than_announced(G):
+    b = R.make_batch([9000, 40000, 300], [1] * 3, num_kv_heads=2)
+    rng = np.random.default_rng(5)
+    w = rng.random((b.num_blocks, 2, 16)).astype(np.float32)
+    ref, ref_counts = R.kv_select(b, w, 700, 4, 64)
+    for bound in (300, 8192, 9000, 40000):
+        keep, counts = ea.kv_select(b.geom, G.dev(w), G.dev(b.block_table), G.dev(b.seq_lens), budget=700,
+                                    keep_first=4, keep_last=64, max_kv_len=bound)
+        assert np.array_equal(counts.cpu().numpy(), ref_counts) and np.array_equal(keep.cpu().numpy(), ref)

@@ -254,3 +254,73 @@ def test_a_page_past_two_to_the_32_bytes(G):
     out = ea.attn_tree(b.geom, G.bf16_dev(q), big[0], big[1], G.dev(bt.astype(np.int32)), G.dev(b.seq_lens),
                        G.dev(b.cu_seqlens_q), G.dev(mask), sinks=G.dev(sinks), max_q_len=5, max_kv_len=100)
     assert np.abs(R.f64(G.bits_host(out)) - ref).max() <= MAX_ABS_TOL
+
+
+@pytest.mark.parametrize("kv_dtype", [KV_BF16, KV_FP8_E4M3])
+@pytest.mark.parametrize("q_lens", [[5, 1], [16, 9], [24, 20], [40, 64]])
+def test_scores_that_rise_along_the_context(G, q_lens, kv_dtype):
+    # every row's scores climb along the context, by 14 log2 units from 64 keys to the next, and fall again
+    # behind its third quarter, so that the reference of a row's weights has to follow.  Scores of up to 245
+    # log2 units whose 64 products have one sign: off by at most 64 * 2^-24 * 245 = 9.4e-4, twice that in
+    # the quotient: below the 2^-8 / 2 of the bound.
+    from eidola_amd import synth
+    from helpers import cpu_caches, fp8_scales, logical_tensors, make_batch
+    b = make_batch([1500, 400], q_lens, num_kv_heads=2, kv_dtype=kv_dtype)
+    q, k, v, sinks = logical_tensors(b)
+    u = np.where(np.arange(64) % 3 == 0, 1.0, -0.5).astype(np.float32)
+    t = np.concatenate([np.minimum(np.arange(n), 1.5 * n - np.arange(n)) / 80.0 for n in b.seq_lens])
+    q = synth.f32_to_bf16_bits((0.25 * synth.bf16_bits_to_f32(q) + 3.0 * u).astype(np.float32))
+    k = synth.f32_to_bf16_bits((synth.bf16_bits_to_f32(k) + t[:, None, None] * u).astype(np.float32))
+    ks, vs = fp8_scales(k, v) if b.geom.kv_dtype == KV_FP8_E4M3 else (None, None)
+    kc, vc = cpu_caches(b, k, v, ks, vs)
+    mask = trees(q_lens, 21)
+    for s in (sinks, np.full_like(sinks, -np.inf)):
+        check(G, b, q, kc, vc, mask, s, ks, vs)
+    # the call without lse sums its weights in another way
+    got = ea.attn_tree(b.geom, G.bf16_dev(q), G.cache_dev(kc), G.cache_dev(vc), G.dev(b.block_table),
+                       G.dev(b.seq_lens), G.dev(b.cu_seqlens_q), G.dev(mask), k_scale=G.dev(ks), v_scale=G.dev(vs),
+                       max_q_len=b.max_q_len, max_kv_len=b.max_kv_len)
+    ref, _ = R.attn_tree(b, q, kc, vc, mask, None, ks, vs)
+    tol = 2.5 * R.BF16_HALF_STEP * bound(b, q, kc, vc, mask, None, ks, vs) + 1e-6
+    assert (np.abs(R.f64(G.bits_host(got)) - ref) <= tol).all()
+
+
+@pytest.mark.parametrize("lens,q_lens", [([3000, 700], [6, 4]), ([2500, 64], [30, 64]), ([900, 200], [200, 100])])
+def test_captured_with_contexts_that_are_cut(G, lens, q_lens):
+    b, q, kc, vc, ks, vs, sinks = R.filled(lens, q_lens, num_kv_heads=2)
+    from eidola_amd import synth
+    g = b.geom
+    words = (max(q_lens) + 63) // 64
+    masks = [trees(q_lens, s, words) for s in (1, 2)]
+    lens_d, mask_d = G.dev(b.seq_lens), G.dev(masks[0])
+    q_d, k_d, v_d, bt, cu = G.bf16_dev(q), G.cache_dev(kc), G.cache_dev(vc), G.dev(b.block_table), G.dev(b.cu_seqlens_q)
+    out = torch.empty_like(q_d)
+    desc = ea.make_desc(g, num_seqs=2, num_q_tokens=len(q), max_q_len=max(q_lens), max_kv_len=lens[0],
+                        max_blocks_per_seq=bt.shape[1], num_blocks=k_d.shape[0])
+    ws = torch.empty(ea.attn_tree_workspace_bytes(desc), dtype=torch.uint8, device="cuda")
+    run = lambda: ea.attn_tree(g, q_d, k_d, v_d, bt, lens_d, cu, mask_d, max_q_len=max(q_lens), max_kv_len=lens[0],
+                               out=out, workspace=ws)
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for turn in range(4):
+        n = np.array([[lens[0], lens[1]], [lens[1], lens[1]], [q_lens[0], lens[1]], [lens[0] - 77, q_lens[1]]][turn],
+                     np.int32)
+        n = np.maximum(n, np.array(q_lens, np.int32))
+        m = masks[turn % 2]
+        lens_d.copy_(G.dev(n))
+        mask_d.copy_(G.dev(m))
+        out.zero_()
+        ws.fill_(255)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = G.bits_host(out)
+        b2 = synth.Batch("other", g, n, b.q_lens, b.block_table, b.num_blocks, b.seed)
+        ref, _ = R.attn_tree(b2, q, kc, vc, m, None)
+        tol = 2.5 * R.BF16_HALF_STEP * bound(b2, q, kc, vc, m, None) + 1e-6
+        assert (np.abs(R.f64(got) - ref) <= tol).all()
+        run()
+        assert np.array_equal(got, G.bits_host(out))
