@@ -366,7 +366,8 @@ __global__ __launch_bounds__(kScoreWaves * 64, 3) void score_rows_kernel(const S
   const int s = blockIdx.y, part = blockIdx.z;
   const ScoreSeq v = score_seq(p, s);
   const int prefix = v.len - v.qlen;
-  if (v.qlen <= kScoreFewRows || tc >= v.len || below_window(p, prefix, tc + kScoreKeys)) return;
+  const bool few = v.qlen <= kScoreFewRows;  // one row pair: no parts
+  if (v.qlen < 1 || (few && (part > 0 || !p.all_rows)) || tc >= v.len || below_window(p, prefix, tc + kScoreKeys)) return;
   const const_i32_ptr bt = as_constant(p.block_table + (size_t)s * p.max_blocks_per_seq);
   const int last_page = (v.len - 1) / kBlock;
   const uint32_t row_bytes = (uint32_t)p.num_kv_heads * kHeadDim * (FP8 ? 1 : 2);
@@ -453,7 +454,7 @@ __global__ __launch_bounds__(kScoreWaves * 64, 3) void score_rows_kernel(const S
     }
     const int j = tc + (4 * h + g) * kBlock + i16;
     if (j >= v.len) continue;
-    if (p.parts > 1) p.ws[(((size_t)part * p.num_seqs + s) * p.num_kv_heads + kvh) * p.tile_keys + j] = w;
+    if (p.parts > 1 && !few) p.ws[(((size_t)part * p.num_seqs + s) * p.num_kv_heads + kvh) * p.tile_keys + j] = w;
     else add_score(p, s, kvh, j, prefix, w);
   }
 }
@@ -731,7 +732,8 @@ __global__ __launch_bounds__(THREADS) void compact_kernel(const CompactParams p,
 
 }  // namespace
 
-hipError_t launch_score(const ScoreParams &p, const bool fp8, const bool few, const bool many, hipStream_t st) {
+hipError_t launch_score(const ScoreParams &p, const bool fp8, const bool many, hipStream_t st) {
+  const bool few = !many || !p.all_rows;
   if (few && p.num_kv_heads % 8 == 0) {
     const unsigned grid = (unsigned)(p.ranges * (p.num_kv_heads / 8));
     if (fp8) score_stream_kernel<true><<<grid, 256, 0, st>>>(p);

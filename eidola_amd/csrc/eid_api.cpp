@@ -57,7 +57,7 @@ hipError_t launch_kv_write(const uint16_t *k_new, const uint16_t *v_new, uint8_t
 int tree_tile_tokens(int max_q_len);
 hipError_t launch_tree(const TreeParams &p, bool fp8, hipStream_t st);
 hipError_t launch_tree_merge(const TreeParams &p, hipStream_t st);
-hipError_t launch_score(const ScoreParams &p, bool fp8, bool few, bool many, hipStream_t st);
+hipError_t launch_score(const ScoreParams &p, bool fp8, bool many, hipStream_t st);
 hipError_t launch_select(const SelectParams &p, hipStream_t st);
 hipError_t launch_compact(const CompactParams &p, int num_layers, hipStream_t st);
 }  // namespace eid
@@ -1362,12 +1362,10 @@ int32_t eid_kv_score(const eid_attn_desc *desc, const void *q, const float *lse,
   p.k_scale = k_scale;
   p.scores = scores;
   p.parts = pl.parts;
-  {
-    const long long keys = desc->sum_kv_len ? desc->sum_kv_len : (long long)desc->num_seqs * desc->max_kv_len;
-    const long long chunks = keys / eid::kChunk + desc->num_seqs;
-    const long long fill = std::max(1, eid::device_cus() * 8 / std::max(8, desc->num_kv_heads) * (fp8 ? 2 : 1));
-    p.ranges = (int32_t)std::max(1LL, std::min(fill, chunks));
-  }
+  const long long keys = desc->sum_kv_len ? desc->sum_kv_len : (long long)desc->num_seqs * desc->max_kv_len;
+  const long long chunks = keys / eid::kChunk + desc->num_seqs;
+  const long long fill = std::max(1, eid::device_cus() * 8 / std::max(8, desc->num_kv_heads) * (fp8 ? 2 : 1));
+  p.ranges = (int32_t)std::max(1LL, std::min(fill, chunks));
   p.tile_keys = pl.tile_keys;
   p.ws = static_cast<float *>(workspace);
   p.num_seqs = desc->num_seqs;
@@ -1380,11 +1378,16 @@ int32_t eid_kv_score(const eid_attn_desc *desc, const void *q, const float *lse,
   p.max_q_len = desc->max_q_len;
   p.max_kv_len = desc->max_kv_len;
   p.softmax_scale = desc->softmax_scale;
-  // Sequences are sorted into two classes by their rows on the device; when every sequence has
-  // max_q_len rows (num_q_tokens says so) only one of them is populated.
-  const bool uniform = (int64_t)desc->num_seqs * desc->max_q_len == desc->num_q_tokens;
+  // Sequences are sorted into two classes by their rows on the device.  In a launch that may hold both,
+  // those of few rows get a kernel of their own, which reads keys faster than the rows kernel does,
+  // where that pays for the launch.  One sequence of 64 rows and others of one, all behind 8192 bf16
+  // keys, 8 KV heads, us with the launch / without: 8 sequences 39 / 34, 16 50 / 48, 32 75 / 91, 128
+  // 232 / 344; fp8 32 57 / 69.  Where num_q_tokens leaves none to be expected the rows kernel takes
+  // what there is all the same (a padded batch may hold some).
   const bool many = desc->max_q_len > eid::kScoreFewRows;
-  const hipError_t e = eid::launch_score(p, fp8, !many || !uniform, many, static_cast<hipStream_t>(hip_stream));
+  const bool uniform = (int64_t)desc->num_seqs * desc->max_q_len == desc->num_q_tokens;
+  p.all_rows = many && (uniform || keys * desc->num_kv_heads <= eid::kScoreOwnKeys);
+  const hipError_t e = eid::launch_score(p, fp8, many, static_cast<hipStream_t>(hip_stream));
   if (e != hipSuccess) return hip_fail(e, "kv_score launch");
   return EID_OK;
 }

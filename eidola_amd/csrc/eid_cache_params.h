@@ -36,6 +36,7 @@ struct TreeParams {
   float softmax_scale;
 };
 
+constexpr long long kScoreOwnKeys = 1 << 20;  // keys x KV heads beyond which sequences of few rows get their own launch
 constexpr int kScoreFewRows = 2;   // q_len that the few-rows kernel takes
 constexpr int kScoreWaves = 4;     // of a workgroup of the rows kernel
 constexpr int kScoreKeys = 128;    // keys of a wave of the rows kernel
@@ -51,6 +52,7 @@ struct ScoreParams {
   int32_t num_seqs, num_q_heads, num_kv_heads, max_blocks_per_seq, last_block;
   int32_t num_q_tokens, window, max_q_len, max_kv_len;
   int32_t ranges;     // workgroups per eight KV heads of the stream kernel
+  int32_t all_rows;   // the rows kernel takes sequences of few rows as well
   int32_t parts;      // the rows kernel's rows are shared out over so many workgroups
   int32_t tile_keys;  // max_kv_len, in whole workgroups' keys
   float *ws;          // [parts][num_seqs][Hkv][tile_keys], parts > 1 only

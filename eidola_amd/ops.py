@@ -6,6 +6,7 @@ library.  Nothing here computes attention: if the HIP library is absent the call
 """
 import ctypes as C
 import math
+from array import array
 from dataclasses import dataclass
 
 import numpy as np
@@ -723,8 +724,8 @@ def kv_compact(geom, k_caches, v_caches, block_table, seq_lens, keep, counts, *,
         _need(starts, "starts", i32, dev, (S,))
         first = starts.data_ptr()
     desc = _rows_desc(geom, S, blocks, cache_shape[0])
-    host = (C.c_int64 * len(at))(*at)
-    base = C.addressof(host)
+    host = array("q", at)   # (a ctypes array of 72 takes 4 us more to fill)
+    base = host.buffer_info()[0]
     lib = load_library()
     _launch(dev, lambda stream: lib.eid_kv_compact(
         C.byref(desc), n, base, base + 8 * n, base + 16 * n if scores is not None else None, block_table.data_ptr(),

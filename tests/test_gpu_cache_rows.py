@@ -296,6 +296,19 @@ def test_scores_of_many_sequences(G, heads, window, kv_dtype):
         assert (np.abs(got - ref) <= REL * ref + 1e-7).all()
 
 
+@pytest.mark.parametrize("heads", [2, 8])
+def test_a_padded_batch_may_hold_sequences_of_few_rows(G, heads):
+    # as many tokens as sequences x max_q_len, the sequences themselves shorter: rows of padding behind them
+    b, q, kc, vc, ks, vs, sinks = R.filled([90, 700, 64], [1, 6, 2], num_kv_heads=heads)
+    lse = lse_of(b, q, kc, vc, sinks, ks, vs)
+    w = pool(b, np.random.default_rng(6))
+    ref = R.kv_score(b, q, lse, kc, w)
+    q2, lse2 = np.concatenate([q, q]), np.concatenate([lse, lse])
+    assert len(q2) == 3 * b.max_q_len
+    got = score(G, b, q2, lse2, kc, w)
+    assert (np.abs(got - ref) <= REL * ref + 1e-7).all()
+
+
 def test_captured_scores_serve_other_lengths(G):
     for q_lens in ([1, 2, 1], [70, 3, 1]):
         b, q, kc, vc, ks, vs, sinks = R.filled([700, 1200, 300], q_lens)
