@@ -1318,26 +1318,9 @@ struct WorkItem {
   int seq, part, nparts, row0, qlen, seq_len;
 };
 
-// Inclusive prefix sum over the 64 lanes with DPP adds (row shifts, then the row totals
-// carried over with row_bcast): six dependent VALU ops instead of six LDS-crossbar
-// permutes.  A lane whose DPP source is out of range, or whose row is masked off, adds
-// the `old` operand, 0.
-template <int CTRL, int ROW_MASK>
-__device__ __forceinline__ int dpp_add(const int v) {
-  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROW_MASK, 0xf, false);
-}
-__device__ __forceinline__ int wave_inclusive_scan(int v, const int /*lane*/) {
-  v = dpp_add<0x111, 0xf>(v);  // row_shr:1
-  v = dpp_add<0x112, 0xf>(v);  // row_shr:2
-  v = dpp_add<0x114, 0xf>(v);  // row_shr:4
-  v = dpp_add<0x118, 0xf>(v);  // row_shr:8
-  v = dpp_add<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
-  v = dpp_add<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
-  return v;
-}
 // Sum over the 64 lanes, returned as a wave-uniform (scalar) value.  v must be >= 0.
 __device__ __forceinline__ int wave_total(const int v) {
-  return __builtin_amdgcn_readlane(wave_inclusive_scan(v, 0), 63);
+  return __builtin_amdgcn_readlane(wave_inclusive_scan(v), 63);
 }
 __device__ __forceinline__ long long wave_total64(const long long v) {
   // three 22-bit limbs: each limb's 64-lane sum stays below 2^28
@@ -1488,7 +1471,7 @@ __device__ __forceinline__ bool find_work_item(const AttnParams &p, const int w,
   for (int s0 = 0; s0 < p.num_seqs; s0 += 64) {
     const SeqView v = s0 == 0 ? first : view_seq(p, s0 + lane);
     const int n = num_partitions(p, v.span, P);
-    const int incl = wave_inclusive_scan(n, lane);
+    const int incl = wave_inclusive_scan(n);
     const int total = __builtin_amdgcn_readlane(incl, 63);
     if (w < base + total) {
       const unsigned long long hit = __ballot(base + incl > w);
@@ -1736,7 +1719,7 @@ __device__ __forceinline__ bool even_find_start(const AttnParams &p, const int b
   long long base = 0;
   for (int s0 = 0; s0 < p.num_seqs; s0 += 64) {
     const int n = even_units(p, view_seq(p, s0 + lane).span);
-    const int incl = wave_inclusive_scan(n, lane);
+    const int incl = wave_inclusive_scan(n);
     const int total = __builtin_amdgcn_readlane(incl, 63);
     if (start < base + total) {
       const int rel = (int)(start - base);
@@ -2064,7 +2047,7 @@ __device__ __forceinline__ bool find_prefill_item(const AttnParams &p, const int
     }
     const int n_sorted = __builtin_amdgcn_ds_permute(rank << 2, n);
     const int lane_sorted = __builtin_amdgcn_ds_permute(rank << 2, lane);
-    const int incl = wave_inclusive_scan(n_sorted, lane);
+    const int incl = wave_inclusive_scan(n_sorted);
     const int total = __builtin_amdgcn_readlane(incl, 63);
     if (w < base + total) {
       const unsigned long long hit = __ballot(base + incl > w);

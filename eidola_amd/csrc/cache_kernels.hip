@@ -193,19 +193,10 @@ __global__ __launch_bounds__(FP8 ? 256 : 512, 2) void score_stream_kernel(const 
     int begin;
     return stream_chunks(p, v, begin);
   };
-  auto scan = [&](const int n) {
-    int incl = n;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int o = __shfl_up(incl, d);
-      if (lane >= d) incl += o;
-    }
-    return incl;
-  };
   int n = 0, incl = 0;
   for (int s0 = 0; s0 < p.num_seqs; s0 += 64) {
     n = units_at(s0 + lane);
-    incl = scan(n);
+    incl = wave_inclusive_scan(n);
     total += __builtin_amdgcn_readlane(incl, 63);
   }
   const int per = (total + p.ranges - 1) / p.ranges;
@@ -215,7 +206,7 @@ __global__ __launch_bounds__(FP8 ? 256 : 512, 2) void score_stream_kernel(const 
   for (int s0 = 0, base = 0;; s0 += 64) {
     if (p.num_seqs > 64) {
       n = units_at(s0 + lane);
-      incl = scan(n);
+      incl = wave_inclusive_scan(n);
     }
     const int sum = __builtin_amdgcn_readlane(incl, 63);
     if (base + sum > range * per) {  // (the unit exists: some batch holds it)
@@ -487,11 +478,12 @@ __global__ __launch_bounds__(256) void score_join_kernel(const ScoreParams p) {
 // usual case in the first pass, queue less on one address.  A pass whose digit is kept whole ends
 // the search.
 // ---------------------------------------------------------------------------------------
-// larger = kept first; NaN lowest, -0 = +0
+// larger = kept first, -0 = +0; NaN ranks lowest, as 1: 0 stands for rows that are no candidates, which
+// are therefore never reached (the candidates are at least as many as the rows wanted)
 __device__ __forceinline__ uint32_t order_key(const float x) {
-  if (x != x) return 0u;
-  const uint32_t u = __float_as_uint(x == 0.f ? 0.f : x);
-  return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+  const uint32_t u = __float_as_uint(x + 0.f);  // (-0 + 0 = +0)
+  const uint32_t k = u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+  return x != x ? 1u : k;
 }
 constexpr int kSelThreads = 1024;
 constexpr int kSelBins = 2048, kSelCopies = 4;
@@ -503,10 +495,12 @@ __global__ __launch_bounds__(kSelThreads) void select_kernel(const SelectParams 
   __shared__ uint32_t wave_sum[kWaves];
   __shared__ uint32_t found[3];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int s = blockIdx.x / p.num_kv_heads, kvh = blockIdx.x % p.num_kv_heads;
+  // consecutive workgroups run on different XCDs: neighbouring heads, which share lines, go to one
+  const int n8 = gridDim.x >> 3, id = (int)blockIdx.x < 8 * n8 ? (blockIdx.x & 7) * n8 + (blockIdx.x >> 3) : (int)blockIdx.x;
+  const int s = id / p.num_kv_heads, kvh = id % p.num_kv_heads;
   const int len = max(0, min(p.seq_lens[s], p.max_blocks_per_seq * kBlock));
   const int budget = p.budget;
-  int32_t *keep = p.keep + (size_t)blockIdx.x * budget;
+  int32_t *keep = p.keep + (size_t)id * budget;
   if (kvh == 0 && tid == 0) p.counts[s] = min(len, budget);
   if (len <= budget) {
     for (int i = tid; i < budget; i += THREADS) keep[i] = i < len ? i : -1;
@@ -516,25 +510,29 @@ __global__ __launch_bounds__(kSelThreads) void select_kernel(const SelectParams 
   const int lo = p.keep_first, hi = len - p.keep_last;  // candidates: lo <= j < hi
   const int last_page = (len - 1) / kBlock;
   uint32_t key[RUN];
-  uint32_t cand;  // bit i: key[i] is a candidate
-  // the thread's rows of the block that starts at row j0
+  // row of key[0] in the block that starts at j0; key[4 k + e] is 256 k + e rows behind
+  const int mine = wave * (64 * RUN) + 4 * lane;
   auto load = [&](const int j0) {
-    const int j = j0 + tid * RUN;
-    cand = 0;
-    if (j < hi && j + RUN > lo) {
-      const int from = max(lo - j, 0), to = min(hi - j, RUN);
-      cand = (to >= 32 ? ~0u : (1u << to) - 1) & ~((1u << from) - 1);
+    const int j = j0 + mine;
 #pragma unroll
-      for (int h = 0; h < (RUN + kBlock - 1) / kBlock; ++h) {
-        const int page = clamp_id(bt[min(j / kBlock + h, last_page)], p.last_block);
-        const f32x4 *src = (const f32x4 *)(p.scores + ((size_t)page * p.num_kv_heads + kvh) * kBlock + j % kBlock);
+    for (int i = 0; i < RUN; ++i) key[i] = 0;
+    const int first = j0 + wave * (64 * RUN);  // the wave's rows
+    if (first >= hi) return;
+    f32x4 x[RUN / 4];
+    int page[RUN / 4];
 #pragma unroll
-        for (int q = 0; q < (RUN < kBlock ? RUN : kBlock) / 4; ++q) {
-          const f32x4 x = src[q];
+    for (int k = 0; k < RUN / 4; ++k) page[k] = bt[min((j + 256 * k) / kBlock, last_page)];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) key[kBlock * h + 4 * q + e] = order_key(x[e]);
-        }
-      }
+    for (int k = 0; k < RUN / 4; ++k)
+      x[k] = *(const f32x4 *)(p.scores + ((size_t)clamp_id(page[k], p.last_block) * p.num_kv_heads + kvh) * kBlock + j % kBlock);
+#pragma unroll
+    for (int i = 0; i < RUN; ++i) {
+      key[i] = order_key(x[i / 4][i % 4]);
+    }
+    if (first < lo || first + 64 * RUN > hi) {
+#pragma unroll
+      for (int i = 0; i < RUN; ++i)
+        if ((uint32_t)(j + 256 * (i / 4) + i % 4 - lo) >= (uint32_t)(hi - lo)) key[i] = 0;
     }
   };
   const bool once = len <= kCap;
@@ -554,7 +552,7 @@ __global__ __launch_bounds__(kSelThreads) void select_kernel(const SelectParams 
         if (!once) load(j0);
 #pragma unroll
         for (int i = 0; i < RUN; ++i)
-          if ((cand >> i & 1) && (pass == 0 || ((key[i] ^ cut) & ~(digits << shift)) >> shift == 0))
+          if (pass == 0 ? key[i] != 0 : (key[i] ^ cut) >> shift <= digits)
             atomicAdd(&hist[(key[i] >> shift & digits) * kSelCopies + (lane & (kSelCopies - 1))], 1u);
       }
       __syncthreads();
@@ -563,17 +561,16 @@ __global__ __launch_bounds__(kSelThreads) void select_kernel(const SelectParams 
 #pragma unroll
       for (int c = 0; c < kBins; ++c) {
         u32x4 *h = (u32x4 *)&hist[(kSelBins - 1 - (tid * kBins + c)) * kSelCopies];
-        const u32x4 x = *h;
-        *h = u32x4{0, 0, 0, 0};  // for the next pass
-        n[c] = x[0] + x[1] + x[2] + x[3];
+        n[c] = 0;
+#pragma unroll
+        for (int v = 0; v < kSelCopies / 4; ++v) {
+          const u32x4 x = h[v];
+          h[v] = u32x4{0, 0, 0, 0};  // for the next pass
+          n[c] += x[0] + x[1] + x[2] + x[3];
+        }
         sum += n[c];
       }
-      uint32_t incl = sum;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t o = __shfl_up(incl, d);
-        if (lane >= d) incl += o;
-      }
+      uint32_t incl = (uint32_t)wave_inclusive_scan((int)sum);
       if (lane == 63) wave_sum[wave] = incl;
       __syncthreads();
 #pragma unroll
@@ -600,49 +597,68 @@ __global__ __launch_bounds__(kSelThreads) void select_kernel(const SelectParams 
   for (int i = tid; i < p.keep_first; i += THREADS) keep[i] = i;
   for (int i = tid; i < p.keep_last; i += THREADS) keep[budget - p.keep_last + i] = hi + i;
   if (budget == p.keep_first + p.keep_last) return;
-  // Keys whose searched bits are above those of `cut` stay; of those equal to it all (`whole`), or
-  // the first `want`.
-  const uint32_t edge = cut >> shift;
+  // Keys from `least` on stay: those whose searched bits are above those of `cut`, and those equal to it
+  // if it is kept whole; else the first `want` of the latter stay as well.  In a wave's share of a
+  // block, the rows before (k, lane, e) are those of a lower k, and of the same k in a lower lane or in
+  // the same lane with a lower e.
+  const uint32_t least = whole ? max(cut, 1u) : cut + 1;
   uint32_t base = (uint32_t)p.keep_first, ties = 0;  // rows written, ties passed
-  for (int j0 = 0; j0 < len; j0 += kCap) {
-    if (!once) load(j0);
-    uint32_t stay = 0, tie = 0;  // bits of the thread's rows
-    if (cand) {
-#pragma unroll
-      for (int i = 0; i < RUN; ++i) {
-        const uint32_t k = key[i] >> shift;
-        stay |= (k > edge || (whole && k == edge) ? 1u : 0u) << i;
-        tie |= (!whole && k == edge ? 1u : 0u) << i;
-      }
-      stay &= cand;
-      tie &= cand;
-    }
-    // rows that stay in the low half, ties in the high half (at most kCap <= 32768 each)
-    const uint32_t count = (uint32_t)__popc(stay) | (uint32_t)__popc(tie) << 16;
-    uint32_t incl = count;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const uint32_t o = __shfl_up(incl, d);
-      if (lane >= d) incl += o;
-    }
+  // sum over the workgroup's waves (`all`), and over those before this one
+  auto before = [&](const uint32_t n, uint32_t &all) {
     __syncthreads();  // (the last use of wave_sum)
-    if (lane == 63) wave_sum[wave] = incl;
+    if (lane == 0) wave_sum[wave] = n;
     __syncthreads();
-    uint32_t mine = incl - count, all = 0;
+    uint32_t sum = 0;
+    all = 0;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      if (w < wave) mine += wave_sum[w];
+      if (w < wave) sum += wave_sum[w];
       all += wave_sum[w];
     }
-    const uint32_t t = ties + (mine >> 16);  // ties before this thread's run
-    uint32_t at = base + (mine & 0xFFFFu) + (min(t, want) - min(ties, want));
-    for (uint32_t room = want > t ? want - t : 0; tie && room; --room) {  // the run's first ties
-      stay |= tie & (0u - tie);
-      tie &= tie - 1;
+    return sum;
+  };
+  // rows of the wave among its four-key groups k that pass `test`; calls take(k, rows of the group in
+  // lower lanes) on the way
+  auto ranks = [&](auto test, auto take) {
+    uint32_t n = 0;
+#pragma unroll
+    for (int k = 0; k < RUN / 4; ++k) {
+      uint32_t below = n;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint64_t m = __ballot(test(key[4 * k + e]));
+        below = __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, below));
+        n += (uint32_t)__popcll(m);
+      }
+      take(k, below);
     }
-    for (const int j = j0 + tid * RUN; stay; stay &= stay - 1) keep[at++] = j + __builtin_ctz(stay);
-    base += (all & 0xFFFFu) + (min(ties + (all >> 16), want) - min(ties, want));
-    ties += all >> 16;
+    return n;
+  };
+  auto stays = [&](const uint32_t k) { return k >= least; };
+  auto is_tie = [&](const uint32_t k) { return k == cut; };
+  auto nothing = [](int, uint32_t) {};
+  const uint32_t room = (uint32_t)(budget - p.keep_last);  // (also if scores change under a long selection)
+  for (int j0 = 0; j0 < len; j0 += kCap) {
+    if (!once) load(j0);
+    uint32_t all;
+    if (!whole) {  // (all bits are searched)
+      const uint32_t t = ties + before(ranks(is_tie, nothing), all);
+      ties += all;
+      ranks(is_tie, [&](const int k, uint32_t at) {
+        at += t;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (is_tie(key[4 * k + e]) && at++ < want) key[4 * k + e] = ~0u;
+      });
+    }
+    const uint32_t row = base + before(ranks(stays, nothing), all);
+    base += all;
+    ranks(stays, [&](const int k, uint32_t at) {
+      at += row;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (stays(key[4 * k + e]) && at < room) keep[at++] = j0 + mine + 256 * k + e;
+    });
   }
 }
 

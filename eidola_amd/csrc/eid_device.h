@@ -95,6 +95,24 @@ __device__ __forceinline__ uint32_t fp8_e4m3_encode(float x) {
 }
 
 
+// Inclusive prefix sum over the 64 lanes with DPP adds (row shifts, then the row totals
+// carried over with row_bcast): six dependent VALU ops instead of six LDS-crossbar
+// permutes.  A lane whose DPP source is out of range, or whose row is masked off, adds
+// the `old` operand, 0.
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ int dpp_add(const int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROW_MASK, 0xf, false);
+}
+__device__ __forceinline__ int wave_inclusive_scan(int v) {
+  v = dpp_add<0x111, 0xf>(v);  // row_shr:1
+  v = dpp_add<0x112, 0xf>(v);  // row_shr:2
+  v = dpp_add<0x114, 0xf>(v);  // row_shr:4
+  v = dpp_add<0x118, 0xf>(v);  // row_shr:8
+  v = dpp_add<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
+  v = dpp_add<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
+  return v;
+}
+
 // LDS transpose read (gfx950 ds_read_b64_tr_b16).  Within each 16-lane row, treat the
 // 16 lanes x 4 halfwords addressed by the lanes as a flat array F[lane*4 + e]; lane i
 // receives F[i], F[16+i], F[32+i], F[48+i].

@@ -44,15 +44,6 @@ struct TreePlace {
   int per, u, u_end;  // units per range; this range's
   int seq, before;    // the sequence that holds unit u, and the units before it
 };
-__device__ __forceinline__ int inclusive_scan(int x) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int o = __shfl_up(x, d);
-    if (lane >= d) x += o;
-  }
-  return x;
-}
 __device__ __forceinline__ TreePlace find_place(const TreeParams &p, const int range, const int tile_tok) {
   const int lane = threadIdx.x & 63;
   TreePlace w;
@@ -66,7 +57,7 @@ __device__ __forceinline__ TreePlace find_place(const TreeParams &p, const int r
     }
     const TreeSeq v = tree_seq(p, w.lane_row0, w.lane_row1, w.lane_len, tile_tok);
     n = v.tiles * v.chunks;
-    incl = inclusive_scan(n);
+    incl = wave_inclusive_scan(n);
     return __builtin_amdgcn_readlane(incl, 63);
   };
   for (int s0 = 0; s0 < p.num_seqs; s0 += 64) total += load(s0 + lane);
