@@ -326,7 +326,8 @@ int32_t eid_qkv_rope_kv_write(const eid_attn_desc *desc, const void *hidden, con
  * split_done_event is recorded behind the first of the two launches.  `out` rows of no sequence
  * (behind cu_seqlens_q[num_seqs]) are left as they were.
  * Sums are fp32; the softmax weights enter the value product as bf16, and the outputs of pieces of a
- * long context are kept as fp16 beside a power of two per row.
+ * long context are kept as fp16 beside a power of two per row.  A row's weights may stand up to 2^60
+ * above 1 before they are scaled down: finite values of V beyond 2^48 can overflow.
  * Reference counterpart: none.  Engine call site: per layer of a verification step, in place of
  * eid_attn_varlen.
  */

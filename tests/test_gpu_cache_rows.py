@@ -357,3 +357,44 @@ def test_selection_of_sequences_longer_than_announced(G):
         keep, counts = ea.kv_select(b.geom, G.dev(w), G.dev(b.block_table), G.dev(b.seq_lens), budget=700,
                                     keep_first=4, keep_last=64, max_kv_len=bound)
         assert np.array_equal(counts.cpu().numpy(), ref_counts) and np.array_equal(keep.cpu().numpy(), ref)
+
+
+def test_tensors_that_do_not_fit_are_refused(G):
+    b, q, kc, vc, ks, vs, sinks = R.filled([50, 30], [4, 1], num_kv_heads=2)
+    g, lse = b.geom, np.zeros((5, 16), np.float32)
+    w = torch.zeros((b.num_blocks, 2, 16), device="cuda")
+    base = dict(q=G.bf16_dev(q), lse=G.dev(lse), k_cache=G.cache_dev(kc), block_table=G.dev(b.block_table),
+                seq_lens=G.dev(b.seq_lens), cu_seqlens_q=G.dev(b.cu_seqlens_q), scores=w)
+    def bad(f, good, *changes):
+        for change in changes:
+            with pytest.raises((ValueError, TypeError, ea.EidError)):
+                f(g, **{**good, **change})
+    hints = dict(max_q_len=4, max_kv_len=50)
+    ea.kv_score(g, **base, **hints)
+    bad(lambda *a, **k: ea.kv_score(*a, **{**hints, **k}), base,
+        dict(q=base["q"].float()), dict(q=base["q"][:, :8]), dict(q=base["q"].cpu()), dict(q=base["q"][:4]),
+        dict(lse=base["lse"].double()), dict(lse=base["lse"].t()), dict(k_cache=base["k_cache"][:, :8]),
+        dict(scores=w[:-1]), dict(scores=w.half()), dict(seq_lens=base["seq_lens"].long()), dict(seq_lens=None),
+        dict(cu_seqlens_q=base["cu_seqlens_q"][:2]), dict(max_kv_len=50000), dict(max_q_len=0))
+    tree = dict(q=base["q"], k_cache=base["k_cache"], v_cache=G.cache_dev(vc), block_table=base["block_table"],
+                seq_lens=base["seq_lens"], cu_seqlens_q=base["cu_seqlens_q"],
+                tree_mask=torch.ones((5, 1), dtype=torch.int64, device="cuda"))
+    ea.attn_tree(g, **tree, **hints)
+    bad(lambda *a, **k: ea.attn_tree(*a, **{**hints, **k}), tree,
+        dict(tree_mask=tree["tree_mask"].int()), dict(tree_mask=tree["tree_mask"][:4]), dict(v_cache=tree["v_cache"].cpu()),
+        dict(v_cache=tree["v_cache"][:-1]), dict(max_q_len=300), dict(out=torch.empty_like(base["q"])[:, ::2]),
+        dict(sinks=torch.zeros(3, device="cuda")), dict(max_kv_len=0),
+        dict(workspace=torch.empty(0, dtype=torch.uint8)))
+    sel = dict(scores=w, block_table=base["block_table"], seq_lens=base["seq_lens"])
+    hints = dict(budget=20, max_kv_len=50)
+    keep, counts = ea.kv_select(g, **sel, **hints)
+    bad(lambda *a, **k: ea.kv_select(*a, **{**hints, **k}), sel,
+        dict(scores=w[:, :1]), dict(scores=w.double()), dict(budget=0), dict(keep_first=15, keep_last=6),
+        dict(keep=keep[:, :, :10]), dict(counts=counts.long()), dict(max_kv_len=10 ** 6), dict(block_table=None))
+    k1, v1 = base["k_cache"], tree["v_cache"]
+    com = dict(k_caches=[k1], v_caches=[v1], block_table=base["block_table"], seq_lens=base["seq_lens"], keep=keep,
+               counts=counts)
+    bad(ea.kv_compact, com, dict(v_caches=[k1]), dict(k_caches=[k1, k1], v_caches=[v1, v1]), dict(k_caches=[]),
+        dict(k_caches=[k1, v1]), dict(scores=[w, w]), dict(scores=[w.half()]), dict(keep=keep.long()),
+        dict(keep=keep[:1]), dict(counts=counts[:1]), dict(starts=counts.float()), dict(k_caches=[k1[:-1]]),
+        dict(k_caches=[k1.transpose(1, 2)]))
