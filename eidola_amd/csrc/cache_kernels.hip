@@ -96,7 +96,8 @@ __device__ __forceinline__ bool below_window(const ScoreParams &p, const int pre
 //
 // Sequences of one or two rows: bound by reading K.  A wave takes 64 keys of one KV head; the
 // workgroup's waves take neighbouring heads of the same keys, so that whole pages are read at
-// once.  grid = (chunks, sequences, head groups).
+// once.  grid = (chunks, sequences, head groups).  For head counts that the stream below does not
+// take; at 8 heads 64 sequences of one row behind 8192 bf16 keys are 117 us, 4.9 TB/s.
 // ---------------------------------------------------------------------------------------
 template <bool FP8>
 __global__ __launch_bounds__(512) void score_few_kernel(const ScoreParams p) {
@@ -346,7 +347,9 @@ __global__ __launch_bounds__(FP8 ? 256 : 512, 2) void score_stream_kernel(const 
 // tiles alone do not fill the device, and the tiles that see the causal edge have less to do.
 //
 // A stage is one 16-key page: its two matrix instructions are issued a stage ahead of its four
-// (multiply-add, exponential, add) per lane.
+// (multiply-add, exponential, add) per lane, which is what bounds the kernel: 2048 rows of one sequence
+// behind 4k keys, 8 KV heads, 0.4 G weights, 106 us with the join, 3.8 weights per ns (51 GFLOP of
+// products, 0.48 PFLOP/s); 8 x 37 rows behind 8k fp8 keys 34 us.
 // ---------------------------------------------------------------------------------------
 template <bool FP8>
 __global__ __launch_bounds__(kScoreWaves * 64, 3) void score_rows_kernel(const ScoreParams p) {
@@ -471,12 +474,15 @@ __global__ __launch_bounds__(256) void score_join_kernel(const ScoreParams p) {
 // ---------------------------------------------------------------------------------------
 // Rows to keep.  A workgroup per (sequence, KV head) finds the score of the last row that stays
 // by radix selection over order-preserving keys, eleven bits a pass, then writes the rows in
-// order.  A thread holds a run of RUN consecutive rows as keys in its registers: the scores are
-// read once, every pass works on registers, and one scan over the workgroup gives each thread the
-// places of its rows.  Sequences beyond 32 rows per thread are walked in blocks of that size and
-// read again by every pass.  Four copies of the histogram: lanes with equal digits, the
-// usual case in the first pass, queue less on one address.  A pass whose digit is kept whole ends
-// the search.
+// order.  A thread holds RUN rows as keys in its registers: the scores are read once, every pass
+// works on registers, and ballots give each row its place.  Sequences beyond 32 rows per thread are
+// walked in blocks of that size and read again by every pass.  A wave reads whole pages, four lanes
+// each; workgroups of neighbouring heads, which share cache lines of scores, run on one XCD (32
+// sequences of 32k rows: 24 us against 28).  Four copies of the histogram: lanes with equal digits,
+// the usual case in the first pass, queue less on one address (8 and 16 copies cost more to clear
+// than they save: 31 and 44 us against 28).  A pass whose digit is kept whole ends the search.
+// 32 sequences of up to 32k rows to 4096, 28 MB: 21 us, the second and third pass 4 of them; one of
+// 3000: 6.4 us, a chain of passes in one workgroup.
 // ---------------------------------------------------------------------------------------
 // larger = kept first, -0 = +0; NaN ranks lowest, as 1: 0 stands for rows that are no candidates, which
 // are therefore never reached (the candidates are at least as many as the rows wanted)
@@ -779,7 +785,8 @@ hipError_t launch_score(const ScoreParams &p, const bool fp8, const bool many, h
 }
 
 hipError_t launch_select(const SelectParams &p, hipStream_t st) {
-  // rows per thread: as few as hold the longest sequence
+  // rows per thread: as few as hold the longest sequence (8 of 3000: 6.8 us with 4, 10.0 with 16, 14.5
+  // with 32; 8 of 12000: 11.4 with 16, 16.4 with 32)
   const unsigned grid = (unsigned)(p.num_seqs * p.num_kv_heads);
   if (p.max_kv_len <= kSelThreads * 4) select_kernel<4><<<grid, kSelThreads, 0, st>>>(p);
   else if (p.max_kv_len <= kSelThreads * 16) select_kernel<16><<<grid, kSelThreads, 0, st>>>(p);
@@ -791,6 +798,8 @@ hipError_t launch_compact(const CompactParams &p, const int num_layers, hipStrea
   const int heads = p.keep_head != 0 ? 1 : p.num_kv_heads < 8 ? p.num_kv_heads : 8;
   const unsigned x = (unsigned)(p.num_seqs * (p.num_kv_heads / heads) * (p.has_scores ? 3 : 2));
   const dim3 grid(x, (unsigned)num_layers);
+  // A column's rows in one step of the larger workgroup or a few of the smaller: a commit of 36 layers
+  // 9.0 us with 256 threads, 25 with 1024; 8 sequences cut from 16k to 4k rows 55 and 47.
   if ((long long)p.max_rows * heads * kHeadDim * p.elt > 64 * 1024) compact_kernel<1024><<<grid, 1024, 0, st>>>(p, heads);
   else compact_kernel<256><<<grid, 256, 0, st>>>(p, heads);
   return hipGetLastError();

@@ -1228,7 +1228,8 @@ struct ScorePlan {
 
 // How many workgroups share the rows of a key tile.  A CU holds three workgroups; with several
 // times as many of them as places the tiles that see few rows even out.  A part keeps at least eight
-// row pairs, so that loading the keys pays.
+// row pairs, so that loading the keys pays.  Aiming at 4 / 8 / 16 workgroups per CU: 2048 rows behind 4k
+// keys 118 / 110 / 123 us (one part 502), 512 rows 41 / 45 / 47 (134), 8 x 37 behind 8k 50 / 51 / 66.
 ScorePlan make_score_plan(const eid_attn_desc *d) {
   ScorePlan pl;
   constexpr long long wg_keys = eid::kScoreWaves * eid::kScoreKeys;

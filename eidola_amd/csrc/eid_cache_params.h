@@ -8,7 +8,8 @@ namespace eid {
 constexpr int kTreeWordsMax = 4;              // mask words per drafted token
 constexpr int kTreeMax = 64 * kTreeWordsMax;  // drafted tokens per sequence
 constexpr int kTreeWaves = 4;
-constexpr int kTreeMinChunks = 2;             // 64-key chunks per workgroup of a range, at least
+// 64-key chunks per range, at least: 1 x 16 tokens behind 4k keys 13.9 us with 2, 15.7 with 1, 14.8 with 4
+constexpr int kTreeMinChunks = 2;
 
 // Where the pieces of a tile of drafted tokens are.
 struct TreeRecord {

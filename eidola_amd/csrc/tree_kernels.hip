@@ -124,6 +124,13 @@ __device__ __forceinline__ uint64_t chunk_bits(const uint64_t *mask, const int l
 // two ways: scores are masked, and values that are not finite are taken out of the operands
 // (0 x inf would be NaN in rows that do not see the key); if there were any, their terms are added
 // afterwards, row by row, where they are seen.
+//
+// What bounds it, 8 KV heads.  Up to 16 tokens the stream of K and V: 16 trees of up to 16 tokens behind
+// up to 8k keys, 199 MB, 54 us, 3.7 TB/s.  From about 24 tokens on the vector units: a 64-key chunk of a
+// 16-row tile takes 16 exponentials, 16 multiply-adds and 8 packings per lane beside its 18 matrix
+// instructions, whose time it hides: 4 x 64 behind 32k, 137 GFLOP, 176 us, 0.78 PFLOP/s; 8 x 32
+// behind 16k fp8 88 us.  Short calls are two launches long: 32 x 24 in a window of 128, 19 MB, 15 us
+// in one launch.
 // ---------------------------------------------------------------------------------------
 typedef __attribute__((address_space(1))) const void gptr_t;
 typedef __attribute__((address_space(3))) void lptr_t;
@@ -158,7 +165,9 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_kernel(const TreePara
   constexpr int ST = FP8 || QLDS ? 2 : 4;  // K/V stages
   constexpr bool DEEP8 = NT <= 3;          // fp8: two chunks under way
   // (separate arrays: the compiler can then tell the stage being filled from the one being read)
-  // one tile per tree: every chunk is read once, past the caches (non-temporal)
+  // Up to 16 tokens are one tile: every chunk is read once, past the caches (non-temporal): 16 x 16 behind
+  // 8k keys 72 us against 75.  Larger trees may be cut, and a chunk then serves several tiles: 4 x 200
+  // behind 4k 98 us from the caches, 109 past them (16 x 24, one tile, 90 and 89).
   constexpr int kAux = NT <= 2 ? 2 : 0;
   constexpr int kMore = ST == 4 ? kTileBytes : 16;
   __shared__ __align__(1024) uint8_t k_st0[kTileBytes], k_st1[kTileBytes], k_st2[kMore], k_st3[kMore];
@@ -698,7 +707,7 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_kernel(const TreePara
 
 // Joins the pieces of a tile that range ends cut: out = sum 2^(m - M) o / (sum 2^(m - M) l + 2^(sink - M)).
 // Eight lanes take a row, PG lane groups every PG-th of its pieces, four at a time; a workgroup holds
-// 32 / PG rows of one tile.
+// 32 / PG rows of one tile.  Bound by launch and memory latency: 4-7 us (16 trees of 16 tokens: 5 us).
 template <int PG>
 __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeParams p, const int tile_tok) {
   constexpr int kTokens = 4 / PG;  // of a workgroup (PG 1: four, PG 4: one)
@@ -780,7 +789,9 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeParams p, con
 
 }  // namespace
 
-// 16-row tiles per wave: a tree is cut into the fewest tiles of at most 32 tokens, of about equal size.
+// 16-row tiles per wave: a tree is cut into the fewest tiles of at most 32 tokens, of about equal size,
+// in steps of 8 tokens.  16 trees of 40 tokens behind 8k keys: two tiles of 24 145 us, of 32 164 us;
+// 8 tokens: a tile of 8 59 us, of 32 79 us.
 int tree_tiles(const int max_q_len) {
   const int tiles = (max_q_len + 31) / 32;
   return ((max_q_len + tiles - 1) / tiles + 7) / 8;
@@ -804,7 +815,8 @@ hipError_t launch_tree(const TreeParams &p, const bool fp8, hipStream_t st) {
 }
 
 hipError_t launch_tree_merge(const TreeParams &p, hipStream_t st) {
-  // many pieces of few tiles: their pieces side by side
+  // Many pieces of few tiles: their pieces side by side (1 x 16 behind 16k keys: 22 us against 28); else
+  // a workgroup takes more rows (32 x 16 behind 4k, two pieces a tile: 73 us against 78).
   const int tile = tree_tile_tokens(p.max_q_len);
   const unsigned tiles = (unsigned)(p.num_seqs * p.max_tiles), cells = tiles * (unsigned)p.num_kv_heads;
   if ((unsigned)p.ranges > 4 * tiles) tree_merge_kernel<4><<<cells * tile, 256, 0, st>>>(p, tile);
