@@ -128,8 +128,8 @@ __device__ __forceinline__ uint64_t chunk_bits(const uint64_t *mask, const int l
 // What bounds it, 8 KV heads.  Up to 16 tokens the stream of K and V: 16 trees of up to 16 tokens behind
 // up to 8k keys, 199 MB, 54 us, 3.7 TB/s.  From about 24 tokens on instructions: a 64-key chunk of a
 // 16-row tile takes 16 exponentials, 16 multiply-adds and 8 packings per lane and 18 matrix instructions,
-// which overlap only in part: 4 x 64 behind 32k, 137 GFLOP, 176 us, 0.78 PFLOP/s (75 us of the
-// former, 127 of the latter); 8 x 32 behind 16k fp8 88 us.  Short calls are two launches long: 32 x 24 in a window of 128, 19 MB, 15 us
+// which overlap only in part: 4 x 64 behind 32k, 137 GFLOP, 174 us, 0.79 PFLOP/s, vector units 59 % and
+// matrix units 36 % busy; 8 x 32 behind 16k fp8 88 us.  Short calls are two launches long: 32 x 24 in a window of 128, 19 MB, 15 us
 // in one launch.
 // ---------------------------------------------------------------------------------------
 typedef __attribute__((address_space(1))) const void gptr_t;
