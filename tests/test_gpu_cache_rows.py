@@ -398,3 +398,28 @@ def test_tensors_that_do_not_fit_are_refused(G):
         dict(k_caches=[k1, v1]), dict(scores=[w, w]), dict(scores=[w.half()]), dict(keep=keep.long()),
         dict(keep=keep[:1]), dict(counts=counts[:1]), dict(starts=counts.float()), dict(k_caches=[k1[:-1]]),
         dict(k_caches=[k1.transpose(1, 2)]))
+
+
+@pytest.mark.parametrize("kv_dtype", [KV_BF16, KV_FP8_E4M3])
+@pytest.mark.parametrize("heads", [4, 24])
+def test_other_head_counts(G, heads, kv_dtype):
+    for q_lens in ([1, 2, 1], [1, 40, 3]):
+        b, q, kc, vc, ks, vs, sinks = R.filled([130, 70, 33], q_lens, num_kv_heads=heads, kv_dtype=kv_dtype)
+        lse = lse_of(b, q, kc, vc, sinks, ks, vs)
+        w = pool(b, np.random.default_rng(8))
+        ref = R.kv_score(b, q, lse, kc, w, ks)
+        assert (np.abs(score(G, b, q, lse, kc, w, ks) - ref) <= REL * ref + 1e-7).all()
+    keep, counts = select(G, b, w, 30, 2, 5)
+    ref, ref_counts = R.kv_select(b, w, 30, 2, 5)
+    assert np.array_equal(keep, ref) and np.array_equal(counts, ref_counts)
+    kd, vd, wd = G.cache_dev(kc), G.cache_dev(vc), G.dev(w)
+    ea.kv_compact(b.geom, [kd], [vd], G.dev(b.block_table), G.dev(b.seq_lens), G.dev(keep), G.dev(counts), scores=[wd])
+    assert np.array_equal(G.cache_host(kd), R.kv_compact(b, kc, keep, counts, [0] * 3, True))
+    assert np.array_equal(G.cache_host(vd), R.kv_compact(b, vc, keep, counts, [0] * 3, True))
+    # the same rows in every head, behind the context
+    path = np.sort(np.random.default_rng(9).choice(np.arange(20, 33), (3, 6), replace=True), axis=1).astype(np.int32)
+    path = np.maximum(path, 20 + np.arange(6, dtype=np.int32))
+    starts, n = np.full(3, 20, np.int32), np.array([6, 0, 4], np.int32)
+    kd = G.cache_dev(kc)
+    ea.kv_compact(b.geom, [kd], [vd], G.dev(b.block_table), G.dev(b.seq_lens), G.dev(path), G.dev(n), starts=G.dev(starts))
+    assert np.array_equal(G.cache_host(kd), R.kv_compact(b, kc, path, n, starts, False))

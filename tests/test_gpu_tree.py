@@ -324,3 +324,11 @@ def test_captured_with_contexts_that_are_cut(G, lens, q_lens):
         assert (np.abs(R.f64(got) - ref) <= tol).all()
         run()
         assert np.array_equal(got, G.bits_host(out))
+
+
+@pytest.mark.parametrize("kv_dtype", [KV_BF16, KV_FP8_E4M3])
+@pytest.mark.parametrize("heads", [4, 24])
+def test_other_head_counts(G, heads, kv_dtype):
+    q_lens = [9, 30]
+    b, q, kc, vc, ks, vs, sinks = R.filled([700, 90], q_lens, num_kv_heads=heads, kv_dtype=kv_dtype)
+    check(G, b, q, kc, vc, trees(q_lens, 5), sinks, ks, vs)
