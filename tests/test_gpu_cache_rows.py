@@ -423,3 +423,30 @@ def test_other_head_counts(G, heads, kv_dtype):
     kd = G.cache_dev(kc)
     ea.kv_compact(b.geom, [kd], [vd], G.dev(b.block_table), G.dev(b.seq_lens), G.dev(path), G.dev(n), starts=G.dev(starts))
     assert np.array_equal(G.cache_host(kd), R.kv_compact(b, kc, path, n, starts, False))
+
+
+def test_pages_past_two_to_the_32_bytes(G):
+    # scores, selections and moves in pages whose byte offsets in the cache do not fit 32 bits
+    nb = (1 << 32) // 16384 + 40
+    b, q, kc, vc, ks, vs, sinks = R.filled([100, 60], [1, 2])
+    far = nb - kc.shape[0]
+    k, v = (torch.zeros((nb, 16, 8, 64), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    w = torch.zeros((nb, 8, 16), device="cuda")
+    bt, sl, cu = G.dev((b.block_table + far).astype(np.int32)), G.dev(b.seq_lens), G.dev(b.cu_seqlens_q)
+    for t, c in ((k, kc), (v, vc)):
+        t[far:] = G.cache_dev(c)
+    start = pool(b, np.random.default_rng(2))
+    lse = lse_of(b, q, kc, vc, sinks, ks, vs)
+    ref = R.kv_score(b, q, lse, kc, start)
+    for max_q in (2, 3):                       # the kernels for few rows and for any number
+        w[far:] = G.dev(start)
+        ea.kv_score(b.geom, G.bf16_dev(q), G.dev(lse), k, bt, sl, cu, w, max_q_len=max_q, max_kv_len=100)
+        assert (np.abs(w[far:].cpu().numpy() - ref) <= REL * ref + 1e-7).all()
+    got = w[far:].cpu().numpy()
+    keep, counts = ea.kv_select(b.geom, w, bt, sl, budget=40, keep_first=2, keep_last=3, max_kv_len=100)
+    rk, rc = R.kv_select(b, got, 40, 2, 3)
+    assert np.array_equal(keep.cpu().numpy(), rk) and np.array_equal(counts.cpu().numpy(), rc)
+    ea.kv_compact(b.geom, [k], [v], bt, sl, keep, counts, scores=[w])
+    assert np.array_equal(G.cache_host(k[far:].contiguous()), R.kv_compact(b, kc, rk, rc, [0, 0], True))
+    assert np.array_equal(G.cache_host(v[far:].contiguous()), R.kv_compact(b, vc, rk, rc, [0, 0], True))
+    assert not k[:far].any() and not w[:far].any()
