@@ -324,7 +324,8 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_kernel(const TreePara
       }
       lds_lo[tid] = p.window > 0 ? prefix + depth - p.window + 1 : 0;
     }
-    if (p.window > 0 && p.window < v.qlen) {  // an ancestor may lie outside the window
+    // A drafted token may lie outside a row's window: depths go from -1 (an empty mask) to qlen - 1.
+    if (p.window > 0 && p.window <= v.qlen) {
       int depth = -1;  // of token tid of the tree
       for (int w = 0; w < p.mask_words; ++w) depth += __popcll(mask_word(tid, w));
       lds_depth[tid] = depth;
