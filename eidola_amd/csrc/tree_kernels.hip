@@ -98,7 +98,8 @@ __device__ __forceinline__ uint64_t chunk_bits(const uint64_t *mask, const int l
   } else {
     w = ((1ull << -d) - 1) | mask[0] << -d;
   }
-  const int cut = min(min(lo, prefix) - tc, 64);  // context keys below the window
+  // context keys below the window (lo is far below 0 in a window near 2^31)
+  const int cut = min(min(max(lo, 0), prefix) - tc, 64);
   if (cut >= 64) w = 0;
   else if (cut > 0) w &= ~((1ull << cut) - 1);
   return w;

@@ -85,3 +85,12 @@ def test_a_window_as_long_as_the_tree(G, n, kv_dtype):
             ints[first] = ints[first + n // 2] = 0
             ints[first + n - 1] = (1 << n) - 1
         check(G, b, q, kc, vc, R.masks_from_ints(ints, (n + 63) // 64), sinks, ks, vs)
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 150])
+@pytest.mark.parametrize("n", [100, 200])
+def test_windows_that_nothing_outgrows(G, n, window):
+    # the largest windows that a descriptor holds, drafted tokens more than a chunk behind a short context
+    b, q, kc, vc, ks, vs, sinks = R.filled([n + 10, n], [n, n], window=window, num_kv_heads=1)
+    rng = np.random.default_rng(n)
+    check(G, b, q, kc, vc, R.tree_masks([R.random_parents(n, rng), list(range(-1, n - 1))], (n + 63) // 64), sinks)
