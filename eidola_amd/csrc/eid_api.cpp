@@ -1185,7 +1185,7 @@ TreePlan make_tree_plan(const eid_attn_desc *d) {
   const size_t rows = (size_t)pl.ranges * d->num_kv_heads * 2 * tile * eid::kGroup;
   pl.rec_bytes = ((size_t)d->num_seqs * tiles * sizeof(eid::TreeRecord) + 255) / 256 * 256;
   pl.o_bytes = rows * eid::kHeadDim * sizeof(_Float16);
-  pl.ml_bytes = rows * 2 * sizeof(float);
+  pl.ml_bytes = rows * sizeof(eid::TreeStats);
   return pl;
 }
 
@@ -1298,7 +1298,7 @@ int32_t eid_attn_tree(const eid_attn_desc *desc, const eid_attn_args *args, cons
   uint8_t *ws = static_cast<uint8_t *>(args->workspace);
   p.ws_rec = reinterpret_cast<eid::TreeRecord *>(ws);
   p.ws_o = reinterpret_cast<_Float16 *>(ws + pl.rec_bytes);
-  p.ws_ml = reinterpret_cast<float *>(ws + pl.rec_bytes + pl.o_bytes);
+  p.ws_ml = reinterpret_cast<eid::TreeStats *>(ws + pl.rec_bytes + pl.o_bytes);
   p.num_seqs = desc->num_seqs;
   p.num_q_heads = desc->num_q_heads;
   p.num_kv_heads = desc->num_kv_heads;

@@ -16,6 +16,13 @@ struct TreeRecord {
   int32_t range, pieces;  // first range that holds some of it, and how many do
 };
 
+// Statistics of one row of a piece.
+struct alignas(16) TreeStats {
+  float m, l;    // reference (log2 units) and sum of the row's weights
+  int32_t e;     // the row's outputs are kept as 2^-e of themselves
+  int32_t unused;
+};
+
 struct TreeParams {
   const uint16_t *q;
   uint16_t *out;
@@ -26,8 +33,8 @@ struct TreeParams {
   const float *k_scale, *v_scale; // fp8 only
   const uint64_t *mask;           // [num_q_tokens][mask_words]
   TreeRecord *ws_rec;  // [num_seqs][max_tiles]
-  _Float16 *ws_o;  // [ranges][Hkv][2][tile rows][64]  sum of 2^(s-m) v of a piece, not normalised
-  float *ws_ml;  // [ranges][Hkv][2][tile rows][2]   m (log2 units), l
+  _Float16 *ws_o;  // [ranges][Hkv][2][tile rows][64]  2^-e sum of 2^(s-m) v of a piece, not normalised
+  TreeStats *ws_ml;    // [ranges][Hkv][2][tile rows]      m (log2 units), l, e
   int32_t num_seqs, num_q_heads, num_kv_heads, max_blocks_per_seq, last_block;
   int32_t num_q_tokens, mask_words, window, max_q_len, max_kv_len;
   int32_t max_tiles;  // tiles of the longest tree

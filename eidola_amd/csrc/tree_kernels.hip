@@ -646,7 +646,7 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_kernel(const TreePara
     const bool whole = n == v.chunks;
     const int part = c0 == 0 ? 1 : 0;  // a range holds at most one piece of each kind that is not whole
     _Float16 *ws_o = p.ws_o + ((size_t)(range * Hkv + kvh) * 2 + part) * (kRows * kHeadDim);
-    float *ws_ml = p.ws_ml + ((size_t)(range * Hkv + kvh) * 2 + part) * (kRows * 2);
+    TreeStats *ws_ml = p.ws_ml + ((size_t)(range * Hkv + kvh) * 2 + part) * kRows;
     if (c0 == 0 && kvh == 0 && tid == 0 && !p.whole) {  // the tile begins here: where its pieces are
       const int last = u + v.chunks - 1;    // its last unit
       p.ws_rec[s * p.max_tiles + tile] = {range, last / place.per - range + 1};
@@ -676,9 +676,10 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_kernel(const TreePara
           if (p.lse && g == 0) p.lse[orow] = any ? (M + __log2f(den)) * kLn2 : -INFINITY;
         } else {
           // The outputs go out as fp16 beside a power of two of the row's own, which brings its largest
-          // (finite) one to [1/2, 1): a rounding of 2^-12 there, one of 2^-25 of that one for those
-          // that are far smaller, against the 2^-9 of the bf16 that the answer is rounded to; and half
-          // the bytes of fp32.  The power moves into m and l: (m + e, l 2^-e, o 2^-e) is the same piece.
+          // (finite) one to [2^14, 2^15): roundings of 2^-11 of an output down to 2^-28 of the largest, and of
+          // 2^-39 of the largest below, against the 2^-8 of the bf16 that the answer is rounded to; and
+          // half the bytes of fp32.  The power stands apart from m and l, which do not depend on V: moved
+          // into them it would overflow l where all outputs of a piece are tiny.
           const int row = tl * kGroup + (i16 & 7);
           float top = 0.f;
 #pragma unroll
@@ -688,7 +689,7 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_kernel(const TreePara
               const float x = fabsf(acc[t][mt][r]);
               top = fmaxf(top, x < INFINITY ? x : 0.f);
             }
-          const int e = top_exponent(rowgroup_max(top));
+          const int e = top_exponent(rowgroup_max(top)) - 15;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {  // (a lane's 16 dims next to each other: 16 mt + 4 g + r at 16 g + 4 mt + r)
             f16x8 x;
@@ -696,10 +697,7 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_kernel(const TreePara
             for (int i = 0; i < 8; ++i) x[i] = (_Float16)ldexpf(acc[t][2 * h + i / 4][i & 3], -e);
             *(f16x8 *)(ws_o + (size_t)row * kHeadDim + 16 * g + 8 * h) = x;
           }
-          if (g == 0) {
-            ws_ml[2 * row] = m[t] + (float)e;
-            ws_ml[2 * row + 1] = ldexpf(lt, -e);
-          }
+          if (g == 0) ws_ml[row] = TreeStats{m[t], lt, e, 0};
         }
       }
     }
@@ -707,7 +705,7 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void tree_kernel(const TreePara
   }
 }
 
-// Joins the pieces of a tile that range ends cut: out = sum 2^(m - M) o / (sum 2^(m - M) l + 2^(sink - M)).
+// Joins the pieces of a tile that range ends cut: out = sum 2^(m + e - M) o / (sum 2^(m - M) l + 2^(sink - M)).
 // Eight lanes take a row, PG lane groups every PG-th of its pieces, four at a time; a workgroup holds
 // 32 / PG rows of one tile.  Bound by launch and memory latency: 4-7 us (16 trees of 16 tokens: 5 us).
 template <int PG>
@@ -733,18 +731,18 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeParams p, con
   for (int k = 0; k < 8; ++k) o[k] = 0.f;
   if (tl < ntok) {
     for (int i = pg; i < rec.pieces; i += 4 * PG) {
-      float2 ml[4];
+      TreeStats ml[4];
       f16x8 x[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int j = min(i + e * PG, rec.pieces - 1);  // (past the end the last one again, without weight)
         const size_t c = cell0 + (size_t)j * Hkv * 2 * rows + (j == 0 ? rows : 0);
-        ml[e] = *(const float2 *)(p.ws_ml + 2 * c);
+        ml[e] = p.ws_ml[c];
         x[e] = *(const f16x8 *)(p.ws_o + c * kHeadDim + 8 * eighth);
       }
       float M1 = M;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) M1 = i + e * PG < rec.pieces ? max2(M1, ml[e].x) : M1;
+      for (int e = 0; e < 4; ++e) M1 = i + e * PG < rec.pieces ? max2(M1, ml[e].m) : M1;
       const float a = fast_exp2(M - M1);
       den *= a;
 #pragma unroll
@@ -752,10 +750,10 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeParams p, con
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (i + e * PG < rec.pieces) {
-          const float w = fast_exp2(ml[e].x - M1);
-          den += ml[e].y * w;
+          const float w = fast_exp2(ml[e].m - M1), wo = ldexpf(w, ml[e].e);
+          den += ml[e].l * w;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) o[k] += (float)x[e][k] * w;
+          for (int k = 0; k < 8; ++k) o[k] += (float)x[e][k] * wo;
         }
       M = M1;
     }

@@ -94,3 +94,33 @@ def test_windows_that_nothing_outgrows(G, n, window):
     b, q, kc, vc, ks, vs, sinks = R.filled([n + 10, n], [n, n], window=window, num_kv_heads=1)
     rng = np.random.default_rng(n)
     check(G, b, q, kc, vc, R.tree_masks([R.random_parents(n, rng), list(range(-1, n - 1))], (n + 63) // 64), sinks)
+
+
+@pytest.mark.parametrize("n", [4, 12, 20, 30])
+def test_small_values_behind_a_cut_context_leave_its_sums_alone(G, n):
+    # Keys that all score 0 and values of 0, but for one key whose weight is 2^-124 of the others' and whose
+    # values are 1; ordinary values further in front.  The statistics do not depend on the values.
+    L = 3000 + n
+    b = make_batch([L], [n], num_kv_heads=1)
+    q, k, v, _ = logical_tensors(b)
+    q[:], k[:] = 0x4080, 0                           # 4 in every element
+    k[2000] = synth.f32_to_bf16_bits(np.full(64, -2.6875, np.float32))   # -688 log2(e) / 8 = -124.07
+    v[1000:2000], v[2000], v[2001:] = 0, 0x3F80, 0
+    kc, vc = cpu_caches(b, k, v)
+    mask = R.tree_masks([list(range(-1, n - 1))], 1)
+    check(G, b, q, kc, vc, mask, None)
+    # values at the lower end of bf16's normal range throughout, in that of fp32 as well
+    q, k, v, sinks = logical_tensors(b)
+    v = synth.f32_to_bf16_bits((synth.bf16_bits_to_f32(v) * np.float32(2.0 ** -124)).astype(np.float32))
+    kc, vc = cpu_caches(b, k, v)
+    check(G, b, q, kc, vc, mask, None)
+    check(G, b, q, kc, vc, mask, sinks)
+    # large ones as well
+    v = synth.f32_to_bf16_bits((synth.bf16_bits_to_f32(v) * np.float32(2.0 ** 124) * np.float32(2.0 ** 44)).astype(np.float32))
+    kc, vc = cpu_caches(b, k, v)
+    check(G, b, q, kc, vc, mask, sinks)
+    # and elements of very different size next to each other
+    q, k, v, sinks = logical_tensors(b)
+    v = synth.f32_to_bf16_bits(synth.bf16_bits_to_f32(v) * np.exp2(np.arange(64) % 13 * 2.0 + 10).astype(np.float32))
+    kc, vc = cpu_caches(b, k, v)
+    check(G, b, q, kc, vc, mask, sinks)
