@@ -44,7 +44,7 @@ __device__ __forceinline__ void load_k(const uint8_t *base, const uint32_t row_b
 }
 
 // 16 rows of q (two tokens x 8 heads) from token `tok` of the sequence on, and what the rows'
-// exponents take off: lse in log2 units; +inf where there is no row (its weights are then 0).
+// exponents take off: lse in log2 units; -inf where there is no row, or one that saw nothing.
 template <bool FP8>
 __device__ __forceinline__ void load_rows(const ScoreParams &p, const ScoreSeq &v, const int kvh, const int tok,
                                           Frag8 (&qf)[2], f32x4 &off) {
@@ -56,23 +56,27 @@ __device__ __forceinline__ void load_rows(const ScoreParams &p, const ScoreSeq &
     qf[0].u = *(const u32x4 *)src;
     qf[1].u = *(const u32x4 *)(src + (FP8 ? 8 : 32));
   }
-  off = f32x4{INFINITY, INFINITY, INFINITY, INFINITY};
+  off = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
   if (tl < v.qlen) {
     const f32x4 e = *(const f32x4 *)(p.lse + (size_t)(v.row0 + tl) * p.num_q_heads + kvh * kGroup + 4 * (g & 1));
 #pragma unroll
-    for (int r = 0; r < 4; ++r) off[r] = e[r] == -INFINITY ? INFINITY : e[r] * kLog2e;  // (a row that saw nothing)
+    for (int r = 0; r < 4; ++r) off[r] = e[r] * kLog2e;
   }
 }
 
 // Weights of 16 keys from 16 rows, summed over the lane's four rows.  D of Q K^T: lane (key i16,
-// rows 4 g + r); rows 8 and up belong to the second token.
+// rows 4 g + r); rows 8 and up belong to the second token.  Rows without an offset add nothing, to keys
+// that are not finite either (whose scores are NaN there: 0 x inf).
 __device__ __forceinline__ float weights(const Frag8 (&qf)[2], const Frag8 (&kf)[2], const f32x4 off, const float c2,
                                          const bool see) {
   f32x4 S = mfma16x32(qf[0], kf[0], f32x4{0.f, 0.f, 0.f, 0.f});
   S = mfma16x32(qf[1], kf[1], S);
   float w = 0.f;
 #pragma unroll
-  for (int r = 0; r < 4; ++r) w += fast_exp2(__builtin_fmaf(S[r], c2, -off[r]));
+  for (int r = 0; r < 4; ++r) {
+    const float x = fast_exp2(__builtin_fmaf(S[r], c2, -off[r]));
+    w += off[r] == -INFINITY ? 0.f : x;
+  }
   return see ? w : 0.f;
 }
 
@@ -394,14 +398,20 @@ __global__ __launch_bounds__(kScoreWaves * 64, 3) void score_rows_kernel(const S
   float sum[kPages];
 #pragma unroll
   for (int b = 0; b < kPages; ++b) sum[b] = 0.f;
-  auto pair = [&](auto edge_c, const int i) {
-    constexpr bool EDGE = decltype(edge_c)::value;
-    // what the exponents take off, in log2 units; a row that saw nothing (-inf) has no weights
+  // EDGE: some row of the pair does not see all keys, or is none.  DROP: a row saw nothing (its lse is -inf)
+  // and adds nothing, to keys that are not finite either.
+  auto pair = [&](auto edge_c, auto drop_c, const int i) {
+    constexpr bool EDGE = decltype(edge_c)::value, DROP = decltype(drop_c)::value;
+    // what the exponents take off, in log2 units
     f32x4 off;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) off[r] = e[r] == -INFINITY ? -INFINITY : -kLog2e * e[r];
+    for (int r = 0; r < 4; ++r) off[r] = -kLog2e * e[r];
     const int pos = prefix + i + (g >> 1);
-    if (EDGE && i + (g >> 1) >= v.qlen) off = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    const bool real = !EDGE || i + (g >> 1) < v.qlen;
+    auto weight = [&](const float S, const int r) {
+      const float x = fast_exp2(__builtin_fmaf(S, c2, off[r]));
+      return !DROP || e[r] != -INFINITY ? x : 0.f;
+    };
     f32x4 S[3];
     auto first_half = [&](const int b) { S[b % 3] = mfma16x32(qf[0], kf[b][0], f32x4{0.f, 0.f, 0.f, 0.f}); };
     auto second_half = [&](const int b) { S[b % 3] = mfma16x32(qf[1], kf[b][1], S[b % 3]); };
@@ -414,15 +424,15 @@ __global__ __launch_bounds__(kScoreWaves * 64, 3) void score_rows_kernel(const S
       __builtin_amdgcn_sched_barrier(0);
       if (b + 1 < kPages) second_half(b + 1);
 #pragma unroll
-      for (int r = 0; r < 2; ++r) w[r] = fast_exp2(__builtin_fmaf(S[b % 3][r], c2, off[r]));
+      for (int r = 0; r < 2; ++r) w[r] = weight(S[b % 3][r], r);
       __builtin_amdgcn_sched_barrier(0);
       if (b + 2 < kPages) first_half(b + 2);
 #pragma unroll
-      for (int r = 2; r < 4; ++r) w[r] = fast_exp2(__builtin_fmaf(S[b % 3][r], c2, off[r]));
+      for (int r = 2; r < 4; ++r) w[r] = weight(S[b % 3][r], r);
       float add = (w[0] + w[1]) + (w[2] + w[3]);
       if constexpr (EDGE) {
         const int j = tc + b * kBlock + i16;
-        add = j <= pos && (p.window <= 0 || pos - j < p.window) ? add : 0.f;
+        add = real && j <= pos && (p.window <= 0 || pos - j < p.window) ? add : 0.f;
       }
       sum[b] += add;
     }
@@ -431,8 +441,9 @@ __global__ __launch_bounds__(kScoreWaves * 64, 3) void score_rows_kernel(const S
   for (int i = first; i < i1; i += stride) {
     fetch(i + stride, qn, en);
     const bool edge = prefix + i < key_end - 1 || (p.window > 0 && prefix + i + 1 - tc >= p.window) || i + 1 >= v.qlen;
-    if (edge) pair(std::true_type{}, i);
-    else pair(std::false_type{}, i);
+    if (__any(fminf(fminf(e[0], e[1]), fminf(e[2], e[3])) == -INFINITY)) pair(std::true_type{}, std::true_type{}, i);
+    else if (edge) pair(std::true_type{}, std::false_type{}, i);
+    else pair(std::false_type{}, std::false_type{}, i);
     qf[0] = qn[0];
     qf[1] = qn[1];
     e = en;

@@ -1,0 +1,34 @@
+"""eid_kv_score where rows or keys are not ordinary numbers, and where many parts are joined."""
+import numpy as np
+import pytest
+import torch
+
+import eidola_amd as ea
+from eidola_amd import KV_BF16, KV_FP8_E4M3, synth
+
+import cache_ref as R
+from test_gpu_cache_rows import G, REL, lse_of, pool, score  # noqa: F401 (G: fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("window", [0, 40])
+@pytest.mark.parametrize("heads", [2, 8])
+@pytest.mark.parametrize("q_lens", [[1, 1, 2], [1, 5, 2], [1, 40, 3]])
+def test_rows_that_do_not_exist_or_saw_nothing_add_nothing_beside_infinite_keys(G, q_lens, heads, window):
+    # A key of -inf in one element where every row is positive: its scores are -inf, its weights 0.  Rows whose
+    # lse says that they saw nothing add nothing even to a key that is NaN.
+    b, q, kc, vc, ks, vs, sinks = R.filled([200, 90, 33], q_lens, num_kv_heads=heads, window=window)
+    q[:, :, 5] = 0x3F80
+    kc.reshape(-1, heads, 64)[b.all_slots(0)[190], :, 5] = 0xFF80
+    kc.reshape(-1, heads, 64)[b.all_slots(1)[60], :, 5] = 0xFF80
+    kc.reshape(-1, heads, 64)[b.all_slots(2)[20], :, 5] = 0x7FC0
+    lse = lse_of(b, q, kc, vc, sinks, ks, vs)
+    lse[b.cu_seqlens_q[2]:] = -np.inf
+    if q_lens[1] > 3:
+        lse[b.cu_seqlens_q[1] + 2, ::3] = -np.inf
+    w = pool(b, np.random.default_rng(1))
+    ref = R.kv_score(b, q, lse, kc, w, ks)
+    assert np.isfinite(ref).all()
+    got = score(G, b, q, lse, kc, w, ks)
+    assert (np.abs(got - ref) <= REL * ref + 1e-7).all()
