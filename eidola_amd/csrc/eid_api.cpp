@@ -1189,8 +1189,13 @@ TreePlan make_tree_plan(const eid_attn_desc *d) {
   return pl;
 }
 
+// Longest sequence of the calls below: their kernels look up to 64 Ki rows past its end before they
+// compare, in 32 bits.
+constexpr int32_t kMaxRows = 0x7fff0000;
+
 int32_t check_tree_desc(const eid_attn_desc *d) {
   if (int32_t rc = check_attn_desc(d)) return rc;
+  if (d->max_kv_len > kMaxRows) return fail(EID_ERR_UNSUPPORTED, "max_kv_len %d too large", d->max_kv_len);
   if (d->max_q_len > eid::kTreeMax)
     return fail(EID_ERR_UNSUPPORTED, "max_q_len %d: a tree has at most %d tokens", d->max_q_len, eid::kTreeMax);
   // the kernel counts the launch's 64-key chunks in 32 bits
@@ -1206,14 +1211,14 @@ int32_t check_rows_desc(const eid_attn_desc *d) {
   if (d->num_seqs <= 0) return fail(EID_ERR_INVALID_ARG, "num_seqs must be positive");
   if (d->num_seqs > 65535) return fail(EID_ERR_UNSUPPORTED, "num_seqs > 65535");
   if (d->max_blocks_per_seq <= 0) return fail(EID_ERR_INVALID_ARG, "max_blocks_per_seq must be positive");
-  if (d->max_blocks_per_seq > 0x7fffffff / eid::kBlock)
+  if (d->max_blocks_per_seq > kMaxRows / eid::kBlock)
     return fail(EID_ERR_UNSUPPORTED, "max_blocks_per_seq %d too large", d->max_blocks_per_seq);
   return EID_OK;
 }
 
 int32_t check_score_desc(const eid_attn_desc *d) {
   if (int32_t rc = check_attn_desc(d)) return rc;
-  if (d->max_kv_len > 0x7fff0000 || ((long long)d->max_kv_len / eid::kScoreKeys + 1) * d->num_kv_heads > 0x3fffffffLL ||
+  if (d->max_kv_len > kMaxRows || ((long long)d->max_kv_len / eid::kScoreKeys + 1) * d->num_kv_heads > 0x3fffffffLL ||
       (d->max_kv_len / eid::kChunk + 2LL) * d->num_seqs > 0x3fffffffLL)
     return fail(EID_ERR_UNSUPPORTED, "max_kv_len %d with %d KV heads is too large", d->max_kv_len, d->num_kv_heads);
   return EID_OK;

@@ -314,7 +314,8 @@ int32_t eid_qkv_rope_kv_write(const eid_attn_desc *desc, const void *hidden, con
  * ancestors and itself; nothing is assumed of the bits, a row may see any set, or none):
  *   tree_mask   [num_q_tokens, mask_words] int64, bit j % 64 of word j / 64 of row i = "row i sees
  *               token j of its own sequence"; bits at or beyond the sequence's q_len are ignored
- * max_q_len <= 256, (max_q_len + 63) / 64 <= mask_words <= 4.
+ * max_q_len <= 256, (max_q_len + 63) / 64 <= mask_words <= 4.  A sequence holds at most 2^31 - 65536 rows
+ * here and in the calls below (max_kv_len, or 16 * max_blocks_per_seq where that is what is read).
  * desc->window: the position of a token is prefix + (bits set in its mask) - 1 (its depth), that
  * of a context row its index; row i sees what lies less than `window` positions behind its own.
  * Token ids, positions for the rotary embedding (prefix + depth) and slots are the caller's, as
