@@ -700,7 +700,8 @@ def kv_compact(geom, k_caches, v_caches, block_table, seq_lens, keep, counts, *,
     caches of all layers (lists of [num_blocks, 16, Hkv, D] tensors) and in their `scores`
     (list, optional).  keep is int32 and ascending, keep[..., i] >= starts[s] + i: [S, N] (the same
     rows in every layer and head), [S, Hkv, N] (in every layer) or [layers, S, Hkv, N]; seq_lens is
-    the length before the move.  The sequence's length afterwards is starts[s] + counts[s]."""
+    the length before the move.  The sequence's length afterwards is starts[s] + counts[s]; Scheduler.truncate,
+    called first, refuses sequences that share the pages."""
     n = len(k_caches)
     if n == 0 or len(v_caches) != n or (scores is not None and len(scores) != n):
         raise ValueError("k_caches, v_caches (and scores) must be lists with one tensor per layer")

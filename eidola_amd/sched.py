@@ -60,7 +60,8 @@ class Scheduler:
     def truncate(self, seq_id, new_len, unchanged=None):
         """Cuts a sequence back to its first `new_len` rows and gives the blocks behind them back.
         `unchanged` (default: new_len) leading rows hold what build_batch's tokens put there; the
-        rest was rewritten in place (kv_compact)."""
+        rest is rewritten in place by a kv_compact that follows.  Before the move, not behind it: a
+        sequence whose blocks others share is refused here, and kv_compact would rewrite them."""
         check(self._lib.eid_sched_truncate(self._h, seq_id, new_len, new_len if unchanged is None else unchanged))
 
     def seq_len(self, seq_id):

@@ -523,6 +523,7 @@ impl Scheduler {
     }
 
     /// Cuts a sequence back to its first `new_len` rows, `unchanged` of which hold what they held.
+    /// Before the rows behind those are moved: sequences that share their pages are refused here.
     pub fn truncate(&mut self, seq_id: i64, new_len: i32, unchanged: i32) -> Result<(), AttnError> {
         // SAFETY: live handle.
         check(unsafe { sys::eid_sched_truncate(self.handle, seq_id, new_len, unchanged) })

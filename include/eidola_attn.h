@@ -396,8 +396,9 @@ int32_t eid_kv_select(const eid_attn_desc *desc, const float *scores, const int3
  * moves nothing.  Entries out of order leave unspecified rows, within the sequence's own pages.
  * The pages written must belong to one sequence of the call alone (no prefix shared with others).
  * Of desc only the geometry, num_seqs, max_blocks_per_seq and num_blocks are read.  One launch per
- * 64 layers.  The sequence's new length, starts[s] + counts[s], is the caller's to keep
- * (eid_sched_truncate).  Reference counterpart: none.
+ * 64 layers.  The sequence's new length, starts[s] + counts[s], is the caller's to keep:
+ * eid_sched_truncate, called before this, refuses sequences whose pages others share.  Reference
+ * counterpart: none.
  */
 int32_t eid_kv_compact(const eid_attn_desc *desc, int32_t num_layers, const int64_t *k_caches,
                        const int64_t *v_caches, const int64_t *scores,

@@ -102,9 +102,12 @@ int32_t eid_sched_build_batch(eid_sched *s, const int64_t *seq_ids, const int32_
 
 /*
  * Cuts a sequence back to its first new_len rows: rejected drafted tokens, or a cache that
- * eid_kv_compact has cut to a budget.  Blocks behind the new end are released.  `unchanged`
+ * eid_kv_compact cuts to a budget.  To be called before the rows are moved: a refusal then leaves
+ * everything as it was, and no block is matched by another sequence while its rows change.  Blocks behind
+ * the new end are released; the move may still read them (from the block table of the step before) as long as
+ * whatever is written into them next follows it on its stream.  `unchanged`
  * (<= new_len) is the number of leading rows that hold what build_batch's tokens put there; rows
- * from there to new_len were rewritten in place.  Blocks that hold such rows, and a last block
+ * from there to new_len are rewritten in place.  Blocks that hold such rows, and a last block
  * that is now partly filled (it will be appended to), leave the prefix index, and must not be
  * shared with another sequence (EID_ERR_INVALID_ARG, nothing changes).  With unchanged < new_len
  * the sequence's later blocks are no longer indexed: they would not match their tokens.
