@@ -616,8 +616,9 @@ def kv_score(geom, q, lse, k_cache, block_table, seq_lens, cu_seqlens_q, scores,
              k_scale=None, sum_kv_len=0, workspace=None):
     """Adds the attention weight that every cached key receives from this step's rows to `scores`
     ([num_blocks, num_kv_heads, 16] fp32, paged like the caches; the step's own keys start from 0).
-    `lse` is what the step's attention call returned.  Returns `scores`.  `workspace`: a uint8
-    tensor of kv_score_workspace_bytes, for callers that keep one (one call at a time)."""
+    `lse` is what the step's attention call returned (rows in a line: there is no form for a tree's).
+    Returns `scores`.  `workspace`: a uint8 tensor of kv_score_workspace_bytes, for callers that keep one
+    (one call at a time)."""
     dev = _device_of(q, "q")
     kv, cache_shape = _cache_shape(k_cache, geom, "k_cache")
     if seq_lens is None or block_table is None or block_table.dim() != 2:

@@ -345,7 +345,9 @@ size_t eid_attn_tree_workspace_bytes(const eid_attn_desc *desc);
  *       exp(softmax_scale * q_i . k_j - lse_i)
  * New keys are the last q_len of the sequence: a page needs no clearing when it changes owner, as
  * long as this is called for every step that appends.  Rows see what eid_attn_decode /
- * eid_attn_varlen lets them see (causal, desc->window).
+ * eid_attn_varlen lets them see (causal, desc->window).  There is no form for the rows of a tree
+ * (eid_attn_tree): rows that a tree leaves behind hold what their pages held, so a sequence whose cache
+ * is cut by scores is not verified by trees.
  *   q        [num_q_tokens, num_q_heads, 64] bf16, the step's queries (after rotary embedding)
  *   lse      [num_q_tokens, num_q_heads] fp32, as the step's attention call returned it (-inf:
  *            the row saw nothing and adds nothing)
