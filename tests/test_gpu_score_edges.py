@@ -32,3 +32,20 @@ def test_rows_that_do_not_exist_or_saw_nothing_add_nothing_beside_infinite_keys(
     assert np.isfinite(ref).all()
     got = score(G, b, q, lse, kc, w, ks)
     assert (np.abs(got - ref) <= REL * ref + 1e-7).all()
+
+
+@pytest.mark.parametrize("kv_dtype", [KV_BF16, KV_FP8_E4M3])
+@pytest.mark.parametrize("window", [0, 1, 100])
+def test_many_parts_are_joined(G, window, kv_dtype):
+    # 18 parts.  A sum has up to 8 x 300 terms: 2400 * 2^-24 = 1.43e-4 of it, beside the exponents' 1.2e-5 and the
+    # scores' 2.3e-5: 1.8e-4 in all.
+    b, q, kc, vc, ks, vs, sinks = R.filled([700], [300], num_kv_heads=2, window=window, kv_dtype=kv_dtype)
+    desc = ea.make_desc(b.geom, num_seqs=1, num_q_tokens=300, max_q_len=300, max_kv_len=700,
+                        max_blocks_per_seq=b.block_table.shape[1], num_blocks=b.num_blocks)
+    assert ea.kv_score_workspace_bytes(desc) >= 16 * 2 * 700 * 4
+    lse = lse_of(b, q, kc, vc, sinks, ks, vs)
+    w = pool(b, np.random.default_rng(3))
+    ref = R.kv_score(b, q, lse, kc, w, ks)
+    got = score(G, b, q, lse, kc, w, ks)
+    assert (np.abs(got - ref) <= 1.8e-4 * ref + 1e-7).all()
+    assert np.array_equal(got, score(G, b, q, lse, kc, w, ks))

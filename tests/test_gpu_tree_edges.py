@@ -124,3 +124,98 @@ def test_small_values_behind_a_cut_context_leave_its_sums_alone(G, n):
     v = synth.f32_to_bf16_bits(synth.bf16_bits_to_f32(v) * np.exp2(np.arange(64) % 13 * 2.0 + 10).astype(np.float32))
     kc, vc = cpu_caches(b, k, v)
     check(G, b, q, kc, vc, mask, sinks)
+
+
+def rises_inside_ranges(b, q, kc, ks, tile):
+    """Largest rise, in log2 units, of a row's scores inside one range above those of its first chunk."""
+    heads, best = b.geom.num_kv_heads, 0.0
+    cus = torch.cuda.get_device_properties(0).multi_processor_count
+    chunks = [(int(n) + 63) // 64 for n in b.seq_lens]
+    tiles = [(int(n) + tile - 1) // tile for n in b.q_lens]
+    total = sum(c * t for c, t in zip(chunks, tiles))
+    per = max(-(-total // (2 * cus // heads)), 2)
+    assert per >= 5
+    at = 0
+    for s in range(b.num_seqs):
+        x, y, k = b.cu_seqlens_q[s], b.cu_seqlens_q[s + 1], R.cache_rows(b, kc, ks, s)
+        plain = (int(b.seq_lens[s]) - int(y - x)) // 64          # chunks of context alone
+        top = np.stack([(R.f64(q[x:y, h]) @ k[:plain * 64, h // 8].T).reshape(-1, plain, 64).max(2)
+                        for h in range(8 * heads)], 2) * b.geom.softmax_scale * np.log2(np.e)
+        for i in range(tiles[s]):
+            for first in range(0, plain):
+                if first and (at + first) % per:
+                    continue                                     # (where a range begins)
+                last = min(plain, first + per - (at + first) % per)
+                best = max(best, float((top[tile * i:tile * i + tile, first:last] - top[tile * i:tile * i + tile, first:first + 1]).max()))
+            at += chunks[s]
+    return best
+
+
+@pytest.mark.parametrize("kv_dtype", [KV_BF16, KV_FP8_E4M3])
+@pytest.mark.parametrize("q_lens,tile", [([8, 5, 1], 8), ([16, 9, 12], 16), ([24, 20, 3], 24), ([30, 32, 17], 32), ([64, 40, 33], 32)])
+def test_scores_that_outgrow_their_reference(G, q_lens, tile, kv_dtype):
+    # A row's weights are taken relative to its range's first chunk until their sum reaches 2^60: the scores climb
+    # by 75 log2 units from one chunk to the next, four times, and start again.  Scores of up to 320 log2 units whose
+    # 64 products are off by 64 * 2^-24 * 320 = 1.2e-3 at most, twice that in the quotient: below the 2^-8 / 2 of
+    # the bound; in lse, 1.2e-3 log2 units against 1e-5 * 220.
+    lens = [8000, 7000, 9000]
+    b = make_batch(lens, q_lens, num_kv_heads=8, kv_dtype=kv_dtype)
+    q, k, v, sinks = logical_tensors(b)
+    u = np.where(np.arange(64) % 3 == 0, 1.0, -0.5).astype(np.float32)
+    t = np.concatenate([4.26 * (np.arange(n) // 64 % 5) for n in lens])
+    q = synth.f32_to_bf16_bits((0.1 * synth.bf16_bits_to_f32(q) + 3.0 * u).astype(np.float32))
+    k = synth.f32_to_bf16_bits((synth.bf16_bits_to_f32(k) + t[:, None, None] * u).astype(np.float32))
+    ks, vs = fp8_scales(k, v) if kv_dtype == KV_FP8_E4M3 else (None, None)
+    kc, vc = cpu_caches(b, k, v, ks, vs)
+    assert rises_inside_ranges(b, q, kc, ks, tile) > 65
+    rng = np.random.default_rng(1)
+    mask = R.tree_masks([R.random_parents(n, rng) for n in q_lens], 1)
+    for s in (sinks, None):
+        check(G, b, q, kc, vc, mask, s, ks, vs)
+
+
+@pytest.mark.parametrize("kv_dtype", [KV_BF16, KV_FP8_E4M3])
+@pytest.mark.parametrize("seq_lens,q_lens", [([1], [1]), ([8, 9, 70], [8, 1, 7]), ([300, 65, 16, 17], [16, 9, 16, 1]),
+                                             ([700, 64, 33], [33, 32, 17]), ([5000, 1100], [64, 63]), ([340, 256], [256, 200])])
+@pytest.mark.parametrize("window", [0, 1, 7, 64, 200])
+def test_random_trees_with_lse_and_without(G, seq_lens, q_lens, window, kv_dtype):
+    b, q, kc, vc, ks, vs, sinks = R.filled(seq_lens, q_lens, window=window, kv_dtype=kv_dtype, num_kv_heads=2)
+    rng = np.random.default_rng(window)
+    words = (max(q_lens) + 63) // 64
+    check(G, b, q, kc, vc, R.tree_masks([R.random_parents(n, rng, back=3) for n in q_lens], words), sinks, ks, vs)
+    ints = [int.from_bytes(rng.bytes(8 * words), "little") for _ in range(sum(q_lens))]   # any set, bits behind q_len
+    ints[0] = ints[-1] = 0
+    for s in (sinks, None):
+        check(G, b, q, kc, vc, R.masks_from_ints(ints, words), s, ks, vs)
+
+
+def test_large_scores_without_lse(G):
+    b, q, kc, vc, ks, vs, sinks = R.filled([900, 200], [6, 11], num_kv_heads=2)
+    q = synth.f32_to_bf16_bits(synth.bf16_bits_to_f32(q) * 40)   # scores of hundreds: near one-hot rows
+    rng = np.random.default_rng(4)
+    mask = R.tree_masks([R.random_parents(n, rng) for n in (6, 11)], 1)
+    for s in (sinks, np.full_like(sinks, 1e4), np.full_like(sinks, -np.inf)):
+        check(G, b, q, kc, vc, mask, s)
+
+
+@pytest.mark.parametrize("context", [60, 900])
+def test_what_a_row_does_not_see_cannot_reach_it_without_lse(G, context):
+    # drafted tokens with infinities and NaN in their keys and values; a whole span and a cut one
+    b, q, kc, vc, ks, vs, sinks = R.filled([context + 6], [6], num_kv_heads=1)
+    mask = R.masks_from_ints([0b1, 0b11, 0b101, 0b1011, 0b10101, 0b100001], 1)
+    ref, _, mag = reference(b, q, kc, vc, mask, sinks)
+    slots = b.all_slots(0)
+    for bad in (0x7FC0, 0x7F80, 0xFF80):
+        k2, v2 = kc.copy(), vc.copy()
+        k2.reshape(-1, 1, 64)[slots[context + 2], 0, 3] = bad     # token 2: rows 2 and 4 see it
+        v2.reshape(-1, 1, 64)[slots[context + 2], 0, 7] = bad
+        v2.reshape(-1, 1, 64)[slots[context + 5], 0, 9] = bad     # token 5: row 5 alone
+        out = ea.attn_tree(b.geom, G.bf16_dev(q), G.cache_dev(k2), G.cache_dev(v2), G.dev(b.block_table),
+                           G.dev(b.seq_lens), G.dev(b.cu_seqlens_q), G.dev(mask), max_q_len=6, max_kv_len=b.max_kv_len,
+                           sinks=G.dev(sinks))
+        got, tol = R.f64(G.bits_host(out)), 3.5 * R.BF16_HALF_STEP * mag + 1e-6
+        for i in (0, 1, 3):
+            assert (np.abs(got[i] - ref[i]) <= tol[i]).all()
+        rest = np.arange(64) != 9
+        assert (np.abs(got[5] - ref[5]) <= tol[5])[:, rest].all() and not np.isfinite(got[5][:, 9]).any()
+        assert not np.isfinite(got[2][:, 7]).all()
