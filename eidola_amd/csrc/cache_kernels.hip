@@ -342,6 +342,19 @@ __global__ __launch_bounds__(FP8 ? 256 : 512, 2) void score_stream_kernel(const 
   }
 }
 
+// First tile of sequence s in the workspace: behind those of the sequences before it.  -1 where the
+// workspace has no room for its tiles (a batch of more keys than its descriptor says): its rows are not
+// shared out then.  To be called by whole waves.
+__device__ __forceinline__ int first_ws_tile(const ScoreParams &p, const int s, const int len) {
+  int base = 0;
+  for (int s0 = 0; s0 < s; s0 += 64) {
+    const int i = s0 + (threadIdx.x & 63);
+    const int keys = i < s ? max(0, min(p.seq_lens[i], p.max_kv_len)) : 0;
+    base += __builtin_amdgcn_readlane(wave_inclusive_scan((keys + kScoreTile - 1) / kScoreTile), 63);
+  }
+  return base + (len + kScoreTile - 1) / kScoreTile <= p.ws_tiles ? base : -1;
+}
+
 // ---------------------------------------------------------------------------------------
 // Sequences of more rows: bound by the exponentials and products.  A wave holds 128 keys of one KV
 // head as operands and walks row pairs; one lane adds up one key's weights, so the sums need no
@@ -360,7 +373,7 @@ __global__ __launch_bounds__(kScoreWaves * 64, 3) void score_rows_kernel(const S
   const int lane = threadIdx.x & 63, i16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kvh = blockIdx.x % p.num_kv_heads;
-  const int tc = (blockIdx.x / p.num_kv_heads * kScoreWaves + wave) * kScoreKeys;
+  const int tc = blockIdx.x / p.num_kv_heads * kScoreTile + wave * kScoreKeys;
   const int s = blockIdx.y, part = blockIdx.z;
   const ScoreSeq v = score_seq(p, s);
   const int prefix = v.len - v.qlen;
@@ -376,7 +389,6 @@ __global__ __launch_bounds__(kScoreWaves * 64, 3) void score_rows_kernel(const S
   const int i0 = max(0, tc - prefix) & ~1;
   int i1 = v.qlen;
   if (p.window > 0) i1 = (int)min((long long)i1, (long long)key_end - 1 + p.window - prefix);
-  const int stride = 2 * p.parts;
   const int first = i0 + 2 * part;
 
   Frag8 kf[kPages][2], qf[2], qn[2];
@@ -438,6 +450,10 @@ __global__ __launch_bounds__(kScoreWaves * 64, 3) void score_rows_kernel(const S
     }
   };
   if (first < i1) fetch(first, qf, e);
+  const int ws_tile = p.parts > 1 && !few ? first_ws_tile(p, s, v.len) : -1;  // (while keys and rows arrive)
+  const bool shared = ws_tile >= 0;
+  if (part > 0 && !shared) return;
+  const int stride = shared ? 2 * p.parts : 2;
   for (int i = first; i < i1; i += stride) {
     fetch(i + stride, qn, en);
     const bool edge = prefix + i < key_end - 1 || (p.window > 0 && prefix + i + 1 - tc >= p.window) || i + 1 >= v.qlen;
@@ -459,7 +475,7 @@ __global__ __launch_bounds__(kScoreWaves * 64, 3) void score_rows_kernel(const S
     }
     const int j = tc + (4 * h + g) * kBlock + i16;
     if (j >= v.len) continue;
-    if (p.parts > 1 && !few) p.ws[(((size_t)part * p.num_seqs + s) * p.num_kv_heads + kvh) * p.tile_keys + j] = w;
+    if (shared) p.ws[(((size_t)part * p.num_kv_heads + kvh) * p.ws_tiles + ws_tile) * kScoreTile + j] = w;
     else add_score(p, s, kvh, j, prefix, w);
   }
 }
@@ -468,9 +484,11 @@ __global__ __launch_bounds__(kScoreWaves * 64, 3) void score_rows_kernel(const S
 __global__ __launch_bounds__(256) void score_join_kernel(const ScoreParams p) {
   const int s = blockIdx.z, kvh = blockIdx.y, j = blockIdx.x * 256 + threadIdx.x;
   const ScoreSeq v = score_seq(p, s);
-  if (v.qlen <= kScoreFewRows || j >= v.len || below_window(p, v.len - v.qlen, j + 1)) return;
-  const float *src = p.ws + ((size_t)s * p.num_kv_heads + kvh) * p.tile_keys + j;
-  const size_t step = (size_t)p.num_seqs * p.num_kv_heads * p.tile_keys;
+  if (v.qlen <= kScoreFewRows || (int)blockIdx.x * 256 >= v.len) return;
+  const int ws_tile = first_ws_tile(p, s, v.len);
+  if (ws_tile < 0 || j >= v.len || below_window(p, v.len - v.qlen, j + 1)) return;
+  const float *src = p.ws + ((size_t)kvh * p.ws_tiles + ws_tile) * kScoreTile + j;
+  const size_t step = (size_t)p.num_kv_heads * p.ws_tiles * kScoreTile;
   float w = 0.f;
   for (int part = 0; part < p.parts; part += 8) {  // eight loads under way, added in order
     float x[8];
@@ -790,7 +808,7 @@ hipError_t launch_score(const ScoreParams &p, const bool fp8, const bool many, h
     if (e != hipSuccess) return e;
   }
   if (many) {
-    const dim3 grid((unsigned)(p.tile_keys / (kScoreWaves * kScoreKeys)) * (unsigned)p.num_kv_heads, (unsigned)p.num_seqs,
+    const dim3 grid((unsigned)(p.tile_keys / kScoreTile) * (unsigned)p.num_kv_heads, (unsigned)p.num_seqs,
                     (unsigned)p.parts);
     if (fp8) score_rows_kernel<true><<<grid, kScoreWaves * 64, 0, st>>>(p);
     else score_rows_kernel<false><<<grid, kScoreWaves * 64, 0, st>>>(p);

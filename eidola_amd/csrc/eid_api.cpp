@@ -1227,7 +1227,7 @@ int32_t check_score_desc(const eid_attn_desc *d) {
 constexpr long long kScoreFill = 8;  // workgroups per CU that the parts aim at
 
 struct ScorePlan {
-  int32_t parts, tile_keys;
+  int32_t parts, tile_keys, ws_tiles;
   size_t ws_bytes;  // 0: none needed
 };
 
@@ -1235,21 +1235,27 @@ struct ScorePlan {
 // times as many of them as places the tiles that see few rows even out.  A part keeps at least eight
 // row pairs, so that loading the keys pays.  Aiming at 4 / 8 / 16 workgroups per CU: 2048 rows behind 4k
 // keys 118 / 110 / 123 us (one part 502), 512 rows 41 / 45 / 47 (134), 8 x 37 behind 8k 50 / 51 / 66.
+// The sequences' tiles stand in a line in the workspace, as many as the batch's keys can fill: parts are
+// few where tiles are many, so it stays below kScoreFill tiles per CU (4 MiB), whatever the batch.
 ScorePlan make_score_plan(const eid_attn_desc *d) {
   ScorePlan pl;
-  constexpr long long wg_keys = eid::kScoreWaves * eid::kScoreKeys;
+  constexpr long long wg_keys = eid::kScoreTile;
   const long long tiles = (d->max_kv_len + wg_keys - 1) / wg_keys;
   pl.tile_keys = (int32_t)std::min(tiles * wg_keys, 0x7fffffffLL / wg_keys * wg_keys);
   pl.parts = 1;
+  pl.ws_tiles = 0;
   pl.ws_bytes = 0;
   if (d->max_q_len <= eid::kScoreFewRows) return pl;
   const long long keys = d->sum_kv_len ? d->sum_kv_len : (long long)d->num_seqs * d->max_kv_len;
+  const long long line = std::min(keys / wg_keys + d->num_seqs, tiles * d->num_seqs);
   const long long wgs = (keys / wg_keys + d->num_seqs) * d->num_kv_heads;
   const long long by_fill = kScoreFill * eid::device_cus() / std::max(1LL, wgs);
   const long long by_rows = d->max_q_len / 16;
   pl.parts = (int32_t)std::max(1LL, std::min({by_fill, by_rows, (long long)eid::kScorePartsMax}));
-  if (pl.parts > 1)
-    pl.ws_bytes = (size_t)pl.parts * d->num_seqs * d->num_kv_heads * (size_t)pl.tile_keys * sizeof(float);
+  if (pl.parts > 1) {
+    pl.ws_tiles = (int32_t)line;  // (at most kScoreFill per CU)
+    pl.ws_bytes = (size_t)pl.parts * d->num_kv_heads * (size_t)(line * wg_keys) * sizeof(float);
+  }
   return pl;
 }
 
@@ -1373,6 +1379,7 @@ int32_t eid_kv_score(const eid_attn_desc *desc, const void *q, const float *lse,
   const long long fill = std::max(1, eid::device_cus() * 8 / std::max(8, desc->num_kv_heads) * (fp8 ? 2 : 1));
   p.ranges = (int32_t)std::max(1LL, std::min(fill, chunks));
   p.tile_keys = pl.tile_keys;
+  p.ws_tiles = pl.ws_tiles;
   p.ws = static_cast<float *>(workspace);
   p.num_seqs = desc->num_seqs;
   p.num_q_heads = desc->num_q_heads;

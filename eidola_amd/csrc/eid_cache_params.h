@@ -49,6 +49,7 @@ constexpr int kScoreFewRows = 2;   // q_len that the few-rows kernel takes
 constexpr int kScoreWaves = 4;     // of a workgroup of the rows kernel
 constexpr int kScoreKeys = 128;    // keys of a wave of the rows kernel
 constexpr int kScorePartsMax = 64;
+constexpr int kScoreTile = kScoreWaves * kScoreKeys;
 
 struct ScoreParams {
   const uint16_t *q;
@@ -63,7 +64,8 @@ struct ScoreParams {
   int32_t all_rows;   // the rows kernel takes sequences of few rows as well
   int32_t parts;      // the rows kernel's rows are shared out over so many workgroups
   int32_t tile_keys;  // max_kv_len, in whole workgroups' keys
-  float *ws;          // [parts][num_seqs][Hkv][tile_keys], parts > 1 only
+  int32_t ws_tiles;   // tiles of kScoreTile keys that the workspace has for a part and KV head
+  float *ws;          // [parts][Hkv][ws_tiles][kScoreTile], the sequences' tiles in a line; parts > 1 only
   float softmax_scale;
 };
 

@@ -362,8 +362,9 @@ int32_t eid_kv_score(const eid_attn_desc *desc, const void *q, const float *lse,
                      const int32_t *cu_seqlens_q, const int32_t *seq_lens, const float *k_scale,
                      float *scores, void *workspace, size_t workspace_bytes, void *hip_stream);
 
-/* Bytes of workspace eid_kv_score needs for desc; 0 when it needs none (workspace may then be
- * NULL), or for an invalid desc. */
+/* Bytes of workspace eid_kv_score needs for desc (4 MiB at most); 0 when it needs none (workspace may
+ * then be NULL), or for an invalid desc.  It need not grow with sum_kv_len: fewer keys are shared out
+ * over more workgroups.  A workspace kept for calls of different descriptors has the largest of theirs. */
 size_t eid_kv_score_workspace_bytes(const eid_attn_desc *desc);
 
 /*

@@ -28,3 +28,14 @@ def test_sequences_whose_rows_would_not_be_counted_in_32_bits_are_refused(over):
 def test_the_longest_sequences_are_planned():
     d = desc(num_seqs=1, max_kv_len=ROWS, max_blocks_per_seq=ROWS // 16)
     assert 0 < ea.attn_tree_workspace_bytes(d) <= 256 << 20
+
+
+def test_the_workspace_of_scores_does_not_grow_with_what_a_ragged_batch_could_hold():
+    # one long chunk beside many short sequences: the bound follows the keys, not sequences x longest
+    for heads, seqs, rows, longest in ((1, 256, 512, 131072), (1, 64, 2048, 131072), (8, 32, 512, 32768), (2, 1000, 300, 70000)):
+        geom = ea.AttnGeometry(num_q_heads=8 * heads, num_kv_heads=heads)
+        d = ea.make_desc(geom, num_seqs=seqs, num_q_tokens=rows + seqs - 1, max_q_len=rows, max_kv_len=longest,
+                         max_blocks_per_seq=(longest + 15) // 16, num_blocks=longest, sum_kv_len=longest + 100 * seqs)
+        assert ea.kv_score_workspace_bytes(d) <= 4 << 20
+        d.sum_kv_len = 0
+        assert ea.kv_score_workspace_bytes(d) <= 4 << 20
