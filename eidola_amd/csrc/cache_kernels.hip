@@ -99,18 +99,17 @@ __device__ __forceinline__ bool below_window(const ScoreParams &p, const int pre
 // vis(i, j) e^(c q.k_j - lse_i).
 //
 // Sequences of one or two rows: bound by reading K.  A wave takes 64 keys of one KV head; the
-// workgroup's waves take neighbouring heads of the same keys, so that whole pages are read at
-// once.  grid = (chunks, sequences, head groups).  For head counts that the stream below does not
-// take; at 8 heads 64 sequences of one row behind 8192 bf16 keys are 117 us, 4.9 TB/s.
+// workgroup's waves are the heads of the same keys, so that whole pages are read at once.  grid = (chunks,
+// sequences).  For 1, 2 and 4 heads, which the stream below does not take: at 4 heads 64 sequences of one
+// row behind 8192 bf16 keys are 58.5 us, 4.6 TB/s, fp8 37 us, 3.6 TB/s.
 // ---------------------------------------------------------------------------------------
 template <bool FP8>
-__global__ __launch_bounds__(512) void score_few_kernel(const ScoreParams p) {
+__global__ __launch_bounds__(256) void score_few_kernel(const ScoreParams p) {
   const int lane = threadIdx.x & 63, i16 = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int s = blockIdx.y, kvh = blockIdx.z * (blockDim.x >> 6) + wave;
+  const int s = blockIdx.y, kvh = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const ScoreSeq v = score_seq(p, s);
   const int tc = blockIdx.x * kChunk;
-  if (v.qlen < 1 || v.qlen > kScoreFewRows || tc >= v.len || kvh >= p.num_kv_heads) return;
+  if (v.qlen < 1 || v.qlen > kScoreFewRows || tc >= v.len) return;
   const int prefix = v.len - v.qlen;
   if (below_window(p, prefix, tc + kChunk)) return;
   const const_i32_ptr bt = as_constant(p.block_table + (size_t)s * p.max_blocks_per_seq);
@@ -799,11 +798,10 @@ hipError_t launch_score(const ScoreParams &p, const bool fp8, const bool many, h
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   } else if (few) {
-    const int waves = p.num_kv_heads < 8 ? p.num_kv_heads : 8;
-    const dim3 grid((unsigned)((p.max_kv_len + kChunk - 1) / kChunk), (unsigned)p.num_seqs,
-                    (unsigned)((p.num_kv_heads + waves - 1) / waves));
-    if (fp8) score_few_kernel<true><<<grid, waves * 64, 0, st>>>(p);
-    else score_few_kernel<false><<<grid, waves * 64, 0, st>>>(p);
+    const dim3 grid((unsigned)((p.max_kv_len + kChunk - 1) / kChunk), (unsigned)p.num_seqs);
+    const unsigned threads = (unsigned)p.num_kv_heads * 64;  // (1, 2 or 4 heads)
+    if (fp8) score_few_kernel<true><<<grid, threads, 0, st>>>(p);
+    else score_few_kernel<false><<<grid, threads, 0, st>>>(p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
