@@ -28,18 +28,20 @@ __device__ __forceinline__ ScoreSeq score_seq(const ScoreParams &p, const int s)
 
 // K operand of 16 keys (one page) of a head: lane (key i16, segment g) holds elements 8 g .. 8 g + 7
 // and 32 + 8 g .. 32 + 8 g + 7: a load instruction covers 64 consecutive bytes of each row.  An fp8
-// row is half as long, one load: elements 16 g .. 16 g + 15.  q is read in the same order.
+// row is half as long, one load: elements 16 g .. 16 g + 15.  q is read in the same order.  Through the
+// caches, as lines are picked up in halves: with the non-temporal hint 8 x 37 rows behind 8k bf16 keys take
+// 49.7 us (47), 4 heads of 64 fp8 sequences of one row 37 (34); 4 heads of bf16 58.5 on both sides.
 template <bool FP8>
 __device__ __forceinline__ void load_k(const uint8_t *base, const uint32_t row_bytes, Frag8 (&kf)[2]) {
   const int lane = threadIdx.x & 63, i16 = lane & 15, g = lane >> 4;
   const uint8_t *src = base + (uint32_t)i16 * row_bytes + g * 16;
   if constexpr (FP8) {
-    const u32x4 r = __builtin_nontemporal_load((const u32x4 *)src);
+    const u32x4 r = *(const u32x4 *)src;
     fp8x8_to_bf16x8(r[0], r[1], kf[0].w);
     fp8x8_to_bf16x8(r[2], r[3], kf[1].w);
   } else {
-    kf[0].u = __builtin_nontemporal_load((const u32x4 *)src);
-    kf[1].u = __builtin_nontemporal_load((const u32x4 *)(src + 64));
+    kf[0].u = *(const u32x4 *)src;
+    kf[1].u = *(const u32x4 *)(src + 64);
   }
 }
 
@@ -101,7 +103,7 @@ __device__ __forceinline__ bool below_window(const ScoreParams &p, const int pre
 // Sequences of one or two rows: bound by reading K.  A wave takes 64 keys of one KV head; the
 // workgroup's waves are the heads of the same keys, so that whole pages are read at once.  grid = (chunks,
 // sequences).  For 1, 2 and 4 heads, which the stream below does not take: at 4 heads 64 sequences of one
-// row behind 8192 bf16 keys are 58.5 us, 4.6 TB/s, fp8 37 us, 3.6 TB/s.
+// row behind 8192 bf16 keys are 58.5 us, 4.6 TB/s, fp8 34 us, 3.9 TB/s.
 // ---------------------------------------------------------------------------------------
 template <bool FP8>
 __global__ __launch_bounds__(256) void score_few_kernel(const ScoreParams p) {
@@ -364,8 +366,8 @@ __device__ __forceinline__ int first_ws_tile(const ScoreParams &p, const int s, 
 //
 // A stage is one 16-key page: its two matrix instructions are issued a stage ahead of its four
 // (multiply-add, exponential, add) per lane, which is what bounds the kernel: 2048 rows of one sequence
-// behind 4k keys, 8 KV heads, 0.4 G weights, 106 us with the join, 3.8 weights per ns (51 GFLOP of
-// products, 0.48 PFLOP/s); 8 x 37 rows behind 8k fp8 keys 34 us.
+// behind 4k keys, 8 KV heads, 0.4 G weights, 102 us with the join, 4.0 weights per ns (51 GFLOP of
+// products, 0.51 PFLOP/s); 8 x 37 rows behind 8k fp8 keys 33 us.
 // ---------------------------------------------------------------------------------------
 template <bool FP8>
 __global__ __launch_bounds__(kScoreWaves * 64, 3) void score_rows_kernel(const ScoreParams p) {
