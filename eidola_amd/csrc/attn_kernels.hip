@@ -34,14 +34,6 @@ constexpr int kWaveLdsBytes = 4 * kVPageBytes;  // 64 tokens
 
 __device__ __forceinline__ u32x4 ldg128(const uint8_t *p) { return *(const u32x4 *)p; }
 
-// Block tables are read-only for the lifetime of a launch.  Reading them through the
-// constant address space keeps wave-uniform page-id loads on the scalar unit whatever else
-// the kernel stores, so they never share a wait counter with the K/V vector loads.
-typedef const __attribute__((address_space(4))) int32_t *const_i32_ptr;
-__device__ __forceinline__ const_i32_ptr as_constant(const int32_t *p) {
-  return (const_i32_ptr)(uintptr_t)p;
-}
-
 // Row bookkeeping of a wave's NT 16-row tiles.  Row r = 16 nt + (lane % 16) belongs to query
 // token tq0 + r / 8, so one per-lane value and four wave-uniform ones describe every tile;
 // the bounds are only materialised on chunks that need masking.

@@ -9,10 +9,6 @@ namespace eid {
 
 namespace {
 
-typedef const __attribute__((address_space(4))) int32_t *const_i32_ptr;
-__device__ __forceinline__ const_i32_ptr as_constant(const int32_t *p) { return (const_i32_ptr)(uintptr_t)p; }
-__device__ __forceinline__ int clamp_id(const int id, const int last) { return min(max(id, 0), last); }
-
 struct ScoreSeq {
   int row0, qlen, len;
 };
@@ -148,13 +144,11 @@ __global__ __launch_bounds__(256) void score_few_kernel(const ScoreParams p) {
 // window reaches) stand in a line, cut into equal ranges, and a wave walks a range for one head (two of
 // an fp8 cache, whose rows are half a line) with two chunks under way through direct global -> LDS
 // loads, whole 128-byte rows at a time, without barriers: its tiles are its own.
-// 64 sequences of one row behind 8192 bf16 keys, 8 KV heads: 102 us, 5.6 TB/s (117 us from the kernel
+// 64 sequences of one row behind 8192 bf16 keys, 8 KV heads: 102 us, 5.6 TB/s (117 us in the form of the kernel
 // above, which picks every row up in halves; 116 us here without the non-temporal hint); fp8 63 us
 // (72).  A window of 128 behind 128 x 4096 keys: 8.4 us (47: most workgroups of a grid over all
 // chunks find nothing to do).  One sequence of 500: 4.1 us (4.7); fp8 8 x 8192 alone loses, 13.1 (12.3).
 // ---------------------------------------------------------------------------------------
-typedef __attribute__((address_space(1))) const void gptr_t;
-typedef __attribute__((address_space(3))) void lptr_t;
 constexpr int kStreamTile = kChunk * 128;      // K rows of a chunk
 
 // One cursor of a stream: a chunk of a sequence.

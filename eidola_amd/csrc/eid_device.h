@@ -24,6 +24,21 @@ union Frag8 {  // 8 bf16 = one MFMA 16x16x32 / 32x32x16 operand
   uint32_t w[4];
 };
 
+// Block tables are read-only for the lifetime of a launch.  Reading them through the
+// constant address space keeps wave-uniform page-id loads on the scalar unit whatever else
+// the kernel stores, so they never share a wait counter with the K/V vector loads.
+typedef const __attribute__((address_space(4))) int32_t *const_i32_ptr;
+__device__ __forceinline__ const_i32_ptr as_constant(const int32_t *p) {
+  return (const_i32_ptr)(uintptr_t)p;
+}
+
+// A page id of a block table, held inside the cache whatever stands there.
+__device__ __forceinline__ int clamp_id(const int id, const int last) { return min(max(id, 0), last); }
+
+// operands of the direct global -> LDS loads
+typedef __attribute__((address_space(1))) const void gptr_t;
+typedef __attribute__((address_space(3))) void lptr_t;
+
 __device__ __forceinline__ f32x4 mfma16x32(const Frag8 &a, const Frag8 &b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, b.v, c, 0, 0, 0);
 }

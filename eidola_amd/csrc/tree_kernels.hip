@@ -8,10 +8,6 @@ namespace eid {
 
 namespace {
 
-typedef const __attribute__((address_space(4))) int32_t *const_i32_ptr;
-__device__ __forceinline__ const_i32_ptr as_constant(const int32_t *p) { return (const_i32_ptr)(uintptr_t)p; }
-__device__ __forceinline__ int clamp_id(const int id, const int last) { return min(max(id, 0), last); }
-
 constexpr float kLazyLog2 = 8.0f;  // a row's reference moves when a score outgrows it by this
 constexpr float kRowSumGuard = 1152921504606846976.0f;  // 2^60
 
@@ -133,8 +129,6 @@ __device__ __forceinline__ uint64_t chunk_bits(const uint64_t *mask, const int l
 // matrix units 36 % busy; 8 x 32 behind 16k fp8 88 us.  Short calls are two launches long: 32 x 24 in a window of 128, 19 MB, 15 us
 // in one launch.
 // ---------------------------------------------------------------------------------------
-typedef __attribute__((address_space(1))) const void gptr_t;
-typedef __attribute__((address_space(3))) void lptr_t;
 constexpr int kTileBytes = kChunk * 128;
 
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
