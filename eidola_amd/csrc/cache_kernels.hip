@@ -703,10 +703,12 @@ __global__ __launch_bounds__(kSelThreads) void select_kernel(const SelectParams 
 // column of the sequence (one KV head, or eight where all heads keep the same rows) in one tensor
 // of one layer and moves it in steps; a step's rows are all in registers before its first
 // store, and later steps read only rows behind everything that this one overwrites.  What bounds
-// long moves is the caches' layout: a head's row is 128 bytes of a token's 1 KiB and every head keeps
-// other tokens, so memory sees lone lines (8 sequences cut from 16k to 4k: 40 us for 137 MB; two
-// workgroups per column, 64 bytes of a row each: 49 us).  Neighbouring heads on one XCD: 45.5 us the call
-// against 47.
+// long moves is that order: a column's loads, drain and stores follow one another four times over with
+// nothing in flight during the stores, on as many CUs as there are columns (8 sequences cut from 16k to 4k:
+// 39 us in the kernel for 137 MB, 3.5 TB/s, 128 workgroups for K and V and 64 for scores).  A head's rows are lone
+// lines of 128 bytes of a token's 1 KiB, which alone do not cost that much: a kernel that only loads one head's
+// rows runs at 5.4 TB/s and more; two workgroups per column, 64 bytes of a row each, 49 us.  Neighbouring
+// heads on one XCD: 45.5 us the call against 47.
 // ---------------------------------------------------------------------------------------
 __device__ __forceinline__ void step_loaded() {
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's rows are in registers

@@ -122,12 +122,21 @@ __device__ __forceinline__ uint64_t chunk_bits(const uint64_t *mask, const int l
 // (0 x inf would be NaN in rows that do not see the key); if there were any, their terms are added
 // afterwards, row by row, where they are seen.
 //
-// What bounds it, 8 KV heads.  Up to 16 tokens the stream of K and V: 16 trees of up to 16 tokens behind
-// up to 8k keys, 199 MB, 54 us, 3.7 TB/s.  From about 24 tokens on instructions: a 64-key chunk of a
-// 16-row tile takes 16 exponentials, 16 multiply-adds and 8 packings per lane and 18 matrix instructions,
-// which overlap only in part: 4 x 64 behind 32k, 137 GFLOP, 174 us, 0.79 PFLOP/s, vector units 59 % and
-// matrix units 36 % busy; 8 x 32 behind 16k fp8 88 us.  Short calls are two launches long: 32 x 24 in a window of 128, 19 MB, 15 us
-// in one launch.
+// Roundings: a row's weights enter the value product as bf16 (the matrix unit takes both operands in one type,
+// and V is bf16; fp16 would hold neither V's range nor weights of 2^60; the weights' low halves in a
+// second product would be 8 more matrix instructions per chunk and 16-row tile beside 18, and their
+// subtractions and packings).  Against 64 bits an answer is off by 0.0022 - 0.0024 of its size, of which
+// 0.0017 are the rounding of the answer itself.  Sums and statistics are fp32.
+//
+// What bounds it, 8 KV heads.  4 x 64 behind 32k, 137 GFLOP, 176 us, 0.78 PFLOP/s: a 64-key chunk of a
+// 16-row tile takes 16 exponentials, 16 multiply-adds and 8 packings per lane and 18 matrix instructions;
+// vector units are 60 % and matrix units 36 % busy, which mostly add up instead of overlapping.  Small trees:
+// no unit, but latency and what every piece repeats (lengths, pages, q and masks one after the other, a drain,
+// the join): 16 trees of up to 16 tokens behind up to 8k keys, 199 MB, 54 us, 3.7 TB/s, matrix units 14 %
+// busy, vector units 36 %.  8 x 17 .. 32 tokens behind 16k fp8, 86 us: 23 % of its tiles' rows are nobody's (the
+// longest tree chooses the tile for all), and one chunk is requested ahead; vector units 43 % busy, matrix units
+// 23 %.  32 x 24 in a window of 128, 19 MB, 15 us: three chunks, the third requested when the first is done.
+// 1 x 8 behind 500, 11.5 us: eight chunks one after the other in one workgroup per head.
 // ---------------------------------------------------------------------------------------
 constexpr int kTileBytes = kChunk * 128;
 
